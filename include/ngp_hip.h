@@ -47,7 +47,10 @@ enum { NGP_LENS_PERSPECTIVE = 0, NGP_LENS_OPENCV = 1, NGP_LENS_FTHETA = 2, NGP_L
 enum { NGP_IMAGE_NONE = 0, NGP_IMAGE_BYTE = 1, NGP_IMAGE_HALF = 2, NGP_IMAGE_FLOAT = 3 };
 
 /* ENerfActivation, common.h (None/ReLU/Logistic/Exponential) */
-enum { NGP_ACT_NONE = 0, NGP_ACT_RELU = 1, NGP_ACT_LOGISTIC = 2, NGP_ACT_EXPONENTIAL = 3 };
+enum { NGP_ACT_NONE = 0, NGP_ACT_RELU = 1, NGP_ACT_LOGISTIC = 2, NGP_ACT_EXPONENTIAL = 3,
+       NGP_ACT_SILU = 4 /* z * logistic(z); 4 and 5: ngp_linear_* and ngp_gated_* only */, NGP_ACT_GELU = 5 /* z * Phi(z), Phi the normal distribution function (erf, no approximation) */ };
+/* element types of ngp_linear_*, ngp_gated_* (HALF, BFLOAT16) and ngp_gradient (all three) */
+enum { NGP_TYPE_HALF = 0, NGP_TYPE_BFLOAT16 = 1, NGP_TYPE_FLOAT = 2 };
 
 /* ELossType, common.h */
 enum { NGP_LOSS_L2 = 0, NGP_LOSS_L1 = 1, NGP_LOSS_MAPE = 2, NGP_LOSS_SMAPE = 3, NGP_LOSS_HUBER = 4,
@@ -275,6 +278,52 @@ int ngp_encmlp_training_step_external(ngp_encmlp*, void* stream, const float* in
 int ngp_encmlp_optimizer_step(ngp_encmlp*, void* stream, float loss_scale);    /* Trainer::optimizer_step */
 float ngp_encmlp_learning_rate(const ngp_encmlp*);
 uint32_t ngp_encmlp_step(const ngp_encmlp*);
+
+/* ------------------------------------------------------------------ dense layers --------- */
+/* Layers of any width beside the 64-wide fused networks above (the reference reaches for tiny-cuda-nn's layer-by-layer CutlassMLP there): one layer per call, activations in
+ * global memory.  m samples, n outputs, k inputs; matrices are row-major with `*_stride` elements from row to row, weights [outputs][inputs] like the parameters above; any size
+ * from 0, any stride >= the row's length, any address aligned to its elements.  `type` (NGP_TYPE_HALF | NGP_TYPE_BFLOAT16) is that of every matrix and vector of the call; products,
+ * sums and activations are computed in 32 bits and rounded once into each output.  Outputs must not overlap each other, an input or the workspace (columns of one wider matrix
+ * may be shared out among them); y may be the residual itself.  `workspace` (16-byte aligned, at least ngp_*_workspace_size bytes; a call with a size of 0 takes NULL) is scratch:
+ * calls that can run at the same time -- on two streams, in two graphs -- need one each.  Nothing is kept from call to call, nothing is allocated: calls can be captured. */
+
+/* Z = X W^T + bias;  Y = act(Z) + residual.  bias (n), residual (m x n), pre (m x n: receives Z, for ngp_linear_backward): NULL = none. */
+int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                       const void* bias, const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride,
+                       void* workspace, uint64_t workspace_size);
+/* G = dY * act'(Z);  dX = G W;  dW = G^T X;  dbias = column sums of G (each NULL = not wanted; overwritten).  The residual's gradient is dY itself.  `pre` is not read with
+ * NGP_ACT_NONE.  G is rounded to `type` between the two products. */
+int ngp_linear_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+                        const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias,
+                        void* workspace, uint64_t workspace_size);
+uint64_t ngp_linear_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward);
+
+/* Gated projections of a feed-forward block: Zg = X Wg^T + bias_gate, Zu = X Wu^T + bias_up, Y = act(Zg) * Zu in one kernel (the block's third matrix is an ngp_linear_forward of
+ * Y, with the block's input as residual).  gate_pre, up_pre: receive Zg, Zu, for ngp_gated_backward (each NULL = not kept). */
+int ngp_gated_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up,
+                      uint64_t w_stride, const void* bias_gate, const void* bias_up, void* y, uint64_t y_stride, void* gate_pre, void* up_pre, uint64_t pre_stride,
+                      void* workspace, uint64_t workspace_size);
+/* Gg = dY * Zu * act'(Zg), Gu = dY * act(Zg);  dX = Gg Wg + Gu Wu;  dWg = Gg^T X, dWu = Gu^T X;  dbias_* = column sums.  dx, {dw_gate, dw_up} together, each dbias: NULL = not wanted. */
+int ngp_gated_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up,
+                       uint64_t w_stride, const void* gate_pre, const void* up_pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride,
+                       void* dw_gate, void* dw_up, uint64_t dw_stride, void* dbias_gate, void* dbias_up, void* workspace, uint64_t workspace_size);
+uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward);
+
+/* ------------------------------------------------------------------ gradient clipping ---- */
+/* Between the gradients (ngp_model_training_step, ngp_encmlp_training_step, ngp_linear_backward ...) and the optimizer step, over tensors of any number, size and type.  Gradients
+ * carry the loss scale; `norm` (device, one float) receives the norm of what the optimizer sees, sqrt(sum of g^2) / loss_scale, summed in 64 bits in a fixed order. */
+typedef struct ngp_gradient {
+	const void* grad;    /* `size` elements, aligned to their type */
+	void* clipped;       /* where the clipped gradient goes: grad itself, another buffer, or NULL (counted in the norm, not clipped); not read by ngp_gradient_norm */
+	uint64_t size;
+	int32_t type;        /* NGP_TYPE_* */
+	int32_t reserved;
+} ngp_gradient;
+int ngp_gradient_norm(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float* norm, void* workspace, uint64_t workspace_size);
+/* clipped = grad * min(1, max_norm / norm), rounded once; in place nothing is written where the factor is 1.  A norm that is not finite is reported and leaves the gradients as they
+ * are (the caller skips the step).  What is written must not overlap another tensor.  The table is read before the call returns; `workspace` as for the dense layers. */
+int ngp_clip_gradients(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float max_norm, float* norm, void* workspace, uint64_t workspace_size);
+uint64_t ngp_gradient_workspace_size(void);
 
 /* ------------------------------------------------------------------ image trainer -------- */
 /* Testbed::m_image + train_image (testbed_image.cu:231-302) and compute_image_mse (:490-547): the image lives on the device as RGBA

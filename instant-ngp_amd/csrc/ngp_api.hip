@@ -2638,3 +2638,180 @@ extern "C" int ngp_nerf_set_debug_flags(ngp_nerf* t, int on, uint32_t flags, uin
 	t->model->dbg = t->dbg;
 	return 0;
 }
+
+// ------------------------------------------------------------------------------------------------
+// dense layers (ngp_linear_*, ngp_gated_*) and gradient clipping: argument checks and dispatch; kernels in dense_kernels.hip / clip_kernels.hip
+// ------------------------------------------------------------------------------------------------
+// Where a caller's buffer lies: rows x width elements of `size` bytes, `stride` elements from row to row.
+struct DenseBuffer { const void* p; uint64_t rows, width, stride; const char* name; bool written; uint32_t size = 2; };
+// Two buffers meet where their byte ranges do, unless they are different columns of one wider matrix (same stride).
+static bool dense_overlap(const DenseBuffer& a, const DenseBuffer& b) {
+	if (!a.p || !b.p || !a.rows || !b.rows || !a.width || !b.width) return false;
+	const uint64_t pa = (uint64_t)a.p, pb = (uint64_t)b.p, ea = pa + ((a.rows - 1) * a.stride + a.width) * a.size, eb = pb + ((b.rows - 1) * b.stride + b.width) * b.size;
+	if (pa >= eb || pb >= ea) return false;
+	if (a.stride == b.stride && a.size == b.size && a.rows > 1 && b.rows > 1) {
+		const uint64_t step = a.stride * a.size, d = pb >= pa ? (pb - pa) % step : (step - (pa - pb) % step) % step;
+		if (d >= a.width * a.size && d + b.width * b.size <= step) return false;
+	}
+	return true;
+}
+// One process drives one GPU; with more devices in sight a buffer or a stream of another one is refused here (a kernel would fault on it).
+static int dense_check_device(const char* what, hipStream_t s, const DenseBuffer* b, size_t n) {
+	static int devices = 0;
+	if (devices <= 0 && hipGetDeviceCount(&devices) != hipSuccess) { devices = 0; (void)hipGetLastError(); }
+	REQUIRE(devices > 0, "no HIP device visible: libngp_hip has no CPU fallback");
+	if (devices == 1) return 0;
+	int dev = 0; HIPCHK(hipGetDevice(&dev));
+	if (s) {
+		hipDevice_t on = dev;
+		REQUIRE(hipStreamGetDevice(s, &on) != hipSuccess || on == dev, std::string(what) + ": the stream belongs to another device than the current one");
+	}
+	for (size_t i = 0; i < n; ++i) {
+		if (!b[i].p || !b[i].rows || !b[i].width) continue;
+		hipPointerAttribute_t at;
+		if (hipPointerGetAttributes(&at, b[i].p) != hipSuccess) { (void)hipGetLastError(); return fail(std::string(what) + ": " + b[i].name + " is not a device pointer"); }
+		REQUIRE(at.type != hipMemoryTypeDevice || at.device == dev, std::string(what) + ": " + b[i].name + " lies on another device than the current one");
+	}
+	return 0;
+}
+static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t n, uint32_t k, hipStream_t s, const DenseBuffer* b, size_t nb, const void* may_share_a, const void* may_share_b) {
+	const std::string w = what;
+	REQUIRE(type == NGP_TYPE_HALF || type == NGP_TYPE_BFLOAT16, w + ": type must be NGP_TYPE_HALF or NGP_TYPE_BFLOAT16");
+	REQUIRE(act >= NGP_ACT_NONE && act <= NGP_ACT_GELU, w + ": unknown activation");
+	REQUIRE(m <= 0x7fffffffu && n <= (1u << 24) && k <= (1u << 24), w + ": at most 2^31 - 1 samples and 2^24 inputs / outputs");
+	REQUIRE((((uint64_t)m + 15) / 16) * (((uint64_t)n + 15) / 16) < (1ull << 31) && (((uint64_t)m + 15) / 16) * (((uint64_t)k + 15) / 16) < (1ull << 31), w + ": more output tiles than one launch takes; pass the samples in pieces");
+	for (size_t i = 0; i < nb; ++i) {
+		if (!b[i].p) continue;
+		REQUIRE(b[i].stride >= b[i].width, w + ": stride of " + b[i].name + " too small");
+		REQUIRE(b[i].stride < (1ull << 40), w + ": stride of " + b[i].name + " too large");
+		REQUIRE(((uintptr_t)b[i].p & 1) == 0, w + ": " + b[i].name + " is not aligned to its elements");
+	}
+	for (size_t i = 0; i < nb; ++i) if (b[i].written)
+		for (size_t j = 0; j < nb; ++j) {
+			if (j == i || (j < i && b[j].written)) continue;
+			if (b[i].p == may_share_a && b[j].p == may_share_b && b[i].p == b[j].p && b[i].p && b[i].stride == b[j].stride) continue;
+			REQUIRE(!dense_overlap(b[i], b[j]), w + ": " + b[i].name + " overlaps " + b[j].name);
+		}
+	return dense_check_device(what, s, b, nb);
+}
+extern "C" uint64_t ngp_linear_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, false).bytes : 0; }
+extern "C" uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, true).bytes : 0; }
+extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, const void* bias,
+		const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w, n, k, w_stride, "w", false}, {bias, 1, n, n, "bias", false}, {residual, m, n, residual_stride, "residual", false},
+		{y, m, n, y_stride, "y", true}, {pre, m, n, pre_stride, "pre", true}};
+	REQUIRE((x && w) || !m || !n || !k, "ngp_linear_forward: null argument");
+	REQUIRE(y || !m || !n, "ngp_linear_forward: null argument");
+	if (int rc = dense_check("ngp_linear_forward", type, activation, m, n, k, (hipStream_t)stream, b, 6, y, residual)) return rc;
+	DenseArgs d{};
+	d.gated = false; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w; d.w_stride = w_stride; d.bias[0] = bias;
+	d.residual = residual; d.residual_stride = residual_stride; d.y = y; d.y_stride = y_stride; d.pre[0] = pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;
+	if (type == NGP_TYPE_HALF) launch_dense_forward_half((hipStream_t)stream, d); else launch_dense_forward_bf16((hipStream_t)stream, d);
+	HIPCHK(hipGetLastError());
+	return 0;
+}
+extern "C" int ngp_gated_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up, uint64_t w_stride,
+		const void* bias_gate, const void* bias_up, void* y, uint64_t y_stride, void* gate_pre, void* up_pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w_gate, n, k, w_stride, "w_gate", false}, {w_up, n, k, w_stride, "w_up", false}, {bias_gate, 1, n, n, "bias_gate", false},
+		{bias_up, 1, n, n, "bias_up", false}, {y, m, n, y_stride, "y", true}, {gate_pre, m, n, pre_stride, "gate_pre", true}, {up_pre, m, n, pre_stride, "up_pre", true}};
+	REQUIRE((x && w_gate && w_up) || !m || !n || !k, "ngp_gated_forward: null argument");
+	REQUIRE(y || !m || !n, "ngp_gated_forward: null argument");
+	if (int rc = dense_check("ngp_gated_forward", type, activation, m, n, k, (hipStream_t)stream, b, 8, nullptr, nullptr)) return rc;
+	DenseArgs d{};
+	d.gated = true; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w_gate; d.w[1] = w_up; d.w_stride = w_stride; d.bias[0] = bias_gate; d.bias[1] = bias_up;
+	d.y = y; d.y_stride = y_stride; d.pre[0] = gate_pre; d.pre[1] = up_pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;
+	if (type == NGP_TYPE_HALF) launch_dense_forward_half((hipStream_t)stream, d); else launch_dense_forward_bf16((hipStream_t)stream, d);
+	HIPCHK(hipGetLastError());
+	return 0;
+}
+extern "C" int ngp_linear_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
+		const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias, void* workspace, uint64_t workspace_size) {
+	if (activation == NGP_ACT_NONE) pre = nullptr; // not read
+	const uint64_t need = dense_plan(m, n, k, false).bytes;
+	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w, n, k, w_stride, "w", false}, {pre, m, n, pre_stride, "pre", false}, {dy, m, n, dy_stride, "dy", false},
+		{dx, m, k, dx_stride, "dx", true}, {dw, n, k, dw_stride, "dw", true}, {dbias, 1, n, n, "dbias", true}, {workspace, 1, need, need, "workspace", true, 1}};
+	REQUIRE(dy || !m || !n, "ngp_linear_backward: null argument");
+	REQUIRE(pre || activation == NGP_ACT_NONE || !m || !n, "ngp_linear_backward: the forward pass's pre-activations are missing");
+	REQUIRE(!dx || w || !m || !n || !k, "ngp_linear_backward: dx without w");
+	REQUIRE(!dw || x || !m || !n || !k, "ngp_linear_backward: dw without x");
+	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_linear_backward: workspace smaller than ngp_linear_workspace_size() or not 16-byte aligned");
+	if (int rc = dense_check("ngp_linear_backward", type, activation, m, n, k, (hipStream_t)stream, b, 8, nullptr, nullptr)) return rc;
+	DenseArgs d{};
+	d.gated = false; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w; d.w_stride = w_stride; d.pre[0] = (void*)pre; d.pre_stride = pre_stride;
+	d.dy = dy; d.dy_stride = dy_stride; d.dx = dx; d.dx_stride = dx_stride; d.dw[0] = dw; d.dw_stride = dw_stride; d.dbias[0] = dbias; d.workspace = workspace; d.workspace_size = workspace_size;
+	if (type == NGP_TYPE_HALF) launch_dense_backward_half((hipStream_t)stream, d); else launch_dense_backward_bf16((hipStream_t)stream, d);
+	HIPCHK(hipGetLastError());
+	return 0;
+}
+extern "C" int ngp_gated_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up, uint64_t w_stride,
+		const void* gate_pre, const void* up_pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw_gate, void* dw_up, uint64_t dw_stride,
+		void* dbias_gate, void* dbias_up, void* workspace, uint64_t workspace_size) {
+	const uint64_t need = dense_plan(m, n, k, true).bytes;
+	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w_gate, n, k, w_stride, "w_gate", false}, {w_up, n, k, w_stride, "w_up", false}, {gate_pre, m, n, pre_stride, "gate_pre", false},
+		{up_pre, m, n, pre_stride, "up_pre", false}, {dy, m, n, dy_stride, "dy", false}, {dx, m, k, dx_stride, "dx", true}, {dw_gate, n, k, dw_stride, "dw_gate", true}, {dw_up, n, k, dw_stride, "dw_up", true},
+		{dbias_gate, 1, n, n, "dbias_gate", true}, {dbias_up, 1, n, n, "dbias_up", true}, {workspace, 1, need, need, "workspace", true, 1}};
+	REQUIRE((dy && gate_pre && up_pre) || !m || !n, "ngp_gated_backward: null argument");
+	REQUIRE(!dx || (w_gate && w_up) || !m || !n || !k, "ngp_gated_backward: dx without the weights");
+	REQUIRE((dw_gate != nullptr) == (dw_up != nullptr), "ngp_gated_backward: dw_gate and dw_up come together");
+	REQUIRE(!dw_gate || x || !m || !n || !k, "ngp_gated_backward: dw without x");
+	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_gated_backward: workspace smaller than ngp_gated_workspace_size() or not 16-byte aligned");
+	if (int rc = dense_check("ngp_gated_backward", type, activation, m, n, k, (hipStream_t)stream, b, 12, nullptr, nullptr)) return rc;
+	DenseArgs d{};
+	d.gated = true; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w_gate; d.w[1] = w_up; d.w_stride = w_stride; d.pre[0] = (void*)gate_pre; d.pre[1] = (void*)up_pre;
+	d.pre_stride = pre_stride; d.dy = dy; d.dy_stride = dy_stride; d.dx = dx; d.dx_stride = dx_stride; d.dw[0] = dw_gate; d.dw[1] = dw_up; d.dw_stride = dw_stride; d.dbias[0] = dbias_gate; d.dbias[1] = dbias_up;
+	d.workspace = workspace; d.workspace_size = workspace_size;
+	if (type == NGP_TYPE_HALF) launch_dense_backward_half((hipStream_t)stream, d); else launch_dense_backward_bf16((hipStream_t)stream, d);
+	HIPCHK(hipGetLastError());
+	return 0;
+}
+
+extern "C" uint64_t ngp_gradient_workspace_size(void) { return CLIP_SLOTS * sizeof(double); }
+static int gradient_norm(const char* what, void* stream, uint32_t n, const ngp_gradient* t, float loss_scale, bool clip, float max_norm, float* norm, void* workspace, uint64_t workspace_size) try {
+	const std::string w = what;
+	REQUIRE(t || !n, w + ": null argument");
+	REQUIRE(norm, w + ": null argument");
+	REQUIRE(((uintptr_t)norm & 3) == 0, w + ": norm is not aligned to its element");
+	REQUIRE(loss_scale > 0.f && std::isfinite(loss_scale), w + ": loss_scale must be positive and finite");
+	REQUIRE(!clip || max_norm >= 0.f, w + ": max_norm must not be negative or NaN");
+	REQUIRE(workspace && workspace_size >= ngp_gradient_workspace_size() && ((uintptr_t)workspace & 15) == 0, w + ": workspace smaller than ngp_gradient_workspace_size() or not 16-byte aligned");
+	// every written range against every other one: sorted by address, only neighbours can meet (a tensor clipped in place is one range)
+	struct Span { uint64_t begin, end; bool written; };
+	thread_local std::vector<Span> spans;
+	thread_local std::vector<DenseBuffer> buffers;
+	spans.clear(); buffers.clear();
+	spans.push_back({(uint64_t)workspace, (uint64_t)workspace + ngp_gradient_workspace_size(), true});
+	spans.push_back({(uint64_t)norm, (uint64_t)norm + 4, true});
+	bool sorted = true;
+	for (uint32_t i = 0; i < n; ++i) {
+		REQUIRE(t[i].type == NGP_TYPE_HALF || t[i].type == NGP_TYPE_BFLOAT16 || t[i].type == NGP_TYPE_FLOAT, w + ": type must be NGP_TYPE_HALF, NGP_TYPE_BFLOAT16 or NGP_TYPE_FLOAT");
+		if (!t[i].size) continue;
+		const uint32_t bytes = t[i].type == NGP_TYPE_FLOAT ? 4 : 2;
+		REQUIRE(t[i].grad, w + ": null gradient");
+		REQUIRE(t[i].size <= (1ull << 43), w + ": a tensor of more than 2^43 elements");
+		REQUIRE((((uintptr_t)t[i].grad | (uintptr_t)t[i].clipped) & (bytes - 1)) == 0, w + ": a tensor is not aligned to its elements");
+		const bool in_place = clip && t[i].clipped == t[i].grad;
+		const uint64_t a = (uint64_t)t[i].grad, b = (uint64_t)t[i].clipped, len = t[i].size * bytes;
+		spans.push_back({a, a + len, in_place});
+		if (clip && b && !in_place) spans.push_back({b, b + len, true});
+		buffers.push_back({t[i].grad, 1, t[i].size, t[i].size, "a gradient", false, bytes});
+		if (clip && b && !in_place) buffers.push_back({t[i].clipped, 1, t[i].size, t[i].size, "a clipped gradient", true, bytes});
+	}
+	for (size_t i = 1; i < spans.size() && sorted; ++i) sorted = spans[i - 1].begin <= spans[i].begin;
+	if (!sorted) std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+	uint64_t end_any = 0, end_written = 0;
+	for (const Span& s : spans) {
+		REQUIRE(s.begin >= end_written && !(s.written && s.begin < end_any), w + ": what the call writes overlaps another tensor, the workspace or itself");
+		end_any = std::max(end_any, s.end);
+		if (s.written) end_written = std::max(end_written, s.end);
+	}
+	if (int rc = dense_check_device(what, (hipStream_t)stream, buffers.data(), buffers.size())) return rc;
+	launch_gradient_norm((hipStream_t)stream, n, t, loss_scale, clip, max_norm, norm, (double*)workspace);
+	HIPCHK(hipGetLastError());
+	return 0;
+} catch (const std::bad_alloc&) { return fail("out of host memory"); } // (the table of ranges)
+extern "C" int ngp_gradient_norm(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float* norm, void* workspace, uint64_t workspace_size) {
+	return gradient_norm("ngp_gradient_norm", stream, n_tensors, tensors_host, loss_scale, false, 0.f, norm, workspace, workspace_size);
+}
+extern "C" int ngp_clip_gradients(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float max_norm, float* norm, void* workspace, uint64_t workspace_size) {
+	return gradient_norm("ngp_clip_gradients", stream, n_tensors, tensors_host, loss_scale, true, max_norm, norm, workspace, workspace_size);
+}

@@ -342,6 +342,45 @@ void launch_render_accumulate(hipStream_t s, uint32_t n_floats, const float* fra
 void launch_render_tonemap(hipStream_t s, uint32_t n_pixels, float* rgba, float exposure_scale, const float bg[4], int to_srgb, int curve);
 
 // ---- optional per-kernel HIP-event timing (bench.py roofline leg) -----------------------------
+// ---- dense layers (dense_kernels.hip, compiled once per element type) and gradient clipping (clip_kernels.hip) ----------------
+struct DenseArgs {
+	bool gated; int act; uint32_t m, n, k;              // samples, outputs, inputs; arrays of two: {gate, up} of a gated layer, else [0] alone
+	const void* x; uint64_t x_stride; const void* w[2]; uint64_t w_stride;
+	const void* bias[2]; const void* residual; uint64_t residual_stride; void* y; uint64_t y_stride; // forward
+	void* pre[2]; uint64_t pre_stride;                  // pre-activations: written by the forward pass (optional), read by the backward pass
+	const void* dy; uint64_t dy_stride; void* dx; uint64_t dx_stride; void* dw[2]; uint64_t dw_stride; void* dbias[2]; // backward
+	void* workspace; uint64_t workspace_size;
+};
+// How a backward pass is split and where its pieces lie in the workspace (bytes); derived from the sizes alone so that ngp_*_workspace_size and the launch agree.
+struct DensePlan { uint64_t grad, bias, partial, bytes; uint32_t rows_per_block, row_blocks, splits; };
+inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
+	DensePlan p;
+	const uint64_t problems = gated ? 2 : 1, n8 = ((uint64_t)n + 7) & ~7ull, k8 = ((uint64_t)k + 7) & ~7ull;
+	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
+	// elementwise pass: about 1024 blocks of whole groups of 8 rows
+	const uint64_t col_blocks = (n + 255) / 256, want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
+	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
+	if (!p.rows_per_block) p.rows_per_block = 8;
+	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
+	// weight gradient: a sum over m samples per 128 x 128 tile; split it where the tiles alone leave compute units without work, in pieces of at least 4 chunks of 64 samples
+	const uint64_t tiles = (((uint64_t)n + 127) / 128) * (((uint64_t)k + 127) / 128) * problems, chunks = ((uint64_t)m + 63) / 64, one = problems * n * k8 * 4;
+	uint64_t splits = tiles ? 512 / tiles : 1;
+	if (splits > chunks / 4) splits = chunks / 4;
+	if (one && splits > (256ull << 20) / one) splits = (256ull << 20) / one;
+	if (splits < 1) splits = 1;
+	const uint64_t per = (chunks + splits - 1) / splits;
+	p.splits = (uint32_t)(per ? (chunks + per - 1) / per : 1);
+	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + problems * p.row_blocks * n * 4);
+	p.bytes = p.partial + (p.splits > 1 ? up(p.splits * one) : 0);
+	return p;
+}
+void launch_dense_forward_half(hipStream_t s, const DenseArgs& d);
+void launch_dense_forward_bf16(hipStream_t s, const DenseArgs& d);
+void launch_dense_backward_half(hipStream_t s, const DenseArgs& d);
+void launch_dense_backward_bf16(hipStream_t s, const DenseArgs& d);
+constexpr uint32_t CLIP_SLOTS = 2048; // partial sums (double) of ngp_gradient_norm / ngp_clip_gradients
+void launch_gradient_norm(hipStream_t s, uint32_t n, const ngp_gradient* tensors, float loss_scale, bool clip, float max_norm, float* norm, double* slots);
+
 enum ProfId { P_K1 = 0, P_K2_INFERENCE, P_K3, P_K4, P_T1_FWD_BWD_SCATTER, P_W_WGRAD, P_WGRAD_REDUCE, P_OPTIMIZER, P_GRID_DENSITY, P_GRID_MISC, P_GRAD_MEMSET, P_COUNTERS, P_GRAD_BIN, P_K2_ENCODE_XCD, P_TRAIN_FUSED, P_COUNT };
 
 } // namespace ngp

@@ -15,7 +15,8 @@ vp = C.c_void_p
 
 LENS_PERSPECTIVE, LENS_OPENCV, LENS_FTHETA, LENS_LATLONG, LENS_OPENCV_FISHEYE, LENS_EQUIRECTANGULAR, LENS_ORTHOGRAPHIC = 0, 1, 2, 3, 4, 5, 6
 IMAGE_BYTE, IMAGE_HALF, IMAGE_FLOAT = 1, 2, 3
-ACT_NONE, ACT_RELU, ACT_LOGISTIC, ACT_EXPONENTIAL = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_LOGISTIC, ACT_EXPONENTIAL, ACT_SILU, ACT_GELU = range(6)
+TYPE_HALF, TYPE_BFLOAT16, TYPE_FLOAT = range(3)
 DBG_K4_ZERO_PADDING = 1 << 26  # ngp_debug_set_flags test hook (csrc/ngp_kernels.hpp)
 LOSS_L2, LOSS_L1, LOSS_MAPE, LOSS_SMAPE, LOSS_HUBER, LOSS_LOGL1, LOSS_RELATIVE_L2 = range(7)
 
@@ -123,6 +124,10 @@ class RenderParams(C.Structure):
                 ("min_transmittance", f32), ("near_distance", f32), ("use_inference_params", i32), ("render_aabb", Aabb)]
 
 
+class Gradient(C.Structure):
+    _fields_ = [("grad", vp), ("clipped", vp), ("size", u64), ("type", i32), ("reserved", i32)]
+
+
 def base_model_config(aabb_scale=1, **kw):
     """configs/nerf/base.json + the per_level_scale derivation of testbed.cu:4241-4255."""
     import math
@@ -192,6 +197,17 @@ def load_hip():
             _lib.ngp_model_state_offset.argtypes = [u64, C.c_int]
         _lib.ngp_encmlp_learning_rate.restype = f32
         _lib.ngp_encmlp_step.restype = u32
+        if hasattr(_lib, "ngp_linear_forward"):
+            layer, tail = [vp, C.c_int, C.c_int, u32, u32, u32, vp, u64], [vp, u64]  # stream, type, activation, m, n, k, x, x_stride ... workspace, workspace_size
+            _lib.ngp_linear_forward.argtypes = layer + [vp, u64, vp, vp, u64, vp, u64, vp, u64] + tail
+            _lib.ngp_linear_backward.argtypes = layer + [vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp] + tail
+            _lib.ngp_gated_forward.argtypes = layer + [vp, vp, u64, vp, vp, vp, u64, vp, vp, u64] + tail
+            _lib.ngp_gated_backward.argtypes = layer + [vp, vp, u64, vp, vp, u64, vp, u64, vp, u64, vp, vp, u64, vp, vp] + tail
+            for f in (_lib.ngp_linear_workspace_size, _lib.ngp_gated_workspace_size):
+                f.argtypes, f.restype = [u32, u32, u32, C.c_int], u64
+            _lib.ngp_gradient_norm.argtypes = [vp, u32, vp, f32, vp] + tail
+            _lib.ngp_clip_gradients.argtypes = [vp, u32, vp, f32, f32, vp] + tail
+            _lib.ngp_gradient_workspace_size.restype = u64
     return _lib
 
 
