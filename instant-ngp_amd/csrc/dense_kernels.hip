@@ -13,6 +13,7 @@
 #include <hip/hip_fp16.h>
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 #include "ngp_kernels.hpp"
 
 namespace ngp {
@@ -37,6 +38,22 @@ __device__ inline f4v mfma(T8 a, T8 b, f4v c) {
 	return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 #endif
 }
+// the same with the sums held in place in accumulation registers (the compiler, left to itself, moves 256 of them about and spills).  Whoever reads the sums with
+// other instructions waits first: settle().  The operands come from LDS reads alone (a vector instruction that wrote one would need two wait states in front).
+__device__ inline void mfma_in_place(T8 a, T8 b, f4v& c) {
+#ifdef DENSE_BF16
+	asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+#else
+	asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+#endif
+}
+template <int N, int M> __device__ inline void settle(f4v (&c)[N][M]) { // more wait states than the longest matrix instruction needs, in front of every later use of c
+	asm volatile("s_nop 15\n\ts_nop 15" ::);
+#pragma unroll
+	for (int i = 0; i < N; ++i)
+#pragma unroll
+		for (int j = 0; j < M; ++j) asm volatile("" : "+a"(c[i][j]));
+}
 // 8 consecutive elements at any 2-byte aligned address (one 16-byte access: global memory takes unaligned vectors); the first n of them where n < 8
 __device__ inline T8 load8(const T* p) { T8 v; __builtin_memcpy(&v, p, 16); return v; }
 __device__ inline T8 load8(const T* p, int n) {
@@ -54,24 +71,25 @@ __device__ inline void store8(T* p, T8 v, int n) {
 
 // ---- activations: values and derivatives in 32 bits.  1 / (1 + e^-z) through v_exp_f32 / v_rcp_f32 (1 ulp each): far below the 16-bit rounding of the result
 __device__ inline float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
-__device__ inline float act_value(int act, float z) {
+__device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 values)
+#define EACH for (int e = 0; e < 8; ++e)
 	switch (act) {
-		case NGP_ACT_RELU: return z < 0.f ? 0.f : z; // (NaN stays NaN)
-		case NGP_ACT_LOGISTIC: return logistic(z);
-		case NGP_ACT_EXPONENTIAL: return __expf(z);
-		case NGP_ACT_SILU: return z * logistic(z);
-		case NGP_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);
-		default: return z;
+		case NGP_ACT_RELU: EACH z[e] = z[e] < 0.f ? 0.f : z[e]; break; // (NaN stays NaN)
+		case NGP_ACT_LOGISTIC: EACH z[e] = logistic(z[e]); break;
+		case NGP_ACT_EXPONENTIAL: EACH z[e] = __expf(z[e]); break;
+		case NGP_ACT_SILU: EACH z[e] *= logistic(z[e]); break;
+		case NGP_ACT_GELU: EACH z[e] = 0.5f * z[e] * erfcf(-0.70710678f * z[e]); break;
+		default: break;
 	}
 }
-__device__ inline void act_value_slope(int act, float z, float& value, float& slope) {
+__device__ inline void act_value_slope8(int act, const float z[8], float value[8], float slope[8]) {
 	switch (act) {
-		case NGP_ACT_RELU: value = z < 0.f ? 0.f : z; slope = z > 0.f ? 1.f : 0.f; break;
-		case NGP_ACT_LOGISTIC: { const float p = logistic(z); value = p; slope = p * (1.f - p); break; }
-		case NGP_ACT_EXPONENTIAL: value = slope = __expf(z); break;
-		case NGP_ACT_SILU: { const float p = logistic(z); value = z * p; slope = p * (1.f + z * (1.f - p)); break; }
-		case NGP_ACT_GELU: { const float c = 0.5f * erfcf(-0.70710678f * z); value = z * c; slope = c + z * 0.39894228f * __expf(-0.5f * z * z); break; }
-		default: value = z; slope = 1.f;
+		case NGP_ACT_RELU: EACH { value[e] = z[e] < 0.f ? 0.f : z[e]; slope[e] = z[e] > 0.f ? 1.f : 0.f; } break;
+		case NGP_ACT_LOGISTIC: EACH { const float p = logistic(z[e]); value[e] = p; slope[e] = p * (1.f - p); } break;
+		case NGP_ACT_EXPONENTIAL: EACH value[e] = slope[e] = __expf(z[e]); break;
+		case NGP_ACT_SILU: EACH { const float p = logistic(z[e]); value[e] = z[e] * p; slope[e] = p * (1.f + z[e] * (1.f - p)); } break;
+		case NGP_ACT_GELU: EACH { const float c = 0.5f * erfcf(-0.70710678f * z[e]); value[e] = z[e] * c; slope[e] = c + z[e] * 0.39894228f * __expf(-0.5f * z[e] * z[e]); } break;
+		default: EACH { value[e] = z[e]; slope[e] = 1.f; } break;
 	}
 }
 
@@ -118,6 +136,33 @@ struct GemmArgs {
 	int act; const T* bias[2]; const T* residual; uint64_t ld_residual; T* pre[2]; uint64_t ld_pre;
 };
 __host__ __device__ inline uint32_t up8(uint32_t v) { return (v + 7) & ~7u; }
+
+// What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C
+template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8]) {
+	T8 o, s;
+	if constexpr (EPI == EPI_PARTIAL) {
+		float* q = g.partial + (((uint64_t)split * g.problems + problem) * g.rows + r) * up8(g.cols) + c; // (lines are padded to 8: always whole)
+		*(f4v*)q = f4v{z[0], z[1], z[2], z[3]}; *(f4v*)(q + 4) = f4v{z[4], z[5], z[6], z[7]};
+		return;
+	}
+	if constexpr (EPI == EPI_STORE) {
+		EACH o[e] = (T)z[e];
+		store8(g.c[problem] + (uint64_t)r * g.ldc + c, o, n);
+		return;
+	}
+	if (g.bias[0]) { const T8 b = load8(g.bias[0] + c, n); EACH z[e] += (float)b[e]; }
+	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n); }
+	act_value8(g.act, z);
+	if constexpr (EPI == EPI_LINEAR) {
+		if (g.residual) { const T8 v = load8(g.residual + (uint64_t)r * g.ld_residual + c, n); EACH z[e] += (float)v[e]; }
+		EACH o[e] = (T)z[e];
+	} else {
+		if (g.bias[1]) { const T8 b = load8(g.bias[1] + c, n); EACH u[e] += (float)b[e]; }
+		if (g.pre[1]) { EACH s[e] = (T)u[e]; store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n); }
+		EACH o[e] = (T)(z[e] * u[e]);
+	}
+	store8(g.c[0] + (uint64_t)r * g.ldc + c, o, n);
+}
 
 // C tile BR x BC by WR x WC wavefronts; each owns (BR / WR) x (BC / WC) as 16 x 16 fragments (matrix instruction 16x16x32, C^T: a lane holds one row of C and 4 columns
 // of each fragment).  EPI_GATED: the tile's columns are BC / 2 gate outputs and the same BC / 2 up outputs, every wavefront owns both of its columns.
@@ -197,50 +242,197 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 			const uint32_t c = c0 + pair_at(p) + gq * 8;
 			if (c >= g.cols) continue;
 			const int n = (int)min(8u, g.cols - c);
-			float z[8];
-#pragma unroll
-			for (int e = 0; e < 8; ++e) z[e] = acc[i][2 * p + e / 4][e & 3];
-			if constexpr (EPI == EPI_PARTIAL) {
-				float* o = g.partial + (((uint64_t)split * g.problems + problem) * g.rows + r) * up8(g.cols) + c; // (lines are padded to 8: always whole)
-				*(f4v*)o = f4v{z[0], z[1], z[2], z[3]}; *(f4v*)(o + 4) = f4v{z[4], z[5], z[6], z[7]};
-			} else if constexpr (EPI == EPI_STORE) {
-				T8 o;
-#pragma unroll
-				for (int e = 0; e < 8; ++e) o[e] = (T)z[e];
-				store8(g.c[problem] + (uint64_t)r * g.ldc + c, o, n);
-			} else {
-				T8 o, s;
-				if (g.bias[0]) { const T8 b = load8(g.bias[0] + c, n);
-#pragma unroll
-					for (int e = 0; e < 8; ++e) z[e] += (float)b[e]; }
-				if (g.pre[0]) {
-#pragma unroll
-					for (int e = 0; e < 8; ++e) s[e] = (T)z[e];
-					store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n);
-				}
-				if constexpr (EPI == EPI_LINEAR) {
-					T8 res{};
-					if (g.residual) res = load8(g.residual + (uint64_t)r * g.ld_residual + c, n);
-#pragma unroll
-					for (int e = 0; e < 8; ++e) { const float v = act_value(g.act, z[e]); o[e] = (T)(g.residual ? v + (float)res[e] : v); }
-				} else {
-					float u[8];
-#pragma unroll
-					for (int e = 0; e < 8; ++e) u[e] = acc[i][FC / 2 + 2 * p + e / 4][e & 3];
-					if (g.bias[1]) { const T8 b = load8(g.bias[1] + c, n);
-#pragma unroll
-						for (int e = 0; e < 8; ++e) u[e] += (float)b[e]; }
-					if (g.pre[1]) {
-#pragma unroll
-						for (int e = 0; e < 8; ++e) s[e] = (T)u[e];
-						store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n);
-					}
-#pragma unroll
-					for (int e = 0; e < 8; ++e) o[e] = (T)(act_value(g.act, z[e]) * u[e]);
-				}
-				store8(g.c[0] + (uint64_t)r * g.ldc + c, o, n);
-			}
+			float z[8], u[8];
+			EACH { z[e] = acc[i][2 * p + e / 4][e & 3]; u[e] = EPI == EPI_GATED ? acc[i][(EPI == EPI_GATED ? FC / 2 : 0) + 2 * p + e / 4][e & 3] : 0.f; }
+			epilogue8<EPI>(g, problem, split, r, c, n, z, u);
 		}
+	}
+}
+
+// ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero), AK steps of
+// the sum a stage, STAGES stages in a ring.  The loads of a stage are issued three stages before it is needed (about 3000 clocks at 256 x 256: the latency of HBM).  While the
+// matrix instructions of a stage run, its A fragments come in three ahead of their use and the next stage's B fragments into a second set of registers; one barrier a stage.
+// 4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128 products is what LDS can deliver beside the incoming stage (96 of the 128 bytes a clock; with
+// 8 wavefronts of 128 x 64 it would be all of them).
+constexpr int AK = 32, STAGES = 5, A_RING = 4;
+typedef int i4v __attribute__((ext_vector_type(4)));
+template <int EXTENT, bool T_CONTIG, bool IS_B, int WAVES> struct Async {
+	static constexpr int SLOTS = T_CONTIG ? AK / 8 : EXTENT / 8, BYTES = EXTENT * AK * 2, LOADS = BYTES / 1024 / WAVES;
+	static_assert(LOADS >= 1, "a wavefront has something to load");
+	uint32_t at[LOADS], step[LOADS]; // byte offset from the tile's first element; first step of the chunk (T_CONTIG)
+	__device__ static int source(int line, int slot) {
+		if (T_CONTIG) return slot ^ ((line >> (IS_B ? 3 : 2)) & 3);
+		if (IS_B) return slot ^ ((line & (EXTENT >= 128 ? 3 : 1)) << 2);
+		return slot ^ ((line & (EXTENT >= 128 ? 7 : 3)) << 1);
+	}
+	__device__ void setup(uint32_t lane, uint32_t wave, uint64_t ld, uint32_t skip_lines /* wave-uniform: lines in front of this wavefront's that belong to another matrix */) {
+#pragma unroll
+		for (int q = 0; q < LOADS; ++q) {
+			const int slot = (wave * LOADS + q) * 64 + lane, line = slot / SLOTS, chunk = source(line, slot % SLOTS);
+			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step[q] = chunk * 8;
+		}
+	}
+	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on
+	__device__ void load(int q, i4v rsrc, uint32_t lds, uint32_t left) const {
+		const uint32_t off = T_CONTIG && step[q] >= left ? 0x80000000u : at[q]; // behind the sum's last step: out of range, zero
+		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)); // (M0 lives inside this block alone: the compiler sets it anew wherever it needs it)
+	}
+};
+// buffer resource over `elements` elements (none if negative) from p on: loads beyond them return zero
+__device__ inline i4v resource(const T* p, int64_t elements) {
+	const uint64_t a = (uint64_t)p;
+	const int64_t bytes = elements * 2;
+	const uint32_t records = bytes <= 0 ? 0u : bytes > 0x7ffffff0ll ? 0x7ffffff0u : (uint32_t)bytes;
+	return i4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), __builtin_amdgcn_readfirstlane((int)records), 0x00020000};
+}
+// consecutive blocks go to the 8 dies in turn: give each die one contiguous run of tiles, ordered in strips of 8 row tiles, so that its blocks share operands in its L2
+__device__ inline void tile_of(uint32_t b, uint32_t row_tiles, uint32_t col_tiles, uint32_t& tr, uint32_t& tc) {
+	const uint32_t n = row_tiles * col_tiles, die = b & 7, per = n >> 3, rest = n & 7;
+	const uint32_t t = die * per + min(die, rest) + (b >> 3), strip = 8 * col_tiles, s = t / strip, in = t - s * strip, rows = min(8u, row_tiles - s * 8);
+	tr = s * 8 + in % rows; tc = in / rows;
+}
+template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
+__global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(GemmArgs g) {
+	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = EPI == EPI_GATED ? BC / 2 : BC;
+	typedef Async<BR, A_T, false, WAVES> LA; typedef Async<BC, B_T, true, WAVES> LB;
+	constexpr int STAGE = LA::BYTES + LB::BYTES, D = LA::LOADS + LB::LOADS;
+	constexpr int STRIP = BC / WC + 4, PASS = FR > 4 ? 4 : FR; // epilogue: floats per row of a wavefront's strip of LDS, fragment rows in it
+	static_assert(WAVES * PASS * 16 * STRIP * 4 <= STAGES * STAGE && FR % PASS == 0, "the epilogue's strips fit");
+	static_assert(FC % (EPI == EPI_GATED ? 4 : 2) == 0 && 3 * D < 63, "");
+	__shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+	const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
+	uint32_t tr, tc;
+	tile_of(blockIdx.x, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT, tr, tc);
+	const uint32_t r0 = tr * BR, c0 = tc * OUT, problem = blockIdx.y, split = blockIdx.z;
+	const uint32_t chunks_per_segment = (g.steps + AK - 1) / AK, n_chunks = chunks_per_segment * g.segments;
+	const uint32_t t_begin = min(n_chunks, split * g.chunks_per_split), t_end = min(n_chunks, t_begin + g.chunks_per_split);
+	const uint32_t which = EPI == EPI_GATED && wave * LB::LOADS * 16 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
+	LA la; LB lb;
+	la.setup(lane, wave, g.lda, 0); lb.setup(lane, wave, g.ldb, which * OUT);
+	const T* a0 = g.a + problem * g.a_problem + (A_T ? (uint64_t)r0 * g.lda : (uint64_t)r0);
+	const T* b0 = B_T ? g.b[which] + (uint64_t)c0 * g.ldb : nullptr;
+	const uint32_t steps8 = up8(g.steps);
+	uint32_t seg = t_begin / (chunks_per_segment ? chunks_per_segment : 1), t0 = (t_begin - seg * chunks_per_segment) * AK, loaded = t_begin, slot = 0; // next chunk to load
+	i4v rs_a, rs_b; uint32_t left = 0, lds_load = 0;
+	auto next_chunk = [&]() { // resources of the next chunk to load (empty behind the last one) and its place in the ring
+		const bool any = loaded < t_end;
+		left = any ? g.steps - t0 : 0;
+		if (A_T) rs_a = resource(a0 + seg * g.a_segment + t0, any ? (int64_t)(min((uint32_t)BR, g.rows - r0) - 1) * (int64_t)g.lda + (steps8 - t0) : 0);
+		else rs_a = resource(a0 + seg * g.a_segment + (uint64_t)t0 * g.lda, any ? (int64_t)(min((uint32_t)AK, left) - 1) * (int64_t)g.lda + (up8(g.rows) - r0) : 0);
+		if (B_T) rs_b = resource(b0 + t0, any ? (int64_t)(min((uint32_t)OUT, g.cols - c0) - 1) * (int64_t)g.ldb + (steps8 - t0) : 0);
+		else rs_b = resource(g.b[seg] + (uint64_t)t0 * g.ldb + c0, any ? (int64_t)(min((uint32_t)AK, left) - 1) * (int64_t)g.ldb + (g.cols - c0) : 0);
+		lds_load = lds0 + slot * STAGE; slot = slot + 1 == STAGES ? 0 : slot + 1;
+		++loaded; t0 += AK;
+		if (t0 >= g.steps) { t0 = 0; if (seg + 1 < g.segments) ++seg; }
+	};
+	auto load = [&](int q) {
+		if (q < LA::LOADS) la.load(q, rs_a, lds_load + (wave * LA::LOADS + q) * 1024, left);
+		else lb.load(q - LA::LOADS, rs_b, lds_load + LA::BYTES + (wave * LB::LOADS + q - LA::LOADS) * 1024, left);
+	};
+	// where the lane finds its fragments in a stage
+	typedef __attribute__((address_space(3))) const T8 lds_T8;
+	uint32_t fa_at[FR][2], fb_at[FC / 2][2];
+	auto pair_at = [&](int p) -> int { // first column (in the B tile) of fragment pair p of this wavefront
+		if (EPI == EPI_GATED) return (p >= FC / 4 ? OUT : 0) + (int)wc * (OUT / WC) + (p % (FC / 4)) * 32;
+		return (int)wc * (BC / WC) + p * 32;
+	};
+#pragma unroll
+	for (int i = 0; i < FR; ++i)
+#pragma unroll
+		for (int h = 0; h < 2; ++h) {
+			const int first = wr * (BR / WR) + i * 16;
+			if (A_T) { const int line = first + li; fa_at[i][h] = line * AK * 2 + LA::source(line, gq) * 16; }
+			else { const int line = gq * 8 + h * 4 + (li >> 2), e = first + (li & 3) * 4; fa_at[i][h] = line * BR * 2 + LA::source(line, e >> 3) * 16 + (e & 7) * 2; }
+		}
+#pragma unroll
+	for (int p = 0; p < FC / 2; ++p)
+#pragma unroll
+		for (int h = 0; h < 2; ++h) { // B_T: h = odd fragment of the pair; else h = half of the 8 steps (the odd fragment lies 8 bytes further)
+			const int first = pair_at(p);
+			if (B_T) { const int line = first + (li >> 2) * 8 + h * 4 + (li & 3); fb_at[p][h] = LA::BYTES + line * AK * 2 + LB::source(line, gq) * 16; }
+			else { const int line = gq * 8 + h * 4 + (li >> 2), e = first + (li & 3) * 8; fb_at[p][h] = LA::BYTES + line * BC * 2 + LB::source(line, e >> 3) * 16; }
+		}
+	auto read_a = [&](int i, uint32_t stage) -> T8 {
+		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(stage + fa_at[i][0]);
+		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fa_at[i][0])), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fa_at[i][1]));
+		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+	};
+	auto read_b = [&](int j, uint32_t stage) -> T8 {
+		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(stage + fb_at[j / 2][j & 1]);
+		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fb_at[j / 2][0] + (j & 1) * 8));
+		const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fb_at[j / 2][1] + (j & 1) * 8));
+		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+	};
+	f4v acc[FR][FC];
+#pragma unroll
+	for (int i = 0; i < FR; ++i)
+#pragma unroll
+		for (int j = 0; j < FC; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
+	constexpr int AHEAD = A_RING - 1;
+	static_assert(FR % A_RING == 0, "a stage begins at the ring's first fragment");
+	T8 fa[A_RING], fb[2][FC];
+	uint32_t read_slot = 0;
+	// the matrix instructions of one stage (B fragments `cur`) with, in between, the loads of the stage that takes the slot the last one left and the reads of what comes next
+	auto stage_step = [&](auto cur_c) {
+		constexpr int cur = decltype(cur_c)::value, nxt = cur ^ 1;
+		asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * D) : "memory"); // the next stage has arrived, for every wavefront; the last one's slot has been read by all
+		next_chunk();
+		const uint32_t here = lds0 + read_slot * STAGE;
+		read_slot = read_slot + 1 == STAGES ? 0 : read_slot + 1;
+		const uint32_t next = lds0 + read_slot * STAGE;
+#pragma unroll
+		for (int i = 0; i < FR; ++i) {
+#pragma unroll
+			for (int q = i * D / FR; q < (i + 1) * D / FR; ++q) load(q);
+			fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(i + AHEAD, here) : read_a(i + AHEAD - FR, next);
+#pragma unroll
+			for (int j = i * FC / FR; j < (i + 1) * FC / FR; ++j) fb[nxt][j] = read_b(j, next);
+#pragma unroll
+			for (int j = 0; j < FC; ++j) mfma_in_place(fb[cur][j], fa[i % A_RING], acc[i][j]);
+			__builtin_amdgcn_sched_barrier(0);
+		}
+	};
+	if (t_begin < t_end) {
+#pragma unroll
+		for (int k = 0; k < STAGES - 1; ++k) {
+			next_chunk();
+#pragma unroll
+			for (int q = 0; q < D; ++q) load(q);
+		}
+		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * D) : "memory");
+#pragma unroll
+		for (int i = 0; i < AHEAD; ++i) fa[i] = read_a(i, lds0);
+#pragma unroll
+		for (int j = 0; j < FC; ++j) fb[0][j] = read_b(j, lds0);
+		for (uint32_t t = t_begin; t < t_end; t += 2) { // (an odd last stage is followed by one of zeros)
+			stage_step(std::integral_constant<int, 0>());
+			stage_step(std::integral_constant<int, 1>());
+		}
+		settle(acc);
+		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is under way to LDS any more
+	}
+	// epilogue through the wavefront's own strip of LDS: 8 consecutive columns a lane, whole lines a store
+	float* strip = (float*)lds + wave * PASS * 16 * STRIP;
+	constexpr int LANES = OUT / WC / 8, ROWS = 64 / LANES; // lanes a row, rows at a time
+	const uint32_t er = lane / LANES, ec = (lane % LANES) * 8, c = c0 + wc * (OUT / WC) + ec;
+#pragma unroll
+	for (int pass = 0; pass < FR / PASS; ++pass) {
+#pragma unroll
+		for (int i = 0; i < PASS; ++i)
+#pragma unroll
+			for (int j = 0; j < FC; ++j) *(f4v*)(strip + (i * 16 + li) * STRIP + (j / 2) * 32 + gq * 8 + (j & 1) * 4) = acc[pass * PASS + i][j];
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the strip is this wavefront's alone)
+#pragma unroll 2
+		for (int k = 0; k < PASS * 16; k += ROWS) {
+			const uint32_t r = r0 + wr * (BR / WR) + pass * PASS * 16 + k + er;
+			float z[8], u[8];
+			const float* p = strip + (k + er) * STRIP + ec;
+			*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
+			if constexpr (EPI == EPI_GATED) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
+			if (r < g.rows && c < g.cols) epilogue8<EPI>(g, problem, split, r, c, (int)min(8u, g.cols - c), z, u);
+		}
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
 }
 
@@ -259,13 +451,14 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 			T8 z{}, u{}, o, o2;
 			if (g.pre[0]) z = load8(g.pre[0] + (uint64_t)r * g.ld_pre + c, n);
 			if (GATED) u = load8(g.pre[1] + (uint64_t)r * g.ld_pre + c, n);
+			float zf[8], value[8], slope[8];
+			EACH zf[e] = (float)z[e];
+			act_value_slope8(g.act, zf, value, slope);
 #pragma unroll
 			for (int e = 0; e < 8; ++e) {
-				float value, slope;
-				act_value_slope(g.act, (float)z[e], value, slope);
-				const float v = e < n && slope != 0.f ? (GATED ? (float)dy[e] * (float)u[e] * slope : (float)dy[e] * slope) : 0.f; // (a closed unit passes nothing, whatever arrives)
+				const float v = e < n && slope[e] != 0.f ? (GATED ? (float)dy[e] * (float)u[e] * slope[e] : (float)dy[e] * slope[e]) : 0.f; // (a closed unit passes nothing, whatever arrives)
 				sum[0][e] += v; o[e] = (T)v;
-				if (GATED) { const float w = e < n ? (float)dy[e] * value : 0.f; sum[GATED ? 1 : 0][e] += w; o2[e] = (T)w; }
+				if (GATED) { const float w = e < n ? (float)dy[e] * value[e] : 0.f; sum[GATED ? 1 : 0][e] += w; o2[e] = (T)w; }
 			}
 			if (g.out) {
 				*(T8*)(g.out + (uint64_t)r * g.ld_out + c) = o;
@@ -326,9 +519,19 @@ __global__ __launch_bounds__(256) void k_join_splits(const float* partial, uint3
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g) {
-	constexpr int BR = 128, BC = 128, OUT = EPI == EPI_GATED ? BC / 2 : BC;
-	hipLaunchKernelGGL((k_gemm<BR, BC, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, BR) * div_up(g.cols, OUT), g.problems, g.splits), dim3(256), 0, s, g);
+bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
+// `wholes`: both operands come in whole 16-byte pieces
+template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes) {
+	constexpr int K = EPI == EPI_GATED ? 2 : 1; // weight columns per column of C
+	if (!wholes) {
+		g.chunks_per_split = div_up(div_up(g.steps, TK) * g.segments, g.splits);
+		hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 128) * div_up(g.cols, 128 / K), g.problems, g.splits), dim3(256), 0, s, g);
+		return;
+	}
+	g.chunks_per_split = div_up(div_up(g.steps, AK) * g.segments, g.splits);
+	const uint64_t large = (uint64_t)div_up(g.rows, 256) * div_up(g.cols, 256 / K) * g.problems * g.splits;
+	if (large >= 200) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 256) * div_up(g.cols, 256 / K), g.problems, g.splits), dim3(256), 0, s, g);
+	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 128) * div_up(g.cols, 128 / K), g.problems, g.splits), dim3(256), 0, s, g);
 }
 } // namespace
 
@@ -336,10 +539,11 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	if (!d.m || !d.n) return;
 	GemmArgs g{};
 	g.a = (const T*)d.x; g.lda = d.x_stride; g.ldb = d.w_stride;
-	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1; g.splits = 1; g.chunks_per_split = div_up(d.k, TK);
+	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1; g.splits = 1;
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
-	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g); else launch_gemm<true, true, EPI_LINEAR>(s, g);
+	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
+	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes);
 }
 void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const DensePlan p = dense_plan(d.m, d.n, d.k, d.gated);
@@ -361,22 +565,24 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		}
 		if (bias && d.n) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(256), 0, s, (const float*)(ws + p.bias), p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
 	}
+	const bool g_whole = whole(G, ldg, G == d.dy ? d.n : 8); // (the workspace's lines are padded with zeros)
 	if (d.dx && d.m && d.k) {
 		GemmArgs g{};
 		g.a = G; g.lda = ldg; g.a_segment = up8(d.n); g.segments = problems; g.b[0] = (const T*)d.w[0]; g.b[1] = (const T*)d.w[1]; g.ldb = d.w_stride;
-		g.rows = d.m; g.cols = d.k; g.steps = d.n; g.problems = 1; g.splits = 1; g.chunks_per_split = div_up(d.n, TK) * problems; g.c[0] = (T*)d.dx; g.ldc = d.dx_stride;
-		launch_gemm<true, false, EPI_STORE>(s, g);
+		g.rows = d.m; g.cols = d.k; g.steps = d.n; g.problems = 1; g.splits = 1; g.c[0] = (T*)d.dx; g.ldc = d.dx_stride;
+		launch_gemm<true, false, EPI_STORE>(s, g, g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k));
 	}
 	if ((d.dw[0] || d.dw[1]) && d.n && d.k) {
 		GemmArgs g{};
 		g.a = G; g.lda = ldg; g.a_problem = up8(d.n); g.problems = problems; g.b[0] = g.b[1] = (const T*)d.x; g.ldb = d.x_stride;
 		g.rows = d.n; g.cols = d.k; g.steps = d.m; g.segments = 1; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
-		g.splits = p.splits; g.chunks_per_split = div_up(div_up(d.m, TK), p.splits);
+		g.splits = p.splits;
+		const bool wholes = g_whole && whole(d.x, d.x_stride, d.k);
 		if (p.splits > 1) {
 			g.partial = (float*)(ws + p.partial);
-			launch_gemm<false, false, EPI_PARTIAL>(s, g);
+			launch_gemm<false, false, EPI_PARTIAL>(s, g, wholes);
 			hipLaunchKernelGGL(k_join_splits, dim3(div_up((uint64_t)d.n * up8(d.k) / 8, 256), problems), dim3(256), 0, s, g.partial, p.splits, problems, d.n, d.k, g.c[0], g.c[1], g.ldc);
-		} else launch_gemm<false, false, EPI_STORE>(s, g);
+		} else launch_gemm<false, false, EPI_STORE>(s, g, wholes);
 	}
 }
 } // namespace ngp
