@@ -272,19 +272,22 @@ template <int EXTENT, bool T_CONTIG, bool IS_B, int WAVES> struct Async {
 			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step[q] = chunk * 8;
 		}
 	}
-	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on
+	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on; chunks behind the last of the `left` steps are out of range: zero.  (M0 lives inside this block alone: the compiler sets it anew wherever it needs it)
 	__device__ void load(int q, i4v rsrc, uint32_t lds, uint32_t left) const {
-		const uint32_t off = T_CONTIG && step[q] >= left ? 0x80000000u : at[q]; // behind the sum's last step: out of range, zero
-		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)); // (M0 lives inside this block alone: the compiler sets it anew wherever it needs it)
+		const uint32_t off = T_CONTIG && step[q] >= left ? 0x80000000u : at[q];
+		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
 	}
 };
-// buffer resource over `elements` elements (none if negative) from p on: loads beyond them return zero
-__device__ inline i4v resource(const T* p, int64_t elements) {
-	const uint64_t a = (uint64_t)p;
+// size in bytes of `elements` elements (none if negative) as a buffer resource holds it: loads beyond return zero
+__device__ inline int records(int64_t elements) {
 	const int64_t bytes = elements * 2;
-	const uint32_t records = bytes <= 0 ? 0u : bytes > 0x7ffffff0ll ? 0x7ffffff0u : (uint32_t)bytes;
-	return i4v{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), __builtin_amdgcn_readfirstlane((int)records), 0x00020000};
+	return __builtin_amdgcn_readfirstlane((int)(bytes <= 0 ? 0u : bytes > 0x7ffffff0ll ? 0x7ffffff0u : (uint32_t)bytes));
 }
+__device__ inline const T* uniform(const T* p) { // (a pointer that is the same in every lane, in scalar registers)
+	const uint64_t a = (uint64_t)p;
+	return (const T*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
+}
+__device__ inline i4v resource(const T* p, int records) { const uint64_t a = (uint64_t)p; return i4v{(int)(uint32_t)a, (int)((a >> 32) & 0xffff), records, 0x00020000}; }
 // consecutive blocks go to the 8 dies in turn: give each die one contiguous run of tiles, ordered in strips of 8 row tiles, so that its blocks share operands in its L2
 __device__ inline void tile_of(uint32_t b, uint32_t row_tiles, uint32_t col_tiles, uint32_t& tr, uint32_t& tc) {
 	const uint32_t n = row_tiles * col_tiles, die = b & 7, per = n >> 3, rest = n & 7;
@@ -310,59 +313,73 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	const uint32_t which = EPI == EPI_GATED && wave * LB::LOADS * 16 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
 	LA la; LB lb;
 	la.setup(lane, wave, g.lda, 0); lb.setup(lane, wave, g.ldb, which * OUT);
-	const T* a0 = g.a + problem * g.a_problem + (A_T ? (uint64_t)r0 * g.lda : (uint64_t)r0);
-	const T* b0 = B_T ? g.b[which] + (uint64_t)c0 * g.ldb : nullptr;
-	const uint32_t steps8 = up8(g.steps);
-	uint32_t seg = t_begin / (chunks_per_segment ? chunks_per_segment : 1), t0 = (t_begin - seg * chunks_per_segment) * AK, loaded = t_begin, slot = 0; // next chunk to load
-	i4v rs_a, rs_b; uint32_t left = 0, lds_load = 0;
-	auto next_chunk = [&]() { // resources of the next chunk to load (empty behind the last one) and its place in the ring
+	// The next chunk to load.  T_CONTIG: a line's elements beyond the sum are masked (load()), lines beyond the matrix lie behind `records` wherever the chunk is; otherwise
+	// lines beyond the sum do, in its last chunk alone.
+	const uint32_t lines_a = min((uint32_t)BR, g.rows - r0) - 1, lines_b = min((uint32_t)OUT, g.cols - c0) - 1, steps8 = up8(g.steps);
+	const uint32_t width_a = up8(g.rows) - r0, width_b = g.cols - c0;
+	const int full_a = A_T ? records((int64_t)lines_a * (int64_t)g.lda + steps8) : records((int64_t)(AK - 1) * (int64_t)g.lda + width_a);
+	const int full_b = B_T ? records((int64_t)lines_b * (int64_t)g.ldb + steps8) : records((int64_t)(AK - 1) * (int64_t)g.ldb + width_b);
+	const uint64_t inc_a = A_T ? AK : AK * g.lda, inc_b = B_T ? AK : AK * g.ldb;
+	uint32_t seg, left, loaded = t_begin, slot = 0, lds_load = 0; // segment, steps left in it, chunks loaded, place in the ring
+	const T *at_a, *at_b; int rec_a, rec_b;
+	auto at_chunk = [&](uint32_t segment, uint32_t t0) {
+		seg = segment; left = g.steps - t0;
+		at_a = uniform(g.a + problem * g.a_problem + seg * g.a_segment + (A_T ? (uint64_t)r0 * g.lda + t0 : (uint64_t)t0 * g.lda + r0));
+		at_b = uniform(B_T ? g.b[which] + (uint64_t)c0 * g.ldb + t0 : g.b[seg] + (uint64_t)t0 * g.ldb + c0);
+	};
+	auto limit_chunk = [&]() { // the resources' sizes for the chunk at hand (all zero behind the last one)
 		const bool any = loaded < t_end;
-		left = any ? g.steps - t0 : 0;
-		if (A_T) rs_a = resource(a0 + seg * g.a_segment + t0, any ? (int64_t)(min((uint32_t)BR, g.rows - r0) - 1) * (int64_t)g.lda + (steps8 - t0) : 0);
-		else rs_a = resource(a0 + seg * g.a_segment + (uint64_t)t0 * g.lda, any ? (int64_t)(min((uint32_t)AK, left) - 1) * (int64_t)g.lda + (up8(g.rows) - r0) : 0);
-		if (B_T) rs_b = resource(b0 + t0, any ? (int64_t)(min((uint32_t)OUT, g.cols - c0) - 1) * (int64_t)g.ldb + (steps8 - t0) : 0);
-		else rs_b = resource(g.b[seg] + (uint64_t)t0 * g.ldb + c0, any ? (int64_t)(min((uint32_t)AK, left) - 1) * (int64_t)g.ldb + (g.cols - c0) : 0);
-		lds_load = lds0 + slot * STAGE; slot = slot + 1 == STAGES ? 0 : slot + 1;
-		++loaded; t0 += AK;
-		if (t0 >= g.steps) { t0 = 0; if (seg + 1 < g.segments) ++seg; }
+		rec_a = any ? full_a : 0; rec_b = any ? full_b : 0;
+		if (any && left < AK) {
+			if (!A_T) rec_a = records((int64_t)(left - 1) * (int64_t)g.lda + width_a);
+			if (!B_T) rec_b = records((int64_t)(left - 1) * (int64_t)g.ldb + width_b);
+		}
+	};
+	auto next_chunk = [&]() {
+		++loaded; left -= AK; at_a += inc_a; at_b += inc_b;
+		slot = slot + 1 == STAGES ? 0 : slot + 1; lds_load = lds0 + slot * STAGE;
+		if (loaded >= t_end || (int)left < AK) { // seldom: the sum's or a segment's end
+			if (loaded < t_end && (int)left <= 0) at_chunk(seg + 1, 0);
+			limit_chunk();
+		}
 	};
 	auto load = [&](int q) {
-		if (q < LA::LOADS) la.load(q, rs_a, lds_load + (wave * LA::LOADS + q) * 1024, left);
-		else lb.load(q - LA::LOADS, rs_b, lds_load + LA::BYTES + (wave * LB::LOADS + q - LA::LOADS) * 1024, left);
+		if (q < LA::LOADS) la.load(q, resource(at_a, rec_a), lds_load + (wave * LA::LOADS + q) * 1024, left);
+		else lb.load(q - LA::LOADS, resource(at_b, rec_b), lds_load + LA::BYTES + (wave * LB::LOADS + q - LA::LOADS) * 1024, left);
 	};
-	// where the lane finds its fragments in a stage
+	// where the lane finds its fragments in a stage: one address and constants for operands along t; for the others the XOR leaves one a fragment row (A) or pair (B)
 	typedef __attribute__((address_space(3))) const T8 lds_T8;
-	uint32_t fa_at[FR][2], fb_at[FC / 2][2];
-	auto pair_at = [&](int p) -> int { // first column (in the B tile) of fragment pair p of this wavefront
-		if (EPI == EPI_GATED) return (p >= FC / 4 ? OUT : 0) + (int)wc * (OUT / WC) + (p % (FC / 4)) * 32;
-		return (int)wc * (BC / WC) + p * 32;
-	};
+	auto pair_at = [&](int p) -> int { return EPI == EPI_GATED ? (p >= FC / 4 ? OUT : 0) + (p % (FC / 4)) * 32 : p * 32; }; // column (in the B tile) of fragment pair p behind the wavefront's first one
+	const uint32_t col0 = wc * (EPI == EPI_GATED ? OUT / WC : BC / WC), row0 = wr * (BR / WR), l4 = li >> 2;
+	constexpr bool HALVES = FR == 8; // A across t: the second four steps of fragment i lie where fragment i ^ 4 has its first, one line group further
+	uint32_t fa_at[A_T ? 1 : FR][A_T || HALVES ? 1 : 2], fb_at[B_T ? 1 : FC / 2];
+	if (A_T) fa_at[0][0] = (row0 + li) * AK * 2 + (gq ^ l4) * 16;
+	else {
 #pragma unroll
-	for (int i = 0; i < FR; ++i)
+		for (int i = 0; i < FR; ++i)
 #pragma unroll
-		for (int h = 0; h < 2; ++h) {
-			const int first = wr * (BR / WR) + i * 16;
-			if (A_T) { const int line = first + li; fa_at[i][h] = line * AK * 2 + LA::source(line, gq) * 16; }
-			else { const int line = gq * 8 + h * 4 + (li >> 2), e = first + (li & 3) * 4; fa_at[i][h] = line * BR * 2 + LA::source(line, e >> 3) * 16 + (e & 7) * 2; }
-		}
+			for (int h = 0; h < (HALVES ? 1 : 2); ++h) fa_at[A_T ? 0 : i][A_T || HALVES ? 0 : h] = (gq * 8 + h * 4 + l4) * BR * 2 + ((row0 / 16 + i) ^ (h * 4 + l4)) * 32 + (li & 3) * 8;
+	}
+	if (B_T) fb_at[0] = LA::BYTES + (col0 + l4 * 8 + (li & 3)) * AK * 2 + (gq ^ l4) * 16;
+	else {
 #pragma unroll
-	for (int p = 0; p < FC / 2; ++p)
-#pragma unroll
-		for (int h = 0; h < 2; ++h) { // B_T: h = odd fragment of the pair; else h = half of the 8 steps (the odd fragment lies 8 bytes further)
-			const int first = pair_at(p);
-			if (B_T) { const int line = first + (li >> 2) * 8 + h * 4 + (li & 3); fb_at[p][h] = LA::BYTES + line * AK * 2 + LB::source(line, gq) * 16; }
-			else { const int line = gq * 8 + h * 4 + (li >> 2), e = first + (li & 3) * 8; fb_at[p][h] = LA::BYTES + line * BC * 2 + LB::source(line, e >> 3) * 16; }
-		}
+		for (int p = 0; p < FC / 2; ++p) fb_at[B_T ? 0 : p] = LA::BYTES + (gq * 8 + l4) * BC * 2 + ((col0 / 32 + p) ^ l4) * 64 + (li & 3) * 16;
+	}
+	auto tr4 = [](uint32_t at) -> s4 { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)at); };
 	auto read_a = [&](int i, uint32_t stage) -> T8 {
-		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(stage + fa_at[i][0]);
-		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fa_at[i][0])), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fa_at[i][1]));
-		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(stage + fa_at[0][0] + i * 16 * AK * 2);
+		else {
+			const s4 lo = tr4(stage + fa_at[A_T ? 0 : i][0]), hi = HALVES ? tr4(stage + fa_at[A_T ? 0 : i ^ 4][0] + 4 * BR * 2) : tr4(stage + fa_at[A_T ? 0 : i][A_T || HALVES ? 0 : 1]);
+			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+		}
 	};
 	auto read_b = [&](int j, uint32_t stage) -> T8 {
-		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(stage + fb_at[j / 2][j & 1]);
-		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fb_at[j / 2][0] + (j & 1) * 8));
-		const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(stage + fb_at[j / 2][1] + (j & 1) * 8));
-		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(stage + fb_at[0] + (pair_at(j / 2) + (j & 1) * 4) * AK * 2);
+		else {
+			const uint32_t at = stage + fb_at[B_T ? 0 : j / 2] + (j & 1) * 8;
+			const s4 lo = tr4(at), hi = tr4(at + 4 * BC * 2);
+			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+		}
 	};
 	f4v acc[FR][FC];
 #pragma unroll
@@ -373,32 +390,45 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	static_assert(FR % A_RING == 0, "a stage begins at the ring's first fragment");
 	T8 fa[A_RING], fb[2][FC];
 	uint32_t read_slot = 0;
-	// the matrix instructions of one stage (B fragments `cur`) with, in between, the loads of the stage that takes the slot the last one left and the reads of what comes next
+	// The matrix instructions of one stage (B fragments `cur`).  One wavefront has the SIMD to itself, so whatever else is to be issued stands between two matrix instructions, a little
+	// at a time: the loads of the stage that takes the slot the last one left, the reads of what comes next.  The barrier (the next stage has arrived for every wavefront, the
+	// last one's slot has been read by all: its last fragment went into the matrix instructions before) stands behind the first few of them.
 	auto stage_step = [&](auto cur_c) {
 		constexpr int cur = decltype(cur_c)::value, nxt = cur ^ 1;
-		asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * D) : "memory"); // the next stage has arrived, for every wavefront; the last one's slot has been read by all
-		next_chunk();
 		const uint32_t here = lds0 + read_slot * STAGE;
 		read_slot = read_slot + 1 == STAGES ? 0 : read_slot + 1;
 		const uint32_t next = lds0 + read_slot * STAGE;
 #pragma unroll
 		for (int i = 0; i < FR; ++i) {
+			constexpr int Q = FC / 4; // a quarter of the row's matrix instructions
 #pragma unroll
-			for (int q = i * D / FR; q < (i + 1) * D / FR; ++q) load(q);
-			fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(i + AHEAD, here) : read_a(i + AHEAD - FR, next);
+			for (int j = 0; j < FC; ++j) {
+				mfma_in_place(fb[cur][j], fa[i % A_RING], acc[i][j]);
+				if (j == 0) fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(i + AHEAD, here) : read_a(i + AHEAD - FR, next);
+				if (i == 0 && j == Q) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * D) : "memory");
+				if (j == 2 * Q) {
 #pragma unroll
-			for (int j = i * FC / FR; j < (i + 1) * FC / FR; ++j) fb[nxt][j] = read_b(j, next);
+					for (int q = i * D / FR; q < (i + 1) * D / FR; ++q) load(q);
+				}
+				if (j == 3 * Q) {
 #pragma unroll
-			for (int j = 0; j < FC; ++j) mfma_in_place(fb[cur][j], fa[i % A_RING], acc[i][j]);
-			__builtin_amdgcn_sched_barrier(0);
+					for (int k = i * FC / FR; k < (i + 1) * FC / FR; ++k) fb[nxt][k] = read_b(k, next);
+				}
+				__builtin_amdgcn_sched_barrier(0);
+			}
 		}
+		next_chunk();
 	};
 	if (t_begin < t_end) {
+		const uint32_t first = t_begin / chunks_per_segment;
+		at_chunk(first, (t_begin - first * chunks_per_segment) * AK);
+		limit_chunk();
+		lds_load = lds0;
 #pragma unroll
 		for (int k = 0; k < STAGES - 1; ++k) {
-			next_chunk();
 #pragma unroll
 			for (int q = 0; q < D; ++q) load(q);
+			next_chunk();
 		}
 		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * D) : "memory");
 #pragma unroll
