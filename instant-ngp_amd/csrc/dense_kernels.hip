@@ -249,19 +249,19 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	}
 }
 
-// ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero), AK steps of
-// the sum a stage, STAGES stages in a ring.  The loads of a stage are issued three stages before it is needed (about 3000 clocks at 256 x 256: the latency of HBM).  While the
-// matrix instructions of a stage run, its A fragments come in three ahead of their use and the next stage's B fragments into a second set of registers; one barrier a stage.
-// 4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128 products is what LDS can deliver beside the incoming stage (96 of the 128 bytes a clock; with
-// 8 wavefronts of 128 x 64 it would be all of them).
-constexpr int AK = 32, STAGES = 5, A_RING = 4;
+// ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero) in units of 64 steps
+// of one operand (whole cache lines: 64-byte pieces ask the L2 twice as often, 65 instead of 70 % of the matrix rate).  Three units of A and two of B are in LDS, 160 KB at
+// 256 x 256: the one in use, and what is on its way two halves (A: three) ahead, about 2000 clocks.  The matrix instructions run through a unit in two halves of 32 steps; A fragments
+// come in three ahead of their use, the next half's B fragments into a second set of registers.  4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128
+// products is what LDS can deliver beside the incoming units (96 of the 128 bytes a clock; with 8 wavefronts of 128 x 64 it would be all of them).
+constexpr int AK = 64, UNITS_A = 3, UNITS_B = 2, A_RING = 4;
 typedef int i4v __attribute__((ext_vector_type(4)));
 template <int EXTENT, bool T_CONTIG, bool IS_B, int WAVES> struct Async {
 	static constexpr int SLOTS = T_CONTIG ? AK / 8 : EXTENT / 8, BYTES = EXTENT * AK * 2, LOADS = BYTES / 1024 / WAVES;
-	static_assert(LOADS >= 1, "a wavefront has something to load");
-	uint32_t at[LOADS], step[LOADS]; // byte offset from the tile's first element; first step of the chunk (T_CONTIG)
-	__device__ static int source(int line, int slot) {
-		if (T_CONTIG) return slot ^ ((line >> (IS_B ? 3 : 2)) & 3);
+	static_assert(LOADS >= 2, "a wavefront has something to load");
+	uint32_t at[LOADS], step[2]; // byte offset from the tile's first element; first step of the chunk (T_CONTIG: of even and odd loads)
+	__device__ static int source(int line, int slot) { // chunk that lies in a line's slot (its own inverse)
+		if (T_CONTIG) return IS_B ? slot ^ ((line & 3) | ((line >> 1) & 4)) : slot ^ (line & 7);
 		if (IS_B) return slot ^ ((line & (EXTENT >= 128 ? 3 : 1)) << 2);
 		return slot ^ ((line & (EXTENT >= 128 ? 7 : 3)) << 1);
 	}
@@ -269,12 +269,13 @@ template <int EXTENT, bool T_CONTIG, bool IS_B, int WAVES> struct Async {
 #pragma unroll
 		for (int q = 0; q < LOADS; ++q) {
 			const int slot = (wave * LOADS + q) * 64 + lane, line = slot / SLOTS, chunk = source(line, slot % SLOTS);
-			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step[q] = chunk * 8;
+			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step[q & 1] = chunk * 8;
 		}
 	}
-	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on; chunks behind the last of the `left` steps are out of range: zero.  (M0 lives inside this block alone: the compiler sets it anew wherever it needs it)
-	__device__ void load(int q, i4v rsrc, uint32_t lds, uint32_t left) const {
-		const uint32_t off = T_CONTIG && step[q] >= left ? 0x80000000u : at[q];
+	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on; chunks behind the last of the `left` steps are out of range: zero.  (M0 lives inside this block alone: the
+	// compiler sets it anew wherever it needs it)
+	__device__ void load(int q, i4v rsrc, uint32_t lds, int left) const {
+		const uint32_t off = T_CONTIG && (int)step[q & 1] >= left ? 0x80000000u : at[q];
 		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
 	}
 };
@@ -294,89 +295,84 @@ __device__ inline void tile_of(uint32_t b, uint32_t row_tiles, uint32_t col_tile
 	const uint32_t t = die * per + min(die, rest) + (b >> 3), strip = 8 * col_tiles, s = t / strip, in = t - s * strip, rows = min(8u, row_tiles - s * 8);
 	tr = s * 8 + in % rows; tc = in / rows;
 }
+// Where an operand's next unit comes from and goes to (all in scalar registers).  T_CONTIG: a line's elements beyond the sum are masked (Async::load), lines beyond the matrix lie
+// behind `records` wherever the unit is; otherwise the lines beyond the sum do, in its last unit alone.
+template <bool T_CONTIG, int UNITS, int BYTES> struct Cursor {
+	const T* p; uint64_t inc, ld; uint32_t lds, lds0, seg, loaded, end, width; int left, full, rec;
+	__device__ void limit() { // the size of what may be read of the unit at hand; nothing behind the last one
+		rec = loaded < end ? full : 0;
+		if (!T_CONTIG && loaded < end && left < AK) rec = records((int64_t)(left - 1) * (int64_t)ld + width);
+	}
+	template <typename F> __device__ void next(F&& segment_start, uint32_t steps) {
+		++loaded; left -= AK; p += inc;
+		lds = lds == lds0 + (UNITS - 1) * BYTES ? lds0 : lds + BYTES;
+		if (loaded >= end || left < AK) { // seldom: the sum's or a segment's end
+			if (loaded < end && left <= 0) { ++seg; left = steps; p = segment_start(seg); }
+			limit();
+		}
+	}
+};
 template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
 __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(GemmArgs g) {
 	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = EPI == EPI_GATED ? BC / 2 : BC;
 	typedef Async<BR, A_T, false, WAVES> LA; typedef Async<BC, B_T, true, WAVES> LB;
-	constexpr int STAGE = LA::BYTES + LB::BYTES, D = LA::LOADS + LB::LOADS;
+	constexpr int LDS = UNITS_A * LA::BYTES + UNITS_B * LB::BYTES;
 	constexpr int STRIP = BC / WC + 4, PASS = FR > 4 ? 4 : FR; // epilogue: floats per row of a wavefront's strip of LDS, fragment rows in it
-	static_assert(WAVES * PASS * 16 * STRIP * 4 <= STAGES * STAGE && FR % PASS == 0, "the epilogue's strips fit");
-	static_assert(FC % (EPI == EPI_GATED ? 4 : 2) == 0 && 3 * D < 63, "");
-	__shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+	static_assert(WAVES * PASS * 16 * STRIP * 4 <= LDS && FR % PASS == 0, "the epilogue's strips fit");
+	static_assert(FC % (EPI == EPI_GATED ? 4 : 2) == 0 && FR % A_RING == 0 && LA::LOADS % FR == 0 && LB::LOADS % FR == 0, "");
+	__shared__ __attribute__((aligned(1024))) char lds[LDS];
 	const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
 	uint32_t tr, tc;
 	tile_of(blockIdx.x, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT, tr, tc);
 	const uint32_t r0 = tr * BR, c0 = tc * OUT, problem = blockIdx.y, split = blockIdx.z;
-	const uint32_t chunks_per_segment = (g.steps + AK - 1) / AK, n_chunks = chunks_per_segment * g.segments;
-	const uint32_t t_begin = min(n_chunks, split * g.chunks_per_split), t_end = min(n_chunks, t_begin + g.chunks_per_split);
-	const uint32_t which = EPI == EPI_GATED && wave * LB::LOADS * 16 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
+	const uint32_t units_per_segment = (g.steps + AK - 1) / AK, n_units = units_per_segment * g.segments;
+	const uint32_t t_begin = min(n_units, split * g.chunks_per_split), t_end = min(n_units, t_begin + g.chunks_per_split);
+	const uint32_t which = EPI == EPI_GATED && wave * LB::LOADS * 8 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
 	LA la; LB lb;
 	la.setup(lane, wave, g.lda, 0); lb.setup(lane, wave, g.ldb, which * OUT);
-	// The next chunk to load.  T_CONTIG: a line's elements beyond the sum are masked (load()), lines beyond the matrix lie behind `records` wherever the chunk is; otherwise
-	// lines beyond the sum do, in its last chunk alone.
-	const uint32_t lines_a = min((uint32_t)BR, g.rows - r0) - 1, lines_b = min((uint32_t)OUT, g.cols - c0) - 1, steps8 = up8(g.steps);
-	const uint32_t width_a = up8(g.rows) - r0, width_b = g.cols - c0;
-	const int full_a = A_T ? records((int64_t)lines_a * (int64_t)g.lda + steps8) : records((int64_t)(AK - 1) * (int64_t)g.lda + width_a);
-	const int full_b = B_T ? records((int64_t)lines_b * (int64_t)g.ldb + steps8) : records((int64_t)(AK - 1) * (int64_t)g.ldb + width_b);
-	const uint64_t inc_a = A_T ? AK : AK * g.lda, inc_b = B_T ? AK : AK * g.ldb;
-	uint32_t seg, left, loaded = t_begin, slot = 0, lds_load = 0; // segment, steps left in it, chunks loaded, place in the ring
-	const T *at_a, *at_b; int rec_a, rec_b;
-	auto at_chunk = [&](uint32_t segment, uint32_t t0) {
-		seg = segment; left = g.steps - t0;
-		at_a = uniform(g.a + problem * g.a_problem + seg * g.a_segment + (A_T ? (uint64_t)r0 * g.lda + t0 : (uint64_t)t0 * g.lda + r0));
-		at_b = uniform(B_T ? g.b[which] + (uint64_t)c0 * g.ldb + t0 : g.b[seg] + (uint64_t)t0 * g.ldb + c0);
-	};
-	auto limit_chunk = [&]() { // the resources' sizes for the chunk at hand (all zero behind the last one)
-		const bool any = loaded < t_end;
-		rec_a = any ? full_a : 0; rec_b = any ? full_b : 0;
-		if (any && left < AK) {
-			if (!A_T) rec_a = records((int64_t)(left - 1) * (int64_t)g.lda + width_a);
-			if (!B_T) rec_b = records((int64_t)(left - 1) * (int64_t)g.ldb + width_b);
-		}
-	};
-	auto next_chunk = [&]() {
-		++loaded; left -= AK; at_a += inc_a; at_b += inc_b;
-		slot = slot + 1 == STAGES ? 0 : slot + 1; lds_load = lds0 + slot * STAGE;
-		if (loaded >= t_end || (int)left < AK) { // seldom: the sum's or a segment's end
-			if (loaded < t_end && (int)left <= 0) at_chunk(seg + 1, 0);
-			limit_chunk();
-		}
-	};
-	auto load = [&](int q) {
-		if (q < LA::LOADS) la.load(q, resource(at_a, rec_a), lds_load + (wave * LA::LOADS + q) * 1024, left);
-		else lb.load(q - LA::LOADS, resource(at_b, rec_b), lds_load + LA::BYTES + (wave * LB::LOADS + q - LA::LOADS) * 1024, left);
-	};
-	// where the lane finds its fragments in a stage: one address and constants for operands along t; for the others the XOR leaves one a fragment row (A) or pair (B)
+	auto start_a = [&](uint32_t seg) -> const T* { return uniform(g.a + problem * g.a_problem + seg * g.a_segment + (A_T ? (uint64_t)r0 * g.lda : (uint64_t)r0)); };
+	auto start_b = [&](uint32_t seg) -> const T* { return uniform(B_T ? g.b[which] + (uint64_t)c0 * g.ldb : g.b[seg] + c0); };
+	Cursor<A_T, UNITS_A, LA::BYTES> ca; Cursor<B_T, UNITS_B, LB::BYTES> cb;
+	{
+		const uint32_t seg = units_per_segment ? t_begin / units_per_segment : 0, t0 = (t_begin - seg * units_per_segment) * AK, steps8 = up8(g.steps);
+		ca.ld = g.lda; cb.ld = g.ldb; ca.inc = A_T ? AK : AK * g.lda; cb.inc = B_T ? AK : AK * g.ldb;
+		ca.lds = ca.lds0 = lds0; cb.lds = cb.lds0 = lds0 + UNITS_A * LA::BYTES;
+		ca.width = up8(g.rows) - r0; cb.width = g.cols - c0;
+		ca.full = A_T ? records((int64_t)(min((uint32_t)BR, g.rows - r0) - 1) * (int64_t)g.lda + steps8) : records((int64_t)(AK - 1) * (int64_t)g.lda + ca.width);
+		cb.full = B_T ? records((int64_t)(min((uint32_t)OUT, g.cols - c0) - 1) * (int64_t)g.ldb + steps8) : records((int64_t)(AK - 1) * (int64_t)g.ldb + cb.width);
+		ca.seg = cb.seg = seg; ca.loaded = cb.loaded = t_begin; ca.end = cb.end = t_end; ca.left = cb.left = (int)(g.steps - t0);
+		ca.p = start_a(seg) + (A_T ? t0 : t0 * g.lda); cb.p = start_b(seg) + (B_T ? t0 : t0 * g.ldb);
+		ca.limit(); cb.limit();
+	}
+	auto load_a = [&](int q) { la.load(q, resource(ca.p, ca.rec), ca.lds + (wave * LA::LOADS + q) * 1024, ca.left); };
+	auto load_b = [&](int q) { lb.load(q, resource(cb.p, cb.rec), cb.lds + (wave * LB::LOADS + q) * 1024, cb.left); };
+	// where the lane finds its fragments in a unit: an address for each half and constants for operands along t; for the others the XOR leaves one a fragment row (A) or pair (B)
 	typedef __attribute__((address_space(3))) const T8 lds_T8;
 	auto pair_at = [&](int p) -> int { return EPI == EPI_GATED ? (p >= FC / 4 ? OUT : 0) + (p % (FC / 4)) * 32 : p * 32; }; // column (in the B tile) of fragment pair p behind the wavefront's first one
 	const uint32_t col0 = wc * (EPI == EPI_GATED ? OUT / WC : BC / WC), row0 = wr * (BR / WR), l4 = li >> 2;
-	constexpr bool HALVES = FR == 8; // A across t: the second four steps of fragment i lie where fragment i ^ 4 has its first, one line group further
-	uint32_t fa_at[A_T ? 1 : FR][A_T || HALVES ? 1 : 2], fb_at[B_T ? 1 : FC / 2];
-	if (A_T) fa_at[0][0] = (row0 + li) * AK * 2 + (gq ^ l4) * 16;
-	else {
+	constexpr bool PAIRED = FR == 8; // A across t: the second four steps of fragment i lie where fragment i ^ 4 has its first, four lines further
+	constexpr int NA = A_T ? 2 : PAIRED ? FR : 2 * FR, NB = B_T ? 2 : FC / 2;
+	uint32_t fa_at[NA], fb_at[NB];
 #pragma unroll
-		for (int i = 0; i < FR; ++i)
+	for (int k = 0; k < NA; ++k) fa_at[k] = A_T ? (row0 + li) * AK * 2 + (((k * 4) + gq) ^ (li & 7)) * 16
+		: (gq * 8 + (k / FR) * 4 + l4) * BR * 2 + ((row0 / 16 + k % FR) ^ ((k / FR) * 4 + l4)) * 32 + (li & 3) * 8;
 #pragma unroll
-			for (int h = 0; h < (HALVES ? 1 : 2); ++h) fa_at[A_T ? 0 : i][A_T || HALVES ? 0 : h] = (gq * 8 + h * 4 + l4) * BR * 2 + ((row0 / 16 + i) ^ (h * 4 + l4)) * 32 + (li & 3) * 8;
-	}
-	if (B_T) fb_at[0] = LA::BYTES + (col0 + l4 * 8 + (li & 3)) * AK * 2 + (gq ^ l4) * 16;
-	else {
-#pragma unroll
-		for (int p = 0; p < FC / 2; ++p) fb_at[B_T ? 0 : p] = LA::BYTES + (gq * 8 + l4) * BC * 2 + ((col0 / 32 + p) ^ l4) * 64 + (li & 3) * 16;
-	}
+	for (int k = 0; k < NB; ++k) fb_at[k] = B_T ? (col0 + l4 * 8 + (li & 3)) * AK * 2 + (((k * 4) + gq) ^ ((li & 3) | ((l4 & 1) << 2))) * 16
+		: (gq * 8 + l4) * BC * 2 + ((col0 / 32 + k) ^ l4) * 64 + (li & 3) * 16;
 	auto tr4 = [](uint32_t at) -> s4 { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)at); };
-	auto read_a = [&](int i, uint32_t stage) -> T8 {
-		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(stage + fa_at[0][0] + i * 16 * AK * 2);
+	auto read_a = [&](int half, int i, uint32_t unit) -> T8 {
+		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(unit + fa_at[half] + i * 16 * AK * 2);
 		else {
-			const s4 lo = tr4(stage + fa_at[A_T ? 0 : i][0]), hi = HALVES ? tr4(stage + fa_at[A_T ? 0 : i ^ 4][0] + 4 * BR * 2) : tr4(stage + fa_at[A_T ? 0 : i][A_T || HALVES ? 0 : 1]);
+			const uint32_t base = unit + half * 32 * BR * 2;
+			const s4 lo = tr4(base + fa_at[i % NA]), hi = PAIRED ? tr4(base + fa_at[(i ^ 4) % NA] + 4 * BR * 2) : tr4(base + fa_at[(FR + i) % NA]);
 			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 		}
 	};
-	auto read_b = [&](int j, uint32_t stage) -> T8 {
-		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(stage + fb_at[0] + (pair_at(j / 2) + (j & 1) * 4) * AK * 2);
+	auto read_b = [&](int half, int j, uint32_t unit) -> T8 {
+		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(unit + fb_at[half] + (pair_at(j / 2) + (j & 1) * 4) * AK * 2);
 		else {
-			const uint32_t at = stage + fb_at[B_T ? 0 : j / 2] + (j & 1) * 8;
+			const uint32_t at = unit + half * 32 * BC * 2 + fb_at[(j / 2) % NB] + (j & 1) * 8;
 			const s4 lo = tr4(at), hi = tr4(at + 4 * BC * 2);
 			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 		}
@@ -387,57 +383,58 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 #pragma unroll
 		for (int j = 0; j < FC; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
 	constexpr int AHEAD = A_RING - 1;
-	static_assert(FR % A_RING == 0, "a stage begins at the ring's first fragment");
 	T8 fa[A_RING], fb[2][FC];
-	uint32_t read_slot = 0;
-	// The matrix instructions of one stage (B fragments `cur`).  One wavefront has the SIMD to itself, so whatever else is to be issued stands between two matrix instructions, a little
-	// at a time: the loads of the stage that takes the slot the last one left, the reads of what comes next.  The barrier (the next stage has arrived for every wavefront, the
-	// last one's slot has been read by all: its last fragment went into the matrix instructions before) stands behind the first few of them.
-	auto stage_step = [&](auto cur_c) {
-		constexpr int cur = decltype(cur_c)::value, nxt = cur ^ 1;
-		const uint32_t here = lds0 + read_slot * STAGE;
-		read_slot = read_slot + 1 == STAGES ? 0 : read_slot + 1;
-		const uint32_t next = lds0 + read_slot * STAGE;
+	uint32_t a_here = lds0, b_here = lds0 + UNITS_A * LA::BYTES;
+	// The matrix instructions of one half of a unit.  One wavefront has the SIMD to itself, so whatever else is to be issued stands between two matrix instructions, a little at a
+	// time.  Half 0: the barrier behind its first instructions says that every wavefront is through with the unit of A before this one, whose place the loads of the unit after the
+	// next take.  Half 1: the barrier behind its first row of fragments says that every wavefront has this unit's B in registers and that the next units have arrived.
+	auto half_step = [&](auto half_c, uint32_t a_next, uint32_t b_next) {
+		constexpr int half = decltype(half_c)::value, Q = FC / 4;
 #pragma unroll
 		for (int i = 0; i < FR; ++i) {
-			constexpr int Q = FC / 4; // a quarter of the row's matrix instructions
 #pragma unroll
 			for (int j = 0; j < FC; ++j) {
-				mfma_in_place(fb[cur][j], fa[i % A_RING], acc[i][j]);
-				if (j == 0) fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(i + AHEAD, here) : read_a(i + AHEAD - FR, next);
-				if (i == 0 && j == Q) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * D) : "memory");
-				if (j == 2 * Q) {
-#pragma unroll
-					for (int q = i * D / FR; q < (i + 1) * D / FR; ++q) load(q);
+				mfma_in_place(fb[half][j], fa[i % A_RING], acc[i][j]);
+				if (j == (half == 1 && i == 0 ? FC - 1 : 0)) {
+					if (half == 1 && i == 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LA::LOADS) : "memory");
+					fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(half, i + AHEAD, a_here) : half == 0 ? read_a(1, i + AHEAD - FR, a_here) : read_a(0, i + AHEAD - FR, a_next);
 				}
-				if (j == 3 * Q) {
+				if (half == 0 && i == 0 && j == Q) asm volatile("s_barrier" ::: "memory");
+				if (j == 2 * Q && (half == 0 || i > 0)) { // (half 1: the loads begin with the second row)
 #pragma unroll
-					for (int k = i * FC / FR; k < (i + 1) * FC / FR; ++k) fb[nxt][k] = read_b(k, next);
+					for (int q = 0; q < (half == 0 ? LA::LOADS / FR : LB::LOADS / FR); ++q) { if (half == 0) load_a(i * (LA::LOADS / FR) + q); else load_b((i - 1) * (LB::LOADS / FR) + q); }
+				}
+				if (half == 1 && i == FR - 1 && j == FC - 1) {
+#pragma unroll
+					for (int q = 0; q < LB::LOADS / FR; ++q) load_b((FR - 1) * (LB::LOADS / FR) + q);
+				}
+				if (j == 3 * Q) { // the next half's B fragments (half 1: they are the next unit's, from the second row on)
+#pragma unroll
+					for (int k = 0; k < FC; ++k) {
+						constexpr int PER = FC / FR ? FC / FR : 1;
+						if (half == 0 ? k / PER == i : i > 0 && (k / PER == i - 1 || (i == FR - 1 && k / PER >= FR - 1))) fb[half ^ 1][k] = half == 0 ? read_b(1, k, b_here) : read_b(0, k, b_next);
+					}
 				}
 				__builtin_amdgcn_sched_barrier(0);
 			}
 		}
-		next_chunk();
+		if (half == 0) ca.next(start_a, g.steps); else cb.next(start_b, g.steps);
 	};
 	if (t_begin < t_end) {
-		const uint32_t first = t_begin / chunks_per_segment;
-		at_chunk(first, (t_begin - first * chunks_per_segment) * AK);
-		limit_chunk();
-		lds_load = lds0;
+		auto all_a = [&]() { for (int q = 0; q < LA::LOADS; ++q) load_a(q); ca.next(start_a, g.steps); };
+		auto all_b = [&]() { for (int q = 0; q < LB::LOADS; ++q) load_b(q); cb.next(start_b, g.steps); };
+		all_a(); all_b(); all_a(); all_b();
+		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LA::LOADS + LB::LOADS) : "memory");
 #pragma unroll
-		for (int k = 0; k < STAGES - 1; ++k) {
+		for (int i = 0; i < AHEAD; ++i) fa[i] = read_a(0, i, a_here);
 #pragma unroll
-			for (int q = 0; q < D; ++q) load(q);
-			next_chunk();
-		}
-		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * D) : "memory");
-#pragma unroll
-		for (int i = 0; i < AHEAD; ++i) fa[i] = read_a(i, lds0);
-#pragma unroll
-		for (int j = 0; j < FC; ++j) fb[0][j] = read_b(j, lds0);
-		for (uint32_t t = t_begin; t < t_end; t += 2) { // (an odd last stage is followed by one of zeros)
-			stage_step(std::integral_constant<int, 0>());
-			stage_step(std::integral_constant<int, 1>());
+		for (int j = 0; j < FC; ++j) fb[0][j] = read_b(0, j, b_here);
+		for (uint32_t t = t_begin; t < t_end; ++t) {
+			const uint32_t a_next = a_here == lds0 + (UNITS_A - 1) * LA::BYTES ? lds0 : a_here + LA::BYTES;
+			const uint32_t b_next = b_here == lds0 + UNITS_A * LA::BYTES ? b_here + LB::BYTES : lds0 + UNITS_A * LA::BYTES;
+			half_step(std::integral_constant<int, 0>(), a_next, b_next);
+			half_step(std::integral_constant<int, 1>(), a_next, b_next);
+			a_here = a_next; b_here = b_next;
 		}
 		settle(acc);
 		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is under way to LDS any more
