@@ -71,6 +71,17 @@ __device__ inline void store8(T* p, T8 v, int n) {
 
 // ---- activations: values and derivatives in 32 bits.  1 / (1 + e^-z) through v_exp_f32 / v_rcp_f32 (1 ulp each): far below the 16-bit rounding of the result
 __device__ inline float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// the normal distribution function and e^(-z^2/2).  Lower tail at -|z|: t Q(t) e^(-z^2/2) with t = 1 / (1 + 0.35 |z|), Q = a least-squares fit (reweighted towards the largest relative
+// error) of 0.5 erfcx(|z| / sqrt 2) / t over |z| < 14.5: 3.2e-8 relative, 2.8e-7 in 32 bits, in both tails; erfcf costs the epilogue three times as much
+__device__ inline float normal_cdf(float z, float& e) {
+	const float u = fabsf(z), t = __builtin_amdgcn_rcpf(fmaf(0.35f, u, 1.f));
+	e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+	float q = -0.029158229008316994f;
+	q = fmaf(q, t, 0.1440325528383255f); q = fmaf(q, t, -0.25584226846694946f); q = fmaf(q, t, 0.1593232899904251f); q = fmaf(q, t, -0.02321472205221653f);
+	q = fmaf(q, t, 0.10555345565080643f); q = fmaf(q, t, 0.11982106417417526f); q = fmaf(q, t, 0.13986355066299438f); q = fmaf(q, t, 0.139621302485466f);
+	q *= t * e;
+	return z < 0.f ? q : 1.f - q;
+}
 __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 values)
 #define EACH for (int e = 0; e < 8; ++e)
 	switch (act) {
@@ -78,7 +89,7 @@ __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 va
 		case NGP_ACT_LOGISTIC: EACH z[e] = logistic(z[e]); break;
 		case NGP_ACT_EXPONENTIAL: EACH z[e] = __expf(z[e]); break;
 		case NGP_ACT_SILU: EACH z[e] *= logistic(z[e]); break;
-		case NGP_ACT_GELU: EACH z[e] = 0.5f * z[e] * erfcf(-0.70710678f * z[e]); break;
+		case NGP_ACT_GELU: EACH { float x; z[e] *= normal_cdf(z[e], x); } break;
 		default: break;
 	}
 }
@@ -88,7 +99,7 @@ __device__ inline void act_value_slope8(int act, const float z[8], float value[8
 		case NGP_ACT_LOGISTIC: EACH { const float p = logistic(z[e]); value[e] = p; slope[e] = p * (1.f - p); } break;
 		case NGP_ACT_EXPONENTIAL: EACH value[e] = slope[e] = __expf(z[e]); break;
 		case NGP_ACT_SILU: EACH { const float p = logistic(z[e]); value[e] = z[e] * p; slope[e] = p * (1.f + z[e] * (1.f - p)); } break;
-		case NGP_ACT_GELU: EACH { const float c = 0.5f * erfcf(-0.70710678f * z[e]); value[e] = z[e] * c; slope[e] = c + z[e] * 0.39894228f * __expf(-0.5f * z[e] * z[e]); } break;
+		case NGP_ACT_GELU: EACH { float x; const float c = normal_cdf(z[e], x); value[e] = z[e] * c; slope[e] = fmaf(z[e] * 0.39894228f, x, c); } break;
 		default: EACH { value[e] = z[e]; slope[e] = 1.f; } break;
 	}
 }
@@ -124,7 +135,7 @@ template <int EXTENT, bool T_CONTIG, bool IS_B> struct Tile {
 	}
 };
 
-enum { EPI_LINEAR, EPI_GATED, EPI_STORE, EPI_PARTIAL };
+enum { EPI_LINEAR, EPI_GATED, EPI_STORE, EPI_PARTIAL, EPI_PARTIAL2 /* of both projections */ };
 struct GemmArgs {
 	const T* a; const T* b[2]; uint64_t lda, ldb;
 	uint32_t rows, cols, steps;      // C is rows x cols; the sum runs over `segments` pieces of `steps`
@@ -137,12 +148,15 @@ struct GemmArgs {
 };
 __host__ __device__ inline uint32_t up8(uint32_t v) { return (v + 7) & ~7u; }
 
-// What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C
-template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8]) {
+// What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C.  Biases and the residual come as values: a caller
+// with several rows loads them ahead.
+template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual) {
 	T8 o, s;
-	if constexpr (EPI == EPI_PARTIAL) {
-		float* q = g.partial + (((uint64_t)split * g.problems + problem) * g.rows + r) * up8(g.cols) + c; // (lines are padded to 8: always whole)
+	if constexpr (EPI == EPI_PARTIAL || EPI == EPI_PARTIAL2) {
+		const uint32_t parts = EPI == EPI_PARTIAL2 ? 2 : g.problems;
+		float* q = g.partial + (((uint64_t)split * parts + problem) * g.rows + r) * up8(g.cols) + c; // (lines are padded to 8: always whole)
 		*(f4v*)q = f4v{z[0], z[1], z[2], z[3]}; *(f4v*)(q + 4) = f4v{z[4], z[5], z[6], z[7]};
+		if constexpr (EPI == EPI_PARTIAL2) { q += (uint64_t)g.rows * up8(g.cols); *(f4v*)q = f4v{u[0], u[1], u[2], u[3]}; *(f4v*)(q + 4) = f4v{u[4], u[5], u[6], u[7]}; }
 		return;
 	}
 	if constexpr (EPI == EPI_STORE) {
@@ -150,19 +164,21 @@ template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t 
 		store8(g.c[problem] + (uint64_t)r * g.ldc + c, o, n);
 		return;
 	}
-	if (g.bias[0]) { const T8 b = load8(g.bias[0] + c, n); EACH z[e] += (float)b[e]; }
+	EACH z[e] += (float)bias0[e];
 	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n); }
 	act_value8(g.act, z);
 	if constexpr (EPI == EPI_LINEAR) {
-		if (g.residual) { const T8 v = load8(g.residual + (uint64_t)r * g.ld_residual + c, n); EACH z[e] += (float)v[e]; }
-		EACH o[e] = (T)z[e];
+		EACH o[e] = (T)(z[e] + (float)residual[e]);
 	} else {
-		if (g.bias[1]) { const T8 b = load8(g.bias[1] + c, n); EACH u[e] += (float)b[e]; }
+		EACH u[e] += (float)bias1[e];
 		if (g.pre[1]) { EACH s[e] = (T)u[e]; store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n); }
 		EACH o[e] = (T)(z[e] * u[e]);
 	}
 	store8(g.c[0] + (uint64_t)r * g.ldc + c, o, n);
 }
+template <int EPI> constexpr bool GATED_TILE = EPI == EPI_GATED || EPI == EPI_PARTIAL2; // the tile's columns are gate and up outputs
+template <int EPI> __device__ inline T8 bias8(const GemmArgs& g, int k, uint32_t c, int n) { return (EPI == EPI_LINEAR || EPI == EPI_GATED) && g.bias[k] && n > 0 ? load8(g.bias[k] + c, n) : T8{}; }
+template <int EPI> __device__ inline T8 residual8(const GemmArgs& g, uint32_t r, uint32_t c, int n) { return EPI == EPI_LINEAR && g.residual && n > 0 ? load8(g.residual + (uint64_t)r * g.ld_residual + c, n) : T8{}; }
 
 // C tile BR x BC by WR x WC wavefronts; each owns (BR / WR) x (BC / WC) as 16 x 16 fragments (matrix instruction 16x16x32, C^T: a lane holds one row of C and 4 columns
 // of each fragment).  EPI_GATED: the tile's columns are BC / 2 gate outputs and the same BC / 2 up outputs, every wavefront owns both of its columns.
@@ -170,8 +186,8 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
 __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	typedef Tile<BR, A_T, false> TA; typedef Tile<BC, B_T, true> TB;
 	constexpr int THREADS = 64 * WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, NA = TA::N_SLOTS / THREADS, NB = TB::N_SLOTS / THREADS;
-	constexpr int OUT = EPI == EPI_GATED ? BC / 2 : BC; // columns of C per tile
-	static_assert(FC % (EPI == EPI_GATED ? 4 : 2) == 0, "pairs of fragments");
+	constexpr int OUT = GATED_TILE<EPI> ? BC / 2 : BC; // columns of C per tile
+	static_assert(FC % (GATED_TILE<EPI> ? 4 : 2) == 0, "pairs of fragments");
 	__shared__ __attribute__((aligned(16))) T lds_a[TA::ELEMS];
 	__shared__ __attribute__((aligned(16))) T lds_b[TB::ELEMS];
 	const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
@@ -182,7 +198,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	const uint32_t chunks_per_segment = (g.steps + TK - 1) / TK, n_chunks = chunks_per_segment * g.segments;
 	const uint32_t t_begin = split * g.chunks_per_split, t_end = min(n_chunks, t_begin + g.chunks_per_split);
 	auto pair_at = [&](int p) -> int { // first column (in the B tile) of fragment pair p of this wavefront
-		if (EPI == EPI_GATED) return (p >= FC / 4 ? OUT : 0) + (int)wc * (OUT / WC) + (p % (FC / 4)) * 32;
+		if (GATED_TILE<EPI>) return (p >= FC / 4 ? OUT : 0) + (int)wc * (OUT / WC) + (p % (FC / 4)) * 32;
 		return (int)wc * (BC / WC) + p * 32;
 	};
 	f4v acc[FR][FC];
@@ -205,7 +221,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 		for (int q = 0; q < NB; ++q) {
 			const int slot = q * THREADS + tid, line = slot / TB::SLOTS, chunk = TB::source(line, slot % TB::SLOTS);
 			if (B_T) {
-				const uint32_t which = EPI == EPI_GATED && line >= OUT, col = c0 + line - which * OUT;
+				const uint32_t which = GATED_TILE<EPI> && line >= OUT, col = c0 + line - which * OUT;
 				rb[q] = load8(g.b[which] + (uint64_t)col * g.ldb + t0 + chunk * 8, col < g.cols ? left - chunk * 8 : 0);
 			} else { const uint32_t c = c0 + chunk * 8; rb[q] = load8(g.b[seg] + (uint64_t)(t0 + line) * g.ldb + c, line < left ? (int)g.cols - (int)c : 0); }
 		}
@@ -238,13 +254,13 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 		const uint32_t r = r0 + wr * (BR / WR) + i * 16 + li;
 		if (r >= g.rows) continue;
 #pragma unroll
-		for (int p = 0; p < (EPI == EPI_GATED ? FC / 4 : FC / 2); ++p) {
+		for (int p = 0; p < (GATED_TILE<EPI> ? FC / 4 : FC / 2); ++p) {
 			const uint32_t c = c0 + pair_at(p) + gq * 8;
 			if (c >= g.cols) continue;
 			const int n = (int)min(8u, g.cols - c);
 			float z[8], u[8];
-			EACH { z[e] = acc[i][2 * p + e / 4][e & 3]; u[e] = EPI == EPI_GATED ? acc[i][(EPI == EPI_GATED ? FC / 2 : 0) + 2 * p + e / 4][e & 3] : 0.f; }
-			epilogue8<EPI>(g, problem, split, r, c, n, z, u);
+			EACH { z[e] = acc[i][2 * p + e / 4][e & 3]; u[e] = GATED_TILE<EPI> ? acc[i][(GATED_TILE<EPI> ? FC / 2 : 0) + 2 * p + e / 4][e & 3] : 0.f; }
+			epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
 		}
 	}
 }
@@ -256,26 +272,25 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 // products is what LDS can deliver beside the incoming units (96 of the 128 bytes a clock; with 8 wavefronts of 128 x 64 it would be all of them).
 constexpr int AK = 64, UNITS_A = 3, UNITS_B = 2, A_RING = 4;
 typedef int i4v __attribute__((ext_vector_type(4)));
-template <int EXTENT, bool T_CONTIG, bool IS_B, int WAVES> struct Async {
+template <int EXTENT, bool T_CONTIG, int WAVES> struct Async {
 	static constexpr int SLOTS = T_CONTIG ? AK / 8 : EXTENT / 8, BYTES = EXTENT * AK * 2, LOADS = BYTES / 1024 / WAVES;
 	static_assert(LOADS >= 2, "a wavefront has something to load");
-	uint32_t at[LOADS], step[2]; // byte offset from the tile's first element; first step of the chunk (T_CONTIG: of even and odd loads)
+	uint32_t at[LOADS], step; // byte offset from the tile's first element; first step of the chunk (T_CONTIG: the same for every load)
 	__device__ static int source(int line, int slot) { // chunk that lies in a line's slot (its own inverse)
-		if (T_CONTIG) return IS_B ? slot ^ ((line & 3) | ((line >> 1) & 4)) : slot ^ (line & 7);
-		if (IS_B) return slot ^ ((line & (EXTENT >= 128 ? 3 : 1)) << 2);
-		return slot ^ ((line & (EXTENT >= 128 ? 7 : 3)) << 1);
+		if (T_CONTIG) return slot ^ (line & 7);                         // 8 lanes read 8 lines' 16-byte chunks
+		return slot ^ (((line & 3) | ((line >> 1) & 4)) << 1);          // 32 lanes read 32 bytes of lines 0..3, 8..11 (4..7, 12..15)
 	}
 	__device__ void setup(uint32_t lane, uint32_t wave, uint64_t ld, uint32_t skip_lines /* wave-uniform: lines in front of this wavefront's that belong to another matrix */) {
 #pragma unroll
 		for (int q = 0; q < LOADS; ++q) {
 			const int slot = (wave * LOADS + q) * 64 + lane, line = slot / SLOTS, chunk = source(line, slot % SLOTS);
-			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step[q & 1] = chunk * 8;
+			at[q] = (uint32_t)((line - (int)skip_lines) * ld * 2 + chunk * 16); step = chunk * 8;
 		}
 	}
 	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on; chunks behind the last of the `left` steps are out of range: zero.  (M0 lives inside this block alone: the
 	// compiler sets it anew wherever it needs it)
 	__device__ void load(int q, i4v rsrc, uint32_t lds, int left) const {
-		const uint32_t off = T_CONTIG && (int)step[q & 1] >= left ? 0x80000000u : at[q];
+		const uint32_t off = T_CONTIG && (int)step >= left ? 0x80000000u : at[q];
 		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
 	}
 };
@@ -314,12 +329,12 @@ template <bool T_CONTIG, int UNITS, int BYTES> struct Cursor {
 };
 template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
 __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(GemmArgs g) {
-	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = EPI == EPI_GATED ? BC / 2 : BC;
-	typedef Async<BR, A_T, false, WAVES> LA; typedef Async<BC, B_T, true, WAVES> LB;
+	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = GATED_TILE<EPI> ? BC / 2 : BC;
+	typedef Async<BR, A_T, WAVES> LA; typedef Async<BC, B_T, WAVES> LB;
 	constexpr int LDS = UNITS_A * LA::BYTES + UNITS_B * LB::BYTES;
 	constexpr int STRIP = BC / WC + 4, PASS = FR > 4 ? 4 : FR; // epilogue: floats per row of a wavefront's strip of LDS, fragment rows in it
 	static_assert(WAVES * PASS * 16 * STRIP * 4 <= LDS && FR % PASS == 0, "the epilogue's strips fit");
-	static_assert(FC % (EPI == EPI_GATED ? 4 : 2) == 0 && FR % A_RING == 0 && LA::LOADS % FR == 0 && LB::LOADS % FR == 0, "");
+	static_assert(FC % (GATED_TILE<EPI> ? 4 : 2) == 0 && FR % A_RING == 0 && LA::LOADS % FR == 0 && LB::LOADS % FR == 0, "");
 	__shared__ __attribute__((aligned(1024))) char lds[LDS];
 	const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
@@ -328,7 +343,7 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	const uint32_t r0 = tr * BR, c0 = tc * OUT, problem = blockIdx.y, split = blockIdx.z;
 	const uint32_t units_per_segment = (g.steps + AK - 1) / AK, n_units = units_per_segment * g.segments;
 	const uint32_t t_begin = min(n_units, split * g.chunks_per_split), t_end = min(n_units, t_begin + g.chunks_per_split);
-	const uint32_t which = EPI == EPI_GATED && wave * LB::LOADS * 8 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
+	const uint32_t which = GATED_TILE<EPI> && wave * LB::LOADS * 8 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
 	LA la; LB lb;
 	la.setup(lane, wave, g.lda, 0); lb.setup(lane, wave, g.ldb, which * OUT);
 	auto start_a = [&](uint32_t seg) -> const T* { return uniform(g.a + problem * g.a_problem + seg * g.a_segment + (A_T ? (uint64_t)r0 * g.lda : (uint64_t)r0)); };
@@ -349,30 +364,27 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	auto load_b = [&](int q) { lb.load(q, resource(cb.p, cb.rec), cb.lds + (wave * LB::LOADS + q) * 1024, cb.left); };
 	// where the lane finds its fragments in a unit: an address for each half and constants for operands along t; for the others the XOR leaves one a fragment row (A) or pair (B)
 	typedef __attribute__((address_space(3))) const T8 lds_T8;
-	auto pair_at = [&](int p) -> int { return EPI == EPI_GATED ? (p >= FC / 4 ? OUT : 0) + (p % (FC / 4)) * 32 : p * 32; }; // column (in the B tile) of fragment pair p behind the wavefront's first one
-	const uint32_t col0 = wc * (EPI == EPI_GATED ? OUT / WC : BC / WC), row0 = wr * (BR / WR), l4 = li >> 2;
-	constexpr bool PAIRED = FR == 8; // A across t: the second four steps of fragment i lie where fragment i ^ 4 has its first, four lines further
-	constexpr int NA = A_T ? 2 : PAIRED ? FR : 2 * FR, NB = B_T ? 2 : FC / 2;
+	auto frag_at = [&](int j) -> int { return GATED_TILE<EPI> ? (j >= FC / 2 ? OUT : 0) + (j % (FC / 2)) * 16 : j * 16; }; // column (in the B tile) of fragment j behind the wavefront's first one
+	const uint32_t col0 = wc * (GATED_TILE<EPI> ? OUT / WC : BC / WC), row0 = wr * (BR / WR), l4 = li >> 2, xr = l4 | ((gq & 1) << 2);
+	constexpr int NA = A_T ? 2 : FR, NB = B_T ? 2 : FC;
 	uint32_t fa_at[NA], fb_at[NB];
 #pragma unroll
-	for (int k = 0; k < NA; ++k) fa_at[k] = A_T ? (row0 + li) * AK * 2 + (((k * 4) + gq) ^ (li & 7)) * 16
-		: (gq * 8 + (k / FR) * 4 + l4) * BR * 2 + ((row0 / 16 + k % FR) ^ ((k / FR) * 4 + l4)) * 32 + (li & 3) * 8;
+	for (int k = 0; k < NA; ++k) fa_at[k] = A_T ? (row0 + li) * AK * 2 + (((k * 4) + gq) ^ (li & 7)) * 16 : (gq * 8 + l4) * BR * 2 + ((row0 / 16 + k) ^ xr) * 32 + (li & 3) * 8;
 #pragma unroll
-	for (int k = 0; k < NB; ++k) fb_at[k] = B_T ? (col0 + l4 * 8 + (li & 3)) * AK * 2 + (((k * 4) + gq) ^ ((li & 3) | ((l4 & 1) << 2))) * 16
-		: (gq * 8 + l4) * BC * 2 + ((col0 / 32 + k) ^ l4) * 64 + (li & 3) * 16;
+	for (int k = 0; k < NB; ++k) fb_at[k] = B_T ? (col0 + li) * AK * 2 + (((k * 4) + gq) ^ (li & 7)) * 16 : (gq * 8 + l4) * BC * 2 + (((col0 + frag_at(k)) / 16) ^ xr) * 32 + (li & 3) * 8;
 	auto tr4 = [](uint32_t at) -> s4 { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)at); };
 	auto read_a = [&](int half, int i, uint32_t unit) -> T8 {
 		if constexpr (A_T) return *(lds_T8*)(uintptr_t)(unit + fa_at[half] + i * 16 * AK * 2);
 		else {
-			const uint32_t base = unit + half * 32 * BR * 2;
-			const s4 lo = tr4(base + fa_at[i % NA]), hi = PAIRED ? tr4(base + fa_at[(i ^ 4) % NA] + 4 * BR * 2) : tr4(base + fa_at[(FR + i) % NA]);
+			const uint32_t at = unit + fa_at[i % NA] + half * 32 * BR * 2;
+			const s4 lo = tr4(at), hi = tr4(at + 4 * BR * 2);
 			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 		}
 	};
 	auto read_b = [&](int half, int j, uint32_t unit) -> T8 {
-		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(unit + fb_at[half] + (pair_at(j / 2) + (j & 1) * 4) * AK * 2);
+		if constexpr (B_T) return *(lds_T8*)(uintptr_t)(unit + fb_at[half] + frag_at(j) * AK * 2);
 		else {
-			const uint32_t at = unit + half * 32 * BC * 2 + fb_at[(j / 2) % NB] + (j & 1) * 8;
+			const uint32_t at = unit + fb_at[j % NB] + half * 32 * BC * 2;
 			const s4 lo = tr4(at), hi = tr4(at + 4 * BC * 2);
 			return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 		}
@@ -439,25 +451,34 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 		settle(acc);
 		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is under way to LDS any more
 	}
-	// epilogue through the wavefront's own strip of LDS: 8 consecutive columns a lane, whole lines a store
+	// epilogue through the wavefront's own strip of LDS: 8 consecutive columns a lane, whole lines a store, the residual of 8 rows on its way at a time
 	float* strip = (float*)lds + wave * PASS * 16 * STRIP;
-	constexpr int LANES = OUT / WC / 8, ROWS = 64 / LANES; // lanes a row, rows at a time
+	constexpr int LANES = OUT / WC / 8, ROWS = 64 / LANES, AT_ONCE = PASS * 16 / ROWS < 8 ? PASS * 16 / ROWS : 8; // lanes a row, rows at a time
 	const uint32_t er = lane / LANES, ec = (lane % LANES) * 8, c = c0 + wc * (OUT / WC) + ec;
+	const int n = (int)min(8u, g.cols > c ? g.cols - c : 0u);
+	const T8 bias0 = bias8<EPI>(g, 0, c, n), bias1 = bias8<EPI>(g, 1, c, n);
 #pragma unroll
 	for (int pass = 0; pass < FR / PASS; ++pass) {
 #pragma unroll
 		for (int i = 0; i < PASS; ++i)
 #pragma unroll
-			for (int j = 0; j < FC; ++j) *(f4v*)(strip + (i * 16 + li) * STRIP + (j / 2) * 32 + gq * 8 + (j & 1) * 4) = acc[pass * PASS + i][j];
+			for (int j = 0; j < FC; ++j) *(f4v*)(strip + (i * 16 + li) * STRIP + j * 16 + gq * 4) = acc[pass * PASS + i][j];
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the strip is this wavefront's alone)
-#pragma unroll 2
-		for (int k = 0; k < PASS * 16; k += ROWS) {
-			const uint32_t r = r0 + wr * (BR / WR) + pass * PASS * 16 + k + er;
-			float z[8], u[8];
-			const float* p = strip + (k + er) * STRIP + ec;
-			*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
-			if constexpr (EPI == EPI_GATED) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
-			if (r < g.rows && c < g.cols) epilogue8<EPI>(g, problem, split, r, c, (int)min(8u, g.cols - c), z, u);
+		const uint32_t r_pass = r0 + wr * (BR / WR) + pass * PASS * 16 + er;
+#pragma unroll 1
+		for (int k = 0; k < PASS * 16; k += ROWS * AT_ONCE) {
+			T8 residual[AT_ONCE];
+#pragma unroll
+			for (int q = 0; q < AT_ONCE; ++q) residual[q] = residual8<EPI>(g, r_pass + k + q * ROWS, c, r_pass + k + q * ROWS < g.rows ? n : 0);
+#pragma unroll
+			for (int q = 0; q < AT_ONCE; ++q) {
+				const uint32_t r = r_pass + k + q * ROWS;
+				float z[8], u[8];
+				const float* p = strip + (k + q * ROWS + er) * STRIP + ec;
+				*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
+				if constexpr (GATED_TILE<EPI>) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
+				if (r < g.rows && n > 0) epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias0, bias1, residual[q]);
+			}
 		}
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
