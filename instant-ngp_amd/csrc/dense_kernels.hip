@@ -484,6 +484,76 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	}
 }
 
+// ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
+// straight from memory to registers as the matrix instruction's fragments, U loads on the way at a time; the samples (MT x 16 rows, the last one repeated where there are fewer)
+// come out of the caches.  SLICES wavefronts share the sum and add up in LDS, in their order.
+template <int MT, bool GATED> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
+	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4, EPI = GATED ? EPI_GATED : EPI_LINEAR;
+	__shared__ float sums[8][P][MT * 16][20]; // [wavefront][projection][row][output]
+	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gq = lane >> 4, li = lane & 15;
+	const uint32_t slice = wave % slices, tile = blockIdx.x * (8 / slices) + wave / slices, c0 = tile * 16;
+	const uint32_t t_begin = min(g.steps, slice * steps_per_slice), t_end = min(g.steps, t_begin + steps_per_slice);
+	const uint32_t col = min(c0 + li, g.cols - 1); // (outputs behind the last one repeat it and are dropped)
+	const T* w[P]; const T* x[MT];
+#pragma unroll
+	for (int p = 0; p < P; ++p) w[p] = g.b[p] + (uint64_t)col * g.ldb + gq * 8;
+#pragma unroll
+	for (int m = 0; m < MT; ++m) x[m] = g.a + (uint64_t)min(m * 16 + li, g.rows - 1) * g.lda + gq * 8;
+	f4v acc[P][MT];
+#pragma unroll
+	for (int p = 0; p < P; ++p)
+#pragma unroll
+		for (int m = 0; m < MT; ++m) acc[p][m] = f4v{0.f, 0.f, 0.f, 0.f};
+	uint32_t t = t_begin;
+	for (; t + U * 32 <= t_end; t += U * 32) {
+		T8 fw[P][U], fx[MT][U];
+#pragma unroll
+		for (int u = 0; u < U; ++u)
+#pragma unroll
+			for (int p = 0; p < P; ++p) fw[p][u] = load8(w[p] + t + u * 32);
+#pragma unroll
+		for (int u = 0; u < U; ++u)
+#pragma unroll
+			for (int m = 0; m < MT; ++m) fx[m][u] = load8(x[m] + t + u * 32);
+#pragma unroll
+		for (int u = 0; u < U; ++u)
+#pragma unroll
+			for (int p = 0; p < P; ++p)
+#pragma unroll
+				for (int m = 0; m < MT; ++m) acc[p][m] = mfma(fw[p][u], fx[m][u], acc[p][m]);
+	}
+	for (; t < t_end; t += 32) { // what is left, the last chunk in part
+		const int n = (int)(t_end - t) - (int)gq * 8;
+		T8 fw[P], fx[MT];
+#pragma unroll
+		for (int p = 0; p < P; ++p) fw[p] = load8(w[p] + t, n);
+#pragma unroll
+		for (int m = 0; m < MT; ++m) fx[m] = load8(x[m] + t, n);
+#pragma unroll
+		for (int p = 0; p < P; ++p)
+#pragma unroll
+			for (int m = 0; m < MT; ++m) acc[p][m] = mfma(fw[p], fx[m], acc[p][m]);
+	}
+#pragma unroll
+	for (int p = 0; p < P; ++p)
+#pragma unroll
+		for (int m = 0; m < MT; ++m) *(f4v*)&sums[wave][p][m * 16 + li][gq * 4] = acc[p][m];
+	__syncthreads();
+	// 8 outputs a thread: tile, row, half
+	const uint32_t tiles = 8 / slices;
+	for (uint32_t id = threadIdx.x; id < tiles * MT * 32; id += 512) {
+		const uint32_t half = id & 1, r = (id >> 1) % (MT * 16), k = id / (MT * 32), c = (blockIdx.x * tiles + k) * 16 + half * 8;
+		if (r >= g.rows || c >= g.cols) continue;
+		const int n = (int)min(8u, g.cols - c);
+		float z[8] = {}, u[8] = {};
+		for (uint32_t q = 0; q < slices; ++q) {
+			EACH z[e] += sums[k * slices + q][0][r][half * 8 + e];
+			if (GATED) EACH u[e] += sums[k * slices + q][P - 1][r][half * 8 + e];
+		}
+		epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+	}
+}
+
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
 // one line per block of rows, before the rounding).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
@@ -548,38 +618,60 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float* partial, uint32_
 		if (out) out[c] = (T)t;
 	}
 }
-// C = sum over the splits, in their order, rounded once
-__global__ __launch_bounds__(256) void k_join_splits(const float* partial, uint32_t splits, uint32_t problems, uint32_t rows, uint32_t cols, T* c0, T* c1, uint64_t ldc) {
-	const uint32_t cc = up8(cols) / 8, problem = blockIdx.y;
+// the splits' sums in their order, then the product's own epilogue (EPI_GATED: partial sums of both projections)
+template <int EPI> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs g) {
+	const uint32_t cc = up8(g.cols) / 8, problem = blockIdx.y, parts = EPI == EPI_GATED ? 2 : g.problems;
 	const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-	if (id >= (uint64_t)rows * cc) return;
+	if (id >= (uint64_t)g.rows * cc) return;
 	const uint32_t r = (uint32_t)(id / cc), c = (uint32_t)(id % cc) * 8;
-	f4v s0{}, s1{};
+	const uint64_t part = (uint64_t)g.rows * cc * 8;
+	const int n = (int)min(8u, g.cols - c);
+	const T8 bias0 = bias8<EPI>(g, 0, c, n), bias1 = bias8<EPI>(g, 1, c, n), residual = residual8<EPI>(g, r, c, n);
+	float z[8] = {}, u[8] = {};
+	const float* p = g.partial + problem * part + (uint64_t)r * cc * 8 + c;
 #pragma unroll 4
-	for (uint32_t k = 0; k < splits; ++k) {
-		const float* p = partial + (((uint64_t)k * problems + problem) * rows + r) * (cc * 8) + c;
-		s0 += *(const f4v*)p; s1 += *(const f4v*)(p + 4);
-	}
-	T8 o;
+	for (uint32_t k = 0; k < g.splits; ++k, p += parts * part) {
+		const f4v a = *(const f4v*)p, b = *(const f4v*)(p + 4);
 #pragma unroll
-	for (int e = 0; e < 4; ++e) { o[e] = (T)s0[e]; o[e + 4] = (T)s1[e]; }
-	store8((problem ? c1 : c0) + (uint64_t)r * ldc + c, o, (int)min(8u, cols - c));
+		for (int e = 0; e < 4; ++e) { z[e] += a[e]; z[e + 4] += b[e]; }
+		if constexpr (EPI == EPI_GATED) {
+			const f4v d = *(const f4v*)(p + part), f = *(const f4v*)(p + part + 4);
+#pragma unroll
+			for (int e = 0; e < 4; ++e) { u[e] += d[e]; u[e + 4] += f[e]; }
+		}
+	}
+	epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual);
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
 // `wholes`: both operands come in whole 16-byte pieces
-template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes) {
-	constexpr int K = EPI == EPI_GATED ? 2 : 1; // weight columns per column of C
-	if (!wholes) {
-		g.chunks_per_split = div_up(div_up(g.steps, TK) * g.segments, g.splits);
-		hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 128) * div_up(g.cols, 128 / K), g.problems, g.splits), dim3(256), 0, s, g);
-		return;
-	}
-	g.chunks_per_split = div_up(div_up(g.steps, AK) * g.segments, g.splits);
-	const uint64_t large = (uint64_t)div_up(g.rows, 256) * div_up(g.cols, 256 / K) * g.problems * g.splits;
-	if (large >= 200) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 256) * div_up(g.cols, 256 / K), g.problems, g.splits), dim3(256), 0, s, g);
-	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI>), dim3(div_up(g.rows, 128) * div_up(g.cols, 128 / K), g.problems, g.splits), dim3(256), 0, s, g);
+template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs& g, bool wholes, bool large) {
+	constexpr int K = GATED_TILE<EPI> ? 2 : 1; // weight columns per column of C
+	const uint32_t tile = large ? 256 : 128;
+	const dim3 grid(div_up(g.rows, tile) * div_up(g.cols, tile / K), g.problems, g.splits);
+	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
+	static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
+	if (!wholes) hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
+	else if (large) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
+	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
+}
+template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
+	const DenseSplit d = dense_split(g.rows, g.cols, g.steps, g.segments, EPI == EPI_GATED ? 2 : g.problems);
+	g.splits = 1;
+	if (d.splits > 1) {
+		g.splits = d.splits; g.partial = partial;
+		launch_tiles<A_T, B_T, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>(s, g, wholes, wholes && d.large);
+		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), g.problems), dim3(256), 0, s, g);
+	} else launch_tiles<A_T, B_T, EPI>(s, g, wholes, wholes && d.large);
+}
+template <int MT> void launch_few_rows(hipStream_t s, const GemmArgs& g, bool gated) {
+	// slices of at least 128 steps, as many as make enough wavefronts: 8 a block
+	uint32_t slices = 8;
+	while (slices > 1 && g.steps < slices * 128) slices /= 2;
+	const uint32_t per = (div_up(g.steps, slices) + 31) & ~31u, blocks = div_up(div_up(g.cols, 16), 8 / slices);
+	if (gated) hipLaunchKernelGGL((k_few_rows<MT, true>), dim3(blocks), dim3(512), 0, s, g, slices, per);
+	else hipLaunchKernelGGL((k_few_rows<MT, false>), dim3(blocks), dim3(512), 0, s, g, slices, per);
 }
 } // namespace
 
@@ -587,11 +679,16 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	if (!d.m || !d.n) return;
 	GemmArgs g{};
 	g.a = (const T*)d.x; g.lda = d.x_stride; g.ldb = d.w_stride;
-	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1; g.splits = 1;
+	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1;
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
+	if (d.m <= FEW_ROWS && d.k) {
+		if (d.m <= 16) launch_few_rows<1>(s, g, d.gated); else if (d.m <= 32) launch_few_rows<2>(s, g, d.gated); else launch_few_rows<4>(s, g, d.gated);
+		return;
+	}
 	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
-	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes);
+	float* partial = (float*)d.workspace;
+	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes, partial); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes, partial);
 }
 void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const DensePlan p = dense_plan(d.m, d.n, d.k, d.gated);
@@ -614,23 +711,18 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		if (bias && d.n) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(256), 0, s, (const float*)(ws + p.bias), p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
 	}
 	const bool g_whole = whole(G, ldg, G == d.dy ? d.n : 8); // (the workspace's lines are padded with zeros)
+	float* partial = (float*)(ws + p.partial); // (the two products use it in turn)
 	if (d.dx && d.m && d.k) {
 		GemmArgs g{};
 		g.a = G; g.lda = ldg; g.a_segment = up8(d.n); g.segments = problems; g.b[0] = (const T*)d.w[0]; g.b[1] = (const T*)d.w[1]; g.ldb = d.w_stride;
-		g.rows = d.m; g.cols = d.k; g.steps = d.n; g.problems = 1; g.splits = 1; g.c[0] = (T*)d.dx; g.ldc = d.dx_stride;
-		launch_gemm<true, false, EPI_STORE>(s, g, g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k));
+		g.rows = d.m; g.cols = d.k; g.steps = d.n; g.problems = 1; g.c[0] = (T*)d.dx; g.ldc = d.dx_stride;
+		launch_gemm<true, false, EPI_STORE>(s, g, g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k), partial);
 	}
 	if ((d.dw[0] || d.dw[1]) && d.n && d.k) {
 		GemmArgs g{};
 		g.a = G; g.lda = ldg; g.a_problem = up8(d.n); g.problems = problems; g.b[0] = g.b[1] = (const T*)d.x; g.ldb = d.x_stride;
 		g.rows = d.n; g.cols = d.k; g.steps = d.m; g.segments = 1; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
-		g.splits = p.splits;
-		const bool wholes = g_whole && whole(d.x, d.x_stride, d.k);
-		if (p.splits > 1) {
-			g.partial = (float*)(ws + p.partial);
-			launch_gemm<false, false, EPI_PARTIAL>(s, g, wholes);
-			hipLaunchKernelGGL(k_join_splits, dim3(div_up((uint64_t)d.n * up8(d.k) / 8, 256), problems), dim3(256), 0, s, g.partial, p.splits, problems, d.n, d.k, g.c[0], g.c[1], g.ldc);
-		} else launch_gemm<false, false, EPI_STORE>(s, g, wholes);
+		launch_gemm<false, false, EPI_STORE>(s, g, g_whole && whole(d.x, d.x_stride, d.k), partial);
 	}
 }
 } // namespace ngp

@@ -2694,15 +2694,17 @@ static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t
 		}
 	return dense_check_device(what, s, b, nb);
 }
-extern "C" uint64_t ngp_linear_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, false).bytes : 0; }
-extern "C" uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, true).bytes : 0; }
+extern "C" uint64_t ngp_linear_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, false).bytes : dense_forward_bytes(m, n, k, false); }
+extern "C" uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, true).bytes : dense_forward_bytes(m, n, k, true); }
 extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, const void* bias,
 		const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+	const uint64_t need = dense_forward_bytes(m, n, k, false);
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w, n, k, w_stride, "w", false}, {bias, 1, n, n, "bias", false}, {residual, m, n, residual_stride, "residual", false},
-		{y, m, n, y_stride, "y", true}, {pre, m, n, pre_stride, "pre", true}};
+		{y, m, n, y_stride, "y", true}, {pre, m, n, pre_stride, "pre", true}, {workspace, 1, need, need, "workspace", true, 1}};
 	REQUIRE((x && w) || !m || !n || !k, "ngp_linear_forward: null argument");
 	REQUIRE(y || !m || !n, "ngp_linear_forward: null argument");
-	if (int rc = dense_check("ngp_linear_forward", type, activation, m, n, k, (hipStream_t)stream, b, 6, y, residual)) return rc;
+	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_linear_forward: workspace smaller than ngp_linear_workspace_size() or not 16-byte aligned");
+	if (int rc = dense_check("ngp_linear_forward", type, activation, m, n, k, (hipStream_t)stream, b, 7, y, residual)) return rc;
 	DenseArgs d{};
 	d.gated = false; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w; d.w_stride = w_stride; d.bias[0] = bias;
 	d.residual = residual; d.residual_stride = residual_stride; d.y = y; d.y_stride = y_stride; d.pre[0] = pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;
@@ -2712,11 +2714,13 @@ extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32
 }
 extern "C" int ngp_gated_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up, uint64_t w_stride,
 		const void* bias_gate, const void* bias_up, void* y, uint64_t y_stride, void* gate_pre, void* up_pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+	const uint64_t need = dense_forward_bytes(m, n, k, true);
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w_gate, n, k, w_stride, "w_gate", false}, {w_up, n, k, w_stride, "w_up", false}, {bias_gate, 1, n, n, "bias_gate", false},
-		{bias_up, 1, n, n, "bias_up", false}, {y, m, n, y_stride, "y", true}, {gate_pre, m, n, pre_stride, "gate_pre", true}, {up_pre, m, n, pre_stride, "up_pre", true}};
+		{bias_up, 1, n, n, "bias_up", false}, {y, m, n, y_stride, "y", true}, {gate_pre, m, n, pre_stride, "gate_pre", true}, {up_pre, m, n, pre_stride, "up_pre", true}, {workspace, 1, need, need, "workspace", true, 1}};
 	REQUIRE((x && w_gate && w_up) || !m || !n || !k, "ngp_gated_forward: null argument");
 	REQUIRE(y || !m || !n, "ngp_gated_forward: null argument");
-	if (int rc = dense_check("ngp_gated_forward", type, activation, m, n, k, (hipStream_t)stream, b, 8, nullptr, nullptr)) return rc;
+	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_gated_forward: workspace smaller than ngp_gated_workspace_size() or not 16-byte aligned");
+	if (int rc = dense_check("ngp_gated_forward", type, activation, m, n, k, (hipStream_t)stream, b, 9, nullptr, nullptr)) return rc;
 	DenseArgs d{};
 	d.gated = true; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w_gate; d.w[1] = w_up; d.w_stride = w_stride; d.bias[0] = bias_gate; d.bias[1] = bias_up;
 	d.y = y; d.y_stride = y_stride; d.pre[0] = gate_pre; d.pre[1] = up_pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;

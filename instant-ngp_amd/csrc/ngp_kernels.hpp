@@ -351,27 +351,43 @@ struct DenseArgs {
 	const void* dy; uint64_t dy_stride; void* dx; uint64_t dx_stride; void* dw[2]; uint64_t dw_stride; void* dbias[2]; // backward
 	void* workspace; uint64_t workspace_size;
 };
-// How a backward pass is split and where its pieces lie in the workspace (bytes); derived from the sizes alone so that ngp_*_workspace_size and the launch agree.
-struct DensePlan { uint64_t grad, bias, partial, bytes; uint32_t rows_per_block, row_blocks, splits; };
+constexpr uint32_t FEW_ROWS = 64; // up to here the forward pass reads the weights once, straight into registers (k_few_rows)
+// A product of rows x cols with `steps * segments` terms a sum, `parts` times over: tile size and the number of pieces every sum is cut into (each a block of its own, joined by a
+// second launch).  From sizes alone.
+struct DenseSplit { uint32_t splits; bool large; };
+inline DenseSplit dense_split(uint64_t rows, uint64_t cols, uint64_t steps, uint32_t segments, uint32_t parts) {
+	auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+	const uint64_t chunks = up(steps, 64) * segments, large = up(rows, 256) * up(cols, 256) * parts, small = up(rows, 128) * up(cols, 128) * parts;
+	if (large >= 200) return {1, true};
+	// time of a piece: a chunk of a 128 x 128 tile 0.35 us (two blocks a compute unit, 512 at a time); partial sums: written and read at 4 TB/s, a second launch 3 us
+	const double bytes = (double)rows * (double)((cols + 7) & ~7ull) * parts * 8;
+	double best = 1e30; uint32_t pick = 1;
+	for (uint32_t k = 1; k <= 256 && (k == 1 || (chunks >= 2 * k && bytes / 2 * k <= 256e6)); ++k) {
+		const double t = (double)up(small * k, 512) * (3.0 + 0.35 * (double)up(chunks, k)) + (k > 1 ? 3.0 + bytes * k / 4e6 : 0.0);
+		if (t < best * 0.98) { best = t; pick = k; }
+	}
+	return {(uint32_t)(chunks ? up(chunks, up(chunks, pick)) : 1), false};
+}
+inline uint64_t dense_split_bytes(uint64_t rows, uint64_t cols, uint64_t steps, uint32_t segments, uint32_t parts) {
+	const DenseSplit d = dense_split(rows, cols, steps, segments, parts);
+	return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0;
+}
+inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) { return m <= FEW_ROWS ? 0 : (dense_split_bytes(m, n, k, 1, gated ? 2 : 1) + 255) & ~255ull; }
+// Where the pieces of a backward pass lie in the workspace (bytes); from the sizes alone, so that ngp_*_workspace_size and the launch agree.
+struct DensePlan { uint64_t grad, bias, partial, bytes; uint32_t rows_per_block, row_blocks; };
 inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	DensePlan p;
-	const uint64_t problems = gated ? 2 : 1, n8 = ((uint64_t)n + 7) & ~7ull, k8 = ((uint64_t)k + 7) & ~7ull;
+	const uint32_t problems = gated ? 2 : 1;
+	const uint64_t n8 = ((uint64_t)n + 7) & ~7ull;
 	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
 	// elementwise pass: about 1024 blocks of whole groups of 8 rows
-	const uint64_t col_blocks = (n + 255) / 256, want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
+	const uint64_t col_blocks = ((uint64_t)n + 255) / 256, want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
 	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
 	if (!p.rows_per_block) p.rows_per_block = 8;
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
-	// weight gradient: a sum over m samples per 128 x 128 tile; split it where the tiles alone leave compute units without work, in pieces of at least 4 chunks of 64 samples
-	const uint64_t tiles = (((uint64_t)n + 127) / 128) * (((uint64_t)k + 127) / 128) * problems, chunks = ((uint64_t)m + 63) / 64, one = problems * n * k8 * 4;
-	uint64_t splits = tiles ? 512 / tiles : 1;
-	if (splits > chunks / 4) splits = chunks / 4;
-	if (one && splits > (256ull << 20) / one) splits = (256ull << 20) / one;
-	if (splits < 1) splits = 1;
-	const uint64_t per = (chunks + splits - 1) / splits;
-	p.splits = (uint32_t)(per ? (chunks + per - 1) / per : 1);
-	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + problems * p.row_blocks * n * 4);
-	p.bytes = p.partial + (p.splits > 1 ? up(p.splits * one) : 0);
+	const uint64_t dx = dense_split_bytes(m, k, n, problems, 1), dw = dense_split_bytes(n, k, m, 1, problems);
+	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
+	p.bytes = p.partial + up(dx > dw ? dx : dw);
 	return p;
 }
 void launch_dense_forward_half(hipStream_t s, const DenseArgs& d);
