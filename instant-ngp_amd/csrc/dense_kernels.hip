@@ -63,6 +63,22 @@ __device__ inline T8 load8(const T* p, int n) {
 	for (int i = 0; i < 8; ++i) if (i < n) v[i] = p[i];
 	return v;
 }
+// elements c .. c + 7 of a line of `width` >= 8 out of the 16 bytes that were read at min(c, width - 8): moved down, zeros behind the line's end, without a branch
+__device__ inline T8 shift8(T8 raw, int c, int width) {
+	const int by = c - min(c, width - 8), d = by >> 1;
+	uint32_t v[4], t[4];
+	__builtin_memcpy(v, &raw, 16);
+	t[0] = d & 2 ? v[2] : v[0]; t[1] = d & 2 ? v[3] : v[1]; t[2] = d & 2 ? 0 : v[2]; t[3] = d & 2 ? 0 : v[3];
+	v[0] = d & 1 ? t[1] : t[0]; v[1] = d & 1 ? t[2] : t[1]; v[2] = d & 1 ? t[3] : t[2]; v[3] = d & 1 ? 0 : t[3];
+	const bool odd = by & 1, none = by >= 8;
+	t[0] = odd ? __builtin_amdgcn_alignbit(v[1], v[0], 16) : v[0]; t[1] = odd ? __builtin_amdgcn_alignbit(v[2], v[1], 16) : v[1];
+	t[2] = odd ? __builtin_amdgcn_alignbit(v[3], v[2], 16) : v[2]; t[3] = odd ? v[3] >> 16 : v[3];
+	T8 r;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) t[i] = none ? 0 : t[i];
+	__builtin_memcpy(&r, t, 16);
+	return r;
+}
 __device__ inline void store8(T* p, T8 v, int n) {
 	if (n >= 8) { __builtin_memcpy(p, &v, 16); return; }
 #pragma unroll
@@ -207,31 +223,55 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 #pragma unroll
 		for (int j = 0; j < FC; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
 	T8 ra[NA], rb[NB];
+	// An operand's share of a chunk: `extent` of the matrix from e0 on, `left` steps.  What lies outside the matrix only reaches sums that are dropped, so lines and columns are clamped
+	// there; beyond the sum's last step both operands are zero (put right on the way to LDS, when the loads have arrived).
+	auto load_operand = [&](auto tile_c, auto contig_c, T8* out, auto count_c, auto&& matrix, uint64_t ld, uint32_t e0, uint32_t extent, uint32_t t0, int left) {
+		typedef decltype(tile_c) TX; constexpr bool CONTIG = decltype(contig_c)::value; constexpr int COUNT = decltype(count_c)::value;
+		const int width = CONTIG ? (int)g.steps : (int)extent;
+#pragma unroll
+		for (int q = 0; q < COUNT; ++q) {
+			const int slot = q * THREADS + tid, line = slot / TX::SLOTS, chunk = TX::source(line, slot % TX::SLOTS);
+			uint32_t in_tile = line; // (CONTIG)
+			const T* base = matrix(in_tile);
+			const T* p = CONTIG ? base + (uint64_t)min(e0 + in_tile, extent - 1) * ld : base + (uint64_t)(t0 + min(line, left - 1)) * ld;
+			const int c = (CONTIG ? (int)t0 : (int)e0) + chunk * 8;
+			if (width < 8) out[q] = load8(p + c, width - c); else out[q] = load8(p + min(c, width - 8));
+		}
+	};
+	auto to_lds = [&](auto tile_c, auto contig_c, T8* in, auto count_c, T* lds, uint32_t e0, uint32_t extent, uint32_t t0, int left) {
+		typedef decltype(tile_c) TX; constexpr bool CONTIG = decltype(contig_c)::value; constexpr int COUNT = decltype(count_c)::value;
+		const int width = CONTIG ? (int)g.steps : (int)extent;
+		if (width >= 8 && (CONTIG ? left < TK : e0 + TX::ELEMS / TK > extent)) {
+#pragma unroll
+			for (int q = 0; q < COUNT; ++q) {
+				const int slot = q * THREADS + tid, chunk = TX::source(slot / TX::SLOTS, slot % TX::SLOTS);
+				in[q] = shift8(in[q], (CONTIG ? (int)t0 : (int)e0) + chunk * 8, width);
+			}
+		}
+		if (!CONTIG && left < TK) {
+#pragma unroll
+			for (int q = 0; q < COUNT; ++q) if ((q * THREADS + (int)tid) / TX::SLOTS >= left) in[q] = T8{};
+		}
+#pragma unroll
+		for (int q = 0; q < COUNT; ++q) *(T8*)(lds + (q * THREADS + tid) * 8) = in[q];
+	};
+	uint32_t t0 = 0; int left = 0; // of the chunk in the registers
 	auto load = [&](uint32_t t) {
-		const uint32_t seg = t / chunks_per_segment, t0 = (t - seg * chunks_per_segment) * TK;
-		const int left = (int)min((uint32_t)TK, g.steps - t0);
-#pragma unroll
-		for (int q = 0; q < NA; ++q) {
-			const int slot = q * THREADS + tid, line = slot / TA::SLOTS, chunk = TA::source(line, slot % TA::SLOTS);
-			const T* base = a + seg * g.a_segment;
-			if (A_T) { const bool in = r0 + line < g.rows; ra[q] = load8(base + (uint64_t)(r0 + line) * g.lda + t0 + chunk * 8, in ? left - chunk * 8 : 0); }
-			else { const uint32_t r = r0 + chunk * 8; ra[q] = load8(base + (uint64_t)(t0 + line) * g.lda + r, line < left ? (int)g.rows - (int)r : 0); }
-		}
-#pragma unroll
-		for (int q = 0; q < NB; ++q) {
-			const int slot = q * THREADS + tid, line = slot / TB::SLOTS, chunk = TB::source(line, slot % TB::SLOTS);
-			if (B_T) {
-				const uint32_t which = GATED_TILE<EPI> && line >= OUT, col = c0 + line - which * OUT;
-				rb[q] = load8(g.b[which] + (uint64_t)col * g.ldb + t0 + chunk * 8, col < g.cols ? left - chunk * 8 : 0);
-			} else { const uint32_t c = c0 + chunk * 8; rb[q] = load8(g.b[seg] + (uint64_t)(t0 + line) * g.ldb + c, line < left ? (int)g.cols - (int)c : 0); }
-		}
+		const uint32_t seg = t / chunks_per_segment;
+		t0 = (t - seg * chunks_per_segment) * TK;
+		left = (int)min((uint32_t)TK, g.steps - t0);
+		load_operand(TA{}, std::integral_constant<bool, A_T>(), ra, std::integral_constant<int, NA>(), [&](uint32_t&) { return a + seg * g.a_segment; }, g.lda, r0, g.rows, t0, left);
+		load_operand(TB{}, std::integral_constant<bool, B_T>(), rb, std::integral_constant<int, NB>(), [&](uint32_t& line) -> const T* {
+			if (!B_T) return g.b[seg];
+			const uint32_t which = GATED_TILE<EPI> && line >= OUT; // (gated: the tile's second half is the up projection's)
+			line -= which * OUT;
+			return which ? g.b[1] : g.b[0];
+		}, g.ldb, c0, g.cols, t0, left);
 	};
 	if (t_begin < t_end) load(t_begin);
 	for (uint32_t t = t_begin; t < t_end; ++t) {
-#pragma unroll
-		for (int q = 0; q < NA; ++q) *(T8*)(lds_a + (q * THREADS + tid) * 8) = ra[q];
-#pragma unroll
-		for (int q = 0; q < NB; ++q) *(T8*)(lds_b + (q * THREADS + tid) * 8) = rb[q];
+		to_lds(TA{}, std::integral_constant<bool, A_T>(), ra, std::integral_constant<int, NA>(), lds_a, r0, g.rows, t0, left);
+		to_lds(TB{}, std::integral_constant<bool, B_T>(), rb, std::integral_constant<int, NB>(), lds_b, c0, g.cols, t0, left);
 		__syncthreads();
 		if (t + 1 < t_end) load(t + 1);
 #pragma unroll
@@ -266,11 +306,12 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 }
 
 // ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero) in units of 64 steps
-// of one operand (whole cache lines: 64-byte pieces ask the L2 twice as often, 65 instead of 70 % of the matrix rate).  Three units of A and two of B are in LDS, 160 KB at
-// 256 x 256: the one in use, and what is on its way two halves (A: three) ahead, about 2000 clocks.  The matrix instructions run through a unit in two halves of 32 steps; A fragments
+// of one operand (whole cache lines: 64-byte pieces ask the L2 twice as often, 65 instead of 70 % of the matrix rate).  UNITS of B and one more of A are in LDS: the one in use, and
+// what is on its way.  At 256 x 256 that is 160 KB with UNITS = 2 (about 2000 clocks ahead); 128 x 128 tiles take a quarter of the time a unit and get UNITS = 4 where a compute
+// unit has one block to itself (144 KB), 2 where it has two.  The matrix instructions run through a unit in two halves of 32 steps; A fragments
 // come in three ahead of their use, the next half's B fragments into a second set of registers.  4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128
 // products is what LDS can deliver beside the incoming units (96 of the 128 bytes a clock; with 8 wavefronts of 128 x 64 it would be all of them).
-constexpr int AK = 64, UNITS_A = 3, UNITS_B = 2, A_RING = 4;
+constexpr int AK = 64, A_RING = 4;
 typedef int i4v __attribute__((ext_vector_type(4)));
 template <int EXTENT, bool T_CONTIG, int WAVES> struct Async {
 	static constexpr int SLOTS = T_CONTIG ? AK / 8 : EXTENT / 8, BYTES = EXTENT * AK * 2, LOADS = BYTES / 1024 / WAVES;
@@ -327,11 +368,11 @@ template <bool T_CONTIG, int UNITS, int BYTES> struct Cursor {
 		}
 	}
 };
-template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
-__global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(GemmArgs g) {
+template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS>
+__global__ __launch_bounds__(64 * WR * WC, BR >= 256 || UNITS > 2 ? 1 : 2) void k_gemm_async(GemmArgs g) {
 	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = GATED_TILE<EPI> ? BC / 2 : BC;
 	typedef Async<BR, A_T, WAVES> LA; typedef Async<BC, B_T, WAVES> LB;
-	constexpr int LDS = UNITS_A * LA::BYTES + UNITS_B * LB::BYTES;
+	constexpr int UNITS_A = UNITS + 1, UNITS_B = UNITS, LDS = UNITS_A * LA::BYTES + UNITS_B * LB::BYTES;
 	constexpr int STRIP = BC / WC + 4, PASS = FR > 4 ? 4 : FR; // epilogue: floats per row of a wavefront's strip of LDS, fragment rows in it
 	static_assert(WAVES * PASS * 16 * STRIP * 4 <= LDS && FR % PASS == 0, "the epilogue's strips fit");
 	static_assert(FC % (GATED_TILE<EPI> ? 4 : 2) == 0 && FR % A_RING == 0 && LA::LOADS % FR == 0 && LB::LOADS % FR == 0, "");
@@ -398,8 +439,8 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	T8 fa[A_RING], fb[2][FC];
 	uint32_t a_here = lds0, b_here = lds0 + UNITS_A * LA::BYTES;
 	// The matrix instructions of one half of a unit.  One wavefront has the SIMD to itself, so whatever else is to be issued stands between two matrix instructions, a little at a
-	// time.  Half 0: the barrier behind its first instructions says that every wavefront is through with the unit of A before this one, whose place the loads of the unit after the
-	// next take.  Half 1: the barrier behind its first row of fragments says that every wavefront has this unit's B in registers and that the next units have arrived.
+	// time.  Half 0: the barrier behind its first instructions says that every wavefront is through with the unit of A before this one, whose place the loads of the unit UNITS
+	// ahead take.  Half 1: the barrier behind its first row of fragments says that every wavefront has this unit's B in registers and that the next units have arrived.
 	auto half_step = [&](auto half_c, uint32_t a_next, uint32_t b_next) {
 		constexpr int half = decltype(half_c)::value, Q = FC / 4;
 #pragma unroll
@@ -408,7 +449,7 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 			for (int j = 0; j < FC; ++j) {
 				mfma_in_place(fb[half][j], fa[i % A_RING], acc[i][j]);
 				if (j == (half == 1 && i == 0 ? FC - 1 : 0)) {
-					if (half == 1 && i == 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LA::LOADS) : "memory");
+					if (half == 1 && i == 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((UNITS - 1) * LA::LOADS + (UNITS - 2) * LB::LOADS) : "memory");
 					fa[(i + AHEAD) % A_RING] = i + AHEAD < FR ? read_a(half, i + AHEAD, a_here) : half == 0 ? read_a(1, i + AHEAD - FR, a_here) : read_a(0, i + AHEAD - FR, a_next);
 				}
 				if (half == 0 && i == 0 && j == Q) asm volatile("s_barrier" ::: "memory");
@@ -435,15 +476,16 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 	if (t_begin < t_end) {
 		auto all_a = [&]() { for (int q = 0; q < LA::LOADS; ++q) load_a(q); ca.next(start_a, g.steps); };
 		auto all_b = [&]() { for (int q = 0; q < LB::LOADS; ++q) load_b(q); cb.next(start_b, g.steps); };
-		all_a(); all_b(); all_a(); all_b();
-		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LA::LOADS + LB::LOADS) : "memory");
+#pragma unroll
+		for (int k = 0; k < UNITS; ++k) { all_a(); all_b(); }
+		asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((UNITS - 1) * (LA::LOADS + LB::LOADS)) : "memory");
 #pragma unroll
 		for (int i = 0; i < AHEAD; ++i) fa[i] = read_a(0, i, a_here);
 #pragma unroll
 		for (int j = 0; j < FC; ++j) fb[0][j] = read_b(0, j, b_here);
 		for (uint32_t t = t_begin; t < t_end; ++t) {
 			const uint32_t a_next = a_here == lds0 + (UNITS_A - 1) * LA::BYTES ? lds0 : a_here + LA::BYTES;
-			const uint32_t b_next = b_here == lds0 + UNITS_A * LA::BYTES ? b_here + LB::BYTES : lds0 + UNITS_A * LA::BYTES;
+			const uint32_t b_next = b_here == lds0 + UNITS_A * LA::BYTES + (UNITS_B - 1) * LB::BYTES ? lds0 + UNITS_A * LA::BYTES : b_here + LB::BYTES;
 			half_step(std::integral_constant<int, 0>(), a_next, b_next);
 			half_step(std::integral_constant<int, 1>(), a_next, b_next);
 			a_here = a_next; b_here = b_next;
@@ -486,13 +528,14 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 ? 1 : 2) void k_gemm_async(
 
 // ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
 // straight from memory to registers as the matrix instruction's fragments, U loads on the way at a time; the samples (MT x 16 rows, the last one repeated where there are fewer)
-// come out of the caches.  SLICES wavefronts share the sum and add up in LDS, in their order.
-template <int MT, bool GATED> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
-	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4, EPI = GATED ? EPI_GATED : EPI_LINEAR;
+// come out of the caches.  `slices` wavefronts share the sum and add up in LDS, in their order; where there are few outputs blocks share it too (EPI_PARTIAL*).
+template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
+	constexpr bool GATED = GATED_TILE<EPI>;
+	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4;
 	__shared__ float sums[8][P][MT * 16][20]; // [wavefront][projection][row][output]
 	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gq = lane >> 4, li = lane & 15;
 	const uint32_t slice = wave % slices, tile = blockIdx.x * (8 / slices) + wave / slices, c0 = tile * 16;
-	const uint32_t t_begin = min(g.steps, slice * steps_per_slice), t_end = min(g.steps, t_begin + steps_per_slice);
+	const uint32_t t_begin = min(g.steps, (blockIdx.y * slices + slice) * steps_per_slice), t_end = min(g.steps, t_begin + steps_per_slice);
 	const uint32_t col = min(c0 + li, g.cols - 1); // (outputs behind the last one repeat it and are dropped)
 	const T* w[P]; const T* x[MT];
 #pragma unroll
@@ -550,7 +593,7 @@ template <int MT, bool GATED> __global__ __launch_bounds__(512) void k_few_rows(
 			EACH z[e] += sums[k * slices + q][0][r][half * 8 + e];
 			if (GATED) EACH u[e] += sums[k * slices + q][P - 1][r][half * 8 + e];
 		}
-		epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+		epilogue8<EPI>(g, 0, blockIdx.y, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
 	}
 }
 
@@ -599,21 +642,21 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 		if (col < g.cols) g.bias_partial[((uint64_t)blockIdx.y * (GATED ? 2 : 1) + k) * g.cols + col] = s;
 	}
 }
-// dbias = sum of the blocks' column sums, in their order
-__global__ __launch_bounds__(256) void k_bias_grad(const float* partial, uint32_t blocks, uint32_t cols, uint32_t problems, T* out0, T* out1) {
-	__shared__ float red[8][32];
+// dbias = sum of the blocks' column sums: 32 columns x 32 shares of the blocks, then the shares in their order
+__global__ __launch_bounds__(1024) void k_bias_grad(const float* partial, uint32_t blocks, uint32_t cols, uint32_t problems, T* out0, T* out1) {
+	__shared__ float red[32][33];
 	const uint32_t cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx, k = blockIdx.y;
 	float s = 0.f;
 	if (c < cols) {
-#pragma unroll 4
-		for (uint32_t b = ry; b < blocks; b += 8) s += partial[((uint64_t)b * problems + k) * cols + c];
+#pragma unroll 8
+		for (uint32_t b = ry; b < blocks; b += 32) s += partial[((uint64_t)b * problems + k) * cols + c];
 	}
 	red[ry][cx] = s;
 	__syncthreads();
 	if (ry == 0 && c < cols) {
 		float t = 0.f;
 #pragma unroll
-		for (int y = 0; y < 8; ++y) t += red[y][cx];
+		for (int y = 0; y < 32; ++y) t += red[y][cx];
 		T* out = k ? out1 : out0;
 		if (out) out[c] = (T)t;
 	}
@@ -653,8 +696,9 @@ template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs
 	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
 	static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
 	if (!wholes) hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
-	else if (large) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
-	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
+	else if (large) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
+	else if (grid.x * g.problems * g.splits <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
+	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
 }
 template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
 	const DenseSplit d = dense_split(g.rows, g.cols, g.steps, g.segments, EPI == EPI_GATED ? 2 : g.problems);
@@ -665,13 +709,15 @@ template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs&
 		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), g.problems), dim3(256), 0, s, g);
 	} else launch_tiles<A_T, B_T, EPI>(s, g, wholes, wholes && d.large);
 }
-template <int MT> void launch_few_rows(hipStream_t s, const GemmArgs& g, bool gated) {
-	// slices of at least 128 steps, as many as make enough wavefronts: 8 a block
-	uint32_t slices = 8;
-	while (slices > 1 && g.steps < slices * 128) slices /= 2;
-	const uint32_t per = (div_up(g.steps, slices) + 31) & ~31u, blocks = div_up(div_up(g.cols, 16), 8 / slices);
-	if (gated) hipLaunchKernelGGL((k_few_rows<MT, true>), dim3(blocks), dim3(512), 0, s, g, slices, per);
-	else hipLaunchKernelGGL((k_few_rows<MT, false>), dim3(blocks), dim3(512), 0, s, g, slices, per);
+template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, float* partial) {
+	const DenseFewRows f = dense_few_rows(g.cols, g.steps);
+	const dim3 grid(div_up(div_up(g.cols, 16), 8 / f.slices), f.splits);
+	const uint32_t per = (div_up(g.steps, f.slices * f.splits) + 31) & ~31u;
+	g.splits = f.splits; g.partial = partial;
+	if (f.splits > 1) {
+		hipLaunchKernelGGL((k_few_rows<MT, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>), grid, dim3(512), 0, s, g, f.slices, per);
+		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), 1), dim3(256), 0, s, g);
+	} else hipLaunchKernelGGL((k_few_rows<MT, EPI>), grid, dim3(512), 0, s, g, f.slices, per);
 }
 } // namespace
 
@@ -682,12 +728,13 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1;
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
+	float* partial = (float*)d.workspace;
 	if (d.m <= FEW_ROWS && d.k) {
-		if (d.m <= 16) launch_few_rows<1>(s, g, d.gated); else if (d.m <= 32) launch_few_rows<2>(s, g, d.gated); else launch_few_rows<4>(s, g, d.gated);
+		if (d.m <= 16) { if (d.gated) launch_few_rows<1, EPI_GATED>(s, g, partial); else launch_few_rows<1, EPI_LINEAR>(s, g, partial); }
+		else { if (d.gated) launch_few_rows<2, EPI_GATED>(s, g, partial); else launch_few_rows<2, EPI_LINEAR>(s, g, partial); }
 		return;
 	}
 	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
-	float* partial = (float*)d.workspace;
 	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes, partial); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes, partial);
 }
 void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
@@ -708,7 +755,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		if (d.m && d.n) {
 			if (d.gated) hipLaunchKernelGGL(k_output_grad<true>, grid, dim3(256), 0, s, a); else hipLaunchKernelGGL(k_output_grad<false>, grid, dim3(256), 0, s, a);
 		}
-		if (bias && d.n) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(256), 0, s, (const float*)(ws + p.bias), p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
+		if (bias && d.n) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, (const float*)(ws + p.bias), p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
 	}
 	const bool g_whole = whole(G, ldg, G == d.dy ? d.n : 8); // (the workspace's lines are padded with zeros)
 	float* partial = (float*)(ws + p.partial); // (the two products use it in turn)
