@@ -196,6 +196,14 @@ template <int EPI> constexpr bool GATED_TILE = EPI == EPI_GATED || EPI == EPI_PA
 template <int EPI> __device__ inline T8 bias8(const GemmArgs& g, int k, uint32_t c, int n) { return (EPI == EPI_LINEAR || EPI == EPI_GATED) && g.bias[k] && n > 0 ? load8(g.bias[k] + c, n) : T8{}; }
 template <int EPI> __device__ inline T8 residual8(const GemmArgs& g, uint32_t r, uint32_t c, int n) { return EPI == EPI_LINEAR && g.residual && n > 0 ? load8(g.residual + (uint64_t)r * g.ld_residual + c, n) : T8{}; }
 
+// Consecutive blocks go to the 8 dies in turn, each with an L2 of its own: give every die one contiguous run of the work, ordered by piece of the sum, product, strips of 8 row
+// tiles, so that its blocks share operands.  (Tiles of one piece on four dies: every operand line missed four L2s, dW of 2^18 samples 86 instead of 60 us.)
+struct Work { uint32_t row, col, problem, split; };
+__device__ inline Work work_of(const GemmArgs& g, uint32_t row_tiles, uint32_t col_tiles) {
+	const uint32_t n = gridDim.x, die = blockIdx.x & 7, per = n >> 3, rest = n & 7, t = die * per + min(die, rest) + (blockIdx.x >> 3), tiles = row_tiles * col_tiles;
+	const uint32_t which = t / tiles, in = t - which * tiles, strip = 8 * col_tiles, s = in / strip, k = in - s * strip, rows = min(8u, row_tiles - s * 8);
+	return {s * 8 + k % rows, k / rows, which % g.problems, which / g.problems};
+}
 // C tile BR x BC by WR x WC wavefronts; each owns (BR / WR) x (BC / WC) as 16 x 16 fragments (matrix instruction 16x16x32, C^T: a lane holds one row of C and 4 columns
 // of each fragment).  EPI_GATED: the tile's columns are BC / 2 gate outputs and the same BC / 2 up outputs, every wavefront owns both of its columns.
 template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
@@ -207,9 +215,8 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	__shared__ __attribute__((aligned(16))) T lds_a[TA::ELEMS];
 	__shared__ __attribute__((aligned(16))) T lds_b[TB::ELEMS];
 	const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
-	const uint32_t col_tiles = (g.cols + OUT - 1) / OUT;
-	const uint32_t r0 = blockIdx.x / col_tiles * BR, c0 = blockIdx.x % col_tiles * OUT;
-	const uint32_t problem = blockIdx.y, split = blockIdx.z;
+	const Work w = work_of(g, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
+	const uint32_t r0 = w.row * BR, c0 = w.col * OUT, problem = w.problem, split = w.split;
 	const T* a = g.a + problem * g.a_problem;
 	const uint32_t chunks_per_segment = (g.steps + TK - 1) / TK, n_chunks = chunks_per_segment * g.segments;
 	const uint32_t t_begin = split * g.chunks_per_split, t_end = min(n_chunks, t_begin + g.chunks_per_split);
@@ -345,12 +352,6 @@ __device__ inline const T* uniform(const T* p) { // (a pointer that is the same 
 	return (const T*)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
 }
 __device__ inline i4v resource(const T* p, int records) { const uint64_t a = (uint64_t)p; return i4v{(int)(uint32_t)a, (int)((a >> 32) & 0xffff), records, 0x00020000}; }
-// consecutive blocks go to the 8 dies in turn: give each die one contiguous run of tiles, ordered in strips of 8 row tiles, so that its blocks share operands in its L2
-__device__ inline void tile_of(uint32_t b, uint32_t row_tiles, uint32_t col_tiles, uint32_t& tr, uint32_t& tc) {
-	const uint32_t n = row_tiles * col_tiles, die = b & 7, per = n >> 3, rest = n & 7;
-	const uint32_t t = die * per + min(die, rest) + (b >> 3), strip = 8 * col_tiles, s = t / strip, in = t - s * strip, rows = min(8u, row_tiles - s * 8);
-	tr = s * 8 + in % rows; tc = in / rows;
-}
 // Where an operand's next unit comes from and goes to (all in scalar registers).  T_CONTIG: a line's elements beyond the sum are masked (Async::load), lines beyond the matrix lie
 // behind `records` wherever the unit is; otherwise the lines beyond the sum do, in its last unit alone.
 template <bool T_CONTIG, int UNITS, int BYTES> struct Cursor {
@@ -379,9 +380,8 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 || UNITS > 2 ? 1 : 2) void 
 	__shared__ __attribute__((aligned(1024))) char lds[LDS];
 	const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
-	uint32_t tr, tc;
-	tile_of(blockIdx.x, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT, tr, tc);
-	const uint32_t r0 = tr * BR, c0 = tc * OUT, problem = blockIdx.y, split = blockIdx.z;
+	const Work w = work_of(g, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
+	const uint32_t r0 = w.row * BR, c0 = w.col * OUT, problem = w.problem, split = w.split;
 	const uint32_t units_per_segment = (g.steps + AK - 1) / AK, n_units = units_per_segment * g.segments;
 	const uint32_t t_begin = min(n_units, split * g.chunks_per_split), t_end = min(n_units, t_begin + g.chunks_per_split);
 	const uint32_t which = GATED_TILE<EPI> && wave * LB::LOADS * 8 >= OUT ? 1 : 0; // gated: this wavefront loads gate or up weights
@@ -692,12 +692,12 @@ bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 
 template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs& g, bool wholes, bool large) {
 	constexpr int K = GATED_TILE<EPI> ? 2 : 1; // weight columns per column of C
 	const uint32_t tile = large ? 256 : 128;
-	const dim3 grid(div_up(g.rows, tile) * div_up(g.cols, tile / K), g.problems, g.splits);
+	const dim3 grid(div_up(g.rows, tile) * div_up(g.cols, tile / K) * g.problems * g.splits);
 	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
 	static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
 	if (!wholes) hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
 	else if (large) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
-	else if (grid.x * g.problems * g.splits <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
+	else if (grid.x <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
 	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
 }
 template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
