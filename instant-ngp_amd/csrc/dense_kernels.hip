@@ -597,6 +597,219 @@ template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(Gem
 	}
 }
 
+// ---- narrow layers (up to 256 inputs and outputs) over many samples: bound by reading and writing the samples once.
+// Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
+// their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
+// NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
+__device__ inline T8 line8(const T* line, int c, int width, bool ragged /* uniform: c + 8 may pass the line's end */) { // zeros behind the end
+	if (!ragged) return load8(line + c);
+	return width < 8 ? load8(line + c, width - c) : shift8(load8(line + min(c, width - 8)), c, width);
+}
+template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
+	constexpr bool GATED = GATED_TILE<EPI>;
+	constexpr int OF = GATED ? NF / 2 : NF; // fragments of outputs
+	__shared__ __attribute__((aligned(16))) T w[NF * KS * 512];
+	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gq = lane >> 4, li = lane & 15;
+	const uint32_t slabs = (g.rows + 15) / 16, stride = gridDim.x * 8;
+	uint32_t slab = blockIdx.x * 8 + wave;
+	const int steps = (int)g.steps, whole_ks = steps / 32; // steps of 32 without a line's end
+	T8 x[KS];
+	auto load_x = [&](uint32_t s) {
+		const T* line = g.a + (uint64_t)min(s * 16 + li, g.rows - 1) * g.lda; // (samples behind the last one repeat it and are dropped)
+#pragma unroll
+		for (int k = 0; k < KS; ++k) x[k] = line8(line, k * 32 + gq * 8, steps, k >= whole_ks);
+	};
+	if (slab < slabs) load_x(slab);
+	for (int q = threadIdx.x; q < NF * KS * 64; q += 512) {
+		const int l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3);
+		const T* line = g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb;
+		*(T8*)(w + q * 8) = line8(line, k * 32 + (l >> 4) * 8, steps, true);
+	}
+	__syncthreads();
+	for (; slab < slabs; slab += stride) {
+		asm volatile("" ::: "memory"); // (the weights stay in LDS: kept in registers across samples they spill)
+		f4v acc[NF];
+#pragma unroll
+		for (int f = 0; f < NF; ++f) acc[f] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+		for (int k = 0; k < KS; ++k)
+#pragma unroll
+			for (int f = 0; f < NF; ++f) acc[f] = mfma(*(const T8*)(w + ((f * KS + k) * 64 + lane) * 8), x[k], acc[f]);
+		if (slab + stride < slabs) load_x(slab + stride);
+		const uint32_t r = slab * 16 + li;
+		if (r < g.rows) {
+#pragma unroll
+			for (int p = 0; p < OF / 2; ++p) {
+				const uint32_t c = p * 32 + gq * 8;
+				if (c >= g.cols) continue;
+				const int n = (int)min(8u, g.cols - c);
+				float z[8], u[8];
+				EACH { z[e] = acc[2 * p + e / 4][e & 3]; u[e] = GATED ? acc[(GATED ? OF : 0) + 2 * p + e / 4][e & 3] : 0.f; }
+				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+			}
+		}
+	}
+}
+// Backward in one pass: a block takes 32 samples at a time (the next 32 on their way), forms G = dY * act'(Z) and lays it and X into LDS; its 8 wavefronts multiply G with the weights
+// (in LDS as fragments) to dX, and G^T with X into their parts of dW, which stay in registers to the end: one partial sum a block, joined by a second launch.  Every sample's
+// dY, Z, X is read once, dX written once.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
+struct NarrowArgs {
+	uint32_t rows, n, k; int act; const T* x; uint64_t ld_x; const T* w[2]; uint64_t ld_w; const T* pre[2]; uint64_t ld_pre; const T* dy; uint64_t ld_dy; T* dx; uint64_t ld_dx;
+	float* partial; float* bias_partial;
+};
+template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void k_narrow_backward(NarrowArgs g) {
+	constexpr int GC = NF * 16, XC = KF * 16, HALF = GC / 2, NS = NF / 2; // columns of G and X in LDS, first column of the up projection, steps of 32 outputs
+	constexpr int CG = (GATED ? HALF : GC) / 8, CX = XC / 8, RG = 512 / CG, RX = 512 / CX, LG = RG >= 32 ? 1 : 32 / RG, LX = RX >= 32 ? 1 : 32 / RX; // chunks a line, lines at once, chunks a thread
+	constexpr int UNITS = KF * 2 / 8, WN = NF / 4, WK = KF / 2; // 16 x 16 pieces of dX a wavefront has, fragments of dW (4 x 2 wavefronts)
+	static_assert(NF >= 4 && KF >= 4, "");
+	constexpr int RL = RG < 32 ? RG : 32, SLABS = 32 * (GC + XC) * 2, RED = RL * GC * 4; // (the bias's sums take the slabs' place at the end)
+	__shared__ __attribute__((aligned(16))) char shared[KF * NS * 1024 + (SLABS > RED ? SLABS : RED)];
+	T* wf = (T*)shared; T* lg = wf + KF * NS * 512; T* lx = lg + 32 * GC;
+	const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gq = lane >> 4, li = lane & 15, l4 = li >> 2;
+	const int gc = (tid % CG) * 8, gr = tid / CG, xc = (tid % CX) * 8, xr = tid / CX;
+	const uint32_t slabs = (g.rows + 31) / 32;
+	const bool ragged_n = g.n & 7 || g.n < (GATED ? HALF : GC), ragged_k = g.k & 7 || g.k < XC;
+	// a line's 16-byte slots are exchanged by an XOR with bits of the line, so that 16 lines' chunks (dX) and 32 bytes of 8 lines (dW's transposing reads) lie in different banks
+	auto slot = [](int line, int s, int slots) -> int { return s ^ ((((line & 3) << 1) | (line & 8) | ((line >> 2) & 1)) & (slots >= 16 ? 15 : slots - 1)); };
+	T8 dy[LG], z[LG], u[GATED ? LG : 1], x[LX];
+	auto load = [&](uint32_t s) {
+#pragma unroll
+		for (int q = 0; q < LG; ++q) if (RG < 32 || gr < 32) {
+			const uint64_t r = min(s * 32 + gr + q * RG, g.rows - 1);
+			dy[q] = line8(g.dy + r * g.ld_dy, gc, g.n, ragged_n);
+			if (g.pre[0]) z[q] = line8(g.pre[0] + r * g.ld_pre, gc, g.n, ragged_n); else z[q] = T8{};
+			if (GATED) u[GATED ? q : 0] = line8(g.pre[1] + r * g.ld_pre, gc, g.n, ragged_n);
+		}
+#pragma unroll
+		for (int q = 0; q < LX; ++q) if (RX < 32 || xr < 32) x[q] = line8(g.x + (uint64_t)min(s * 32 + xr + q * RX, g.rows - 1) * g.ld_x, xc, g.k, ragged_k);
+	};
+	uint32_t s = blockIdx.x;
+	if (s < slabs) load(s);
+	// the weights as fragments: 16 inputs, 32 outputs (8 a lane)
+	if (g.dx) {
+		for (int q = tid; q < KF * NS * 64; q += 512) {
+			const int l = q & 63, n0 = ((q >> 6) % NS) * 32 + (l >> 4) * 8, k = ((q >> 6) / NS) * 16 + (l & 15);
+			T8 v{};
+#pragma unroll
+			for (int e = 0; e < 8; ++e) {
+				const int c = n0 + e, n = GATED && c >= HALF ? c - HALF : c;
+				if (n < (int)g.n && k < (int)g.k) v[e] = g.w[GATED && c >= HALF][(uint64_t)n * g.ld_w + k];
+			}
+			*(T8*)(wf + q * 8) = v;
+		}
+	}
+	float sum[GATED ? 2 : 1][8] = {};
+	f4v acc[WN][WK];
+#pragma unroll
+	for (int i = 0; i < WN; ++i)
+#pragma unroll
+		for (int j = 0; j < WK; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
+	for (; s < slabs; s += gridDim.x) {
+		// G and X into LDS; samples behind the last one are zero
+#pragma unroll
+		for (int q = 0; q < LG; ++q) if (RG < 32 || gr < 32) {
+			const int line = gr + q * RG;
+			const bool in = s * 32 + line < g.rows;
+			float zf[8], value[8], slope[8];
+			T8 o, o2;
+			EACH zf[e] = (float)z[q][e];
+			act_value_slope8(g.act, zf, value, slope);
+#pragma unroll
+			for (int e = 0; e < 8; ++e) {
+				const bool live = in && gc + e < (int)g.n;
+				const float v = live && slope[e] != 0.f ? (GATED ? (float)dy[q][e] * (float)u[GATED ? q : 0][e] * slope[e] : (float)dy[q][e] * slope[e]) : 0.f; // (a closed unit passes nothing, whatever arrives)
+				sum[0][e] += v; o[e] = (T)v;
+				if (GATED) { const float v2 = live ? (float)dy[q][e] * value[e] : 0.f; sum[GATED ? 1 : 0][e] += v2; o2[e] = (T)v2; }
+			}
+			*(T8*)(lg + line * GC + slot(line, gc / 8, GC / 8) * 8) = o;
+			if (GATED) *(T8*)(lg + line * GC + slot(line, (HALF + gc) / 8, GC / 8) * 8) = o2;
+		}
+#pragma unroll
+		for (int q = 0; q < LX; ++q) if (RX < 32 || xr < 32) {
+			const int line = xr + q * RX;
+			*(T8*)(lx + line * XC + slot(line, xc / 8, XC / 8) * 8) = s * 32 + line < g.rows ? x[q] : T8{};
+		}
+		__syncthreads();
+		const uint32_t here = s;
+		if (s + gridDim.x < slabs) load(s + gridDim.x);
+		if (g.dx) {
+			f4v d[UNITS];
+			// pieces of 16 samples x 16 inputs: the wavefronts share out the inputs first
+#pragma unroll
+			for (int q = 0; q < UNITS; ++q) d[q] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+			for (int ns = 0; ns < NS; ++ns) {
+				T8 a[2];
+#pragma unroll
+				for (int h = 0; h < (UNITS == 1 ? 1 : 2); ++h) {
+					const int line = (UNITS == 1 ? (int)(wave & 1) : h) * 16 + li;
+					a[h] = *(const T8*)(lg + line * GC + slot(line, ns * 4 + gq, GC / 8) * 8);
+				}
+#pragma unroll
+				for (int q = 0; q < UNITS; ++q) {
+					const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q / 2;
+					d[q] = mfma(*(const T8*)(wf + ((kf * NS + ns) * 64 + lane) * 8), a[UNITS == 1 ? 0 : q & 1], d[q]);
+				}
+			}
+#pragma unroll
+			for (int q = 0; q < UNITS; ++q) {
+				const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q / 2;
+				const uint32_t r = here * 32 + (UNITS == 1 ? wave & 1 : q & 1) * 16 + li, c = kf * 16 + gq * 4;
+				if (r < g.rows && c < g.k) {
+					T* o = g.dx + (uint64_t)r * g.ld_dx + c;
+					T v[4] = {(T)d[q][0], (T)d[q][1], (T)d[q][2], (T)d[q][3]};
+					if (c + 4 <= g.k) __builtin_memcpy(o, v, 8);
+					else {
+#pragma unroll
+						for (int e = 0; e < 3; ++e) if (c + e < g.k) o[e] = v[e];
+					}
+				}
+			}
+		}
+		if (g.partial) {
+			auto tr8 = [&](const T* base, int cols, int f) -> T8 { // 8 samples (of 32) of column 16 f + li
+				const int line = gq * 8 + l4, e = f * 16 + (li & 3) * 4;
+				const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + line * cols + slot(line, e >> 3, cols / 8) * 8 + (e & 7)));
+				const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + (line + 4) * cols + slot(line + 4, e >> 3, cols / 8) * 8 + (e & 7)));
+				return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+			};
+			T8 a[WN];
+#pragma unroll
+			for (int i = 0; i < WN; ++i) a[i] = tr8(lg, GC, (wave >> 1) * WN + i);
+#pragma unroll
+			for (int j = 0; j < WK; ++j) {
+				const T8 b = tr8(lx, XC, (wave & 1) * WK + j);
+#pragma unroll
+				for (int i = 0; i < WN; ++i) acc[i][j] = mfma(b, a[i], acc[i][j]);
+			}
+		}
+		__syncthreads();
+	}
+	if (g.partial) {
+		const uint32_t k8 = up8(g.k);
+#pragma unroll
+		for (int i = 0; i < WN; ++i)
+#pragma unroll
+			for (int j = 0; j < WK; ++j) {
+				const uint32_t c = ((wave >> 1) * WN + i) * 16 + li, problem = GATED && c >= HALF, n = c - problem * HALF, k = ((wave & 1) * WK + j) * 16 + gq * 4;
+				if (n < g.n && k < k8) *(f4v*)(g.partial + (((uint64_t)blockIdx.x * (GATED ? 2 : 1) + problem) * g.n + n) * k8 + k) = acc[i][j];
+			}
+	}
+	if (g.bias_partial) {
+		float* red = (float*)lg; // [RL][GC]
+#pragma unroll
+		for (int p = 0; p < (GATED ? 2 : 1); ++p)
+			if (gr < RL) { EACH red[gr * GC + p * HALF + gc + e] = sum[p][e]; }
+		__syncthreads();
+		for (uint32_t c = tid; c < (uint32_t)GC; c += 512) {
+			float t = 0.f;
+			for (int y = 0; y < RL; ++y) t += red[y * GC + c];
+			const uint32_t problem = GATED && c >= (uint32_t)HALF, n = c - problem * HALF;
+			if (n < g.n) g.bias_partial[((uint64_t)blockIdx.x * (GATED ? 2 : 1) + problem) * g.n + n] = t;
+		}
+	}
+}
+
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
 // one line per block of rows, before the rounding).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
@@ -719,6 +932,25 @@ template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, floa
 		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), 1), dim3(256), 0, s, g);
 	} else hipLaunchKernelGGL((k_few_rows<MT, EPI>), grid, dim3(512), 0, s, g, f.slices, per);
 }
+template <int NF, int EPI> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
+	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI>), dim3(blocks), dim3(512), 0, s, g);
+	else if (g.steps <= 128) hipLaunchKernelGGL((k_narrow_forward<NF, 4, EPI>), dim3(blocks), dim3(512), 0, s, g);
+	else hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI>), dim3(blocks), dim3(512), 0, s, g);
+}
+template <int EPI> void launch_narrow_forward(hipStream_t s, const GemmArgs& g) {
+	const uint32_t cols = g.cols * (EPI == EPI_GATED ? 2 : 1), blocks = std::min(div_up(g.rows, 128), 512u);
+	if (cols <= 64) launch_narrow_forward_n<4, EPI>(s, g, blocks); else if (cols <= 128) launch_narrow_forward_n<8, EPI>(s, g, blocks); else launch_narrow_forward_n<16, EPI>(s, g, std::min(blocks, g.steps > 128 ? 256u : 512u));
+}
+template <int NF, int KF, bool GATED> void launch_narrow_backward_nk(hipStream_t s, const NarrowArgs& a, uint32_t blocks) {
+	hipLaunchKernelGGL((k_narrow_backward<NF, KF, GATED>), dim3(blocks), dim3(512), 0, s, a);
+}
+template <int NF, bool GATED> void launch_narrow_backward_n(hipStream_t s, const NarrowArgs& a, uint32_t blocks) {
+	if (a.k <= 64) launch_narrow_backward_nk<NF, 4, GATED>(s, a, blocks); else if (a.k <= 128) launch_narrow_backward_nk<NF, 8, GATED>(s, a, blocks); else launch_narrow_backward_nk<NF, 16, GATED>(s, a, blocks);
+}
+template <bool GATED> void launch_narrow_backward(hipStream_t s, const NarrowArgs& a, uint32_t blocks) {
+	const uint32_t cols = a.n * (GATED ? 2 : 1);
+	if (cols <= 64) launch_narrow_backward_n<4, GATED>(s, a, blocks); else if (cols <= 128) launch_narrow_backward_n<8, GATED>(s, a, blocks); else launch_narrow_backward_n<16, GATED>(s, a, blocks);
+}
 } // namespace
 
 void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
@@ -734,6 +966,10 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		else { if (d.gated) launch_few_rows<2, EPI_GATED>(s, g, partial); else launch_few_rows<2, EPI_LINEAR>(s, g, partial); }
 		return;
 	}
+	if (dense_narrow(d.m, d.n, d.k, d.gated) && d.k) {
+		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
+		return;
+	}
 	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
 	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes, partial); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes, partial);
 }
@@ -744,6 +980,22 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const bool bias = d.dbias[0] || d.dbias[1];
 	const bool identity = !d.gated && d.act == NGP_ACT_NONE; // G is dY as it stands
 	const bool products = d.dx || d.dw[0] || d.dw[1];
+	if (products && dense_narrow(d.m, d.n, d.k, d.gated) && d.n && d.k) {
+		NarrowArgs a{};
+		a.rows = d.m; a.n = d.n; a.k = d.k; a.act = d.act; a.x = (const T*)d.x; a.ld_x = d.x_stride; a.ld_w = d.w_stride; a.ld_pre = d.pre_stride; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride;
+		for (int i = 0; i < 2; ++i) { a.w[i] = (const T*)d.w[i]; a.pre[i] = (const T*)d.pre[i]; }
+		if (identity) a.pre[0] = nullptr;
+		if (!a.x) { a.x = a.dy; a.ld_x = 0; } // (dW is not wanted: nothing reads X's place)
+		a.dx = (T*)d.dx; a.ld_dx = d.dx_stride; a.partial = d.dw[0] ? (float*)(ws + p.partial) : nullptr; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr;
+		if (d.gated) launch_narrow_backward<true>(s, a, p.row_blocks); else launch_narrow_backward<false>(s, a, p.row_blocks);
+		if (bias) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, a.bias_partial, p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
+		if (a.partial) {
+			GemmArgs g{};
+			g.rows = d.n; g.cols = d.k; g.problems = problems; g.splits = p.row_blocks; g.partial = a.partial; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
+			hipLaunchKernelGGL((k_join_splits<EPI_STORE>), dim3(div_up((uint64_t)d.n * (up8(d.k) / 8), 256), problems), dim3(256), 0, s, g);
+		}
+		return;
+	}
 	const T* G = (const T*)d.dy; uint64_t ldg = d.dy_stride;
 	if ((!identity && products) || bias) {
 		GradArgs a{};

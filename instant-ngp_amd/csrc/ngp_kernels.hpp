@@ -382,10 +382,12 @@ inline uint64_t dense_split_bytes(uint64_t rows, uint64_t cols, uint64_t steps, 
 	const DenseSplit d = dense_split(rows, cols, steps, segments, parts);
 	return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0;
 }
+// layers that k_narrow_forward / k_narrow_backward take: all weights in one compute unit
+inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) { return m >= 2048 && k <= 256 && (gated ? 2 * (uint64_t)n : n) <= 256; }
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
-	return ((m <= FEW_ROWS ? few : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull;
+	return ((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull;
 }
 // Where the pieces of a backward pass lie in the workspace (bytes); from the sizes alone, so that ngp_*_workspace_size and the launch agree.
 struct DensePlan { uint64_t grad, bias, partial, bytes; uint32_t rows_per_block, row_blocks; };
@@ -394,6 +396,13 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t problems = gated ? 2 : 1;
 	const uint64_t n8 = ((uint64_t)n + 7) & ~7ull;
 	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
+	if (dense_narrow(m, n, k, gated)) { // one pass, a partial sum a block
+		const uint32_t slabs = (m + 31) / 32;
+		p.rows_per_block = 0; p.row_blocks = slabs < 256 ? slabs : 256;
+		p.grad = p.bias = 0; p.partial = up((uint64_t)problems * p.row_blocks * n * 4);
+		p.bytes = p.partial + up((uint64_t)problems * p.row_blocks * n * (((uint64_t)k + 7) & ~7ull) * 4);
+		return p;
+	}
 	// elementwise pass: about 1024 blocks of whole groups of 8 rows
 	const uint64_t col_blocks = ((uint64_t)n + 255) / 256, want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
 	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
