@@ -620,10 +620,21 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 		for (int k = 0; k < KS; ++k) x[k] = line8(line, k * 32 + gq * 8, steps, k >= whole_ks);
 	};
 	if (slab < slabs) load_x(slab);
-	for (int q = threadIdx.x; q < NF * KS * 64; q += 512) {
-		const int l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3);
-		const T* line = g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb;
-		*(T8*)(w + q * 8) = line8(line, k * 32 + (l >> 4) * 8, steps, true);
+	constexpr int EACH_THREAD = NF * KS / 8, BATCH = EACH_THREAD < 8 ? EACH_THREAD : 8;
+#pragma unroll
+	for (int q0 = 0; q0 < EACH_THREAD; q0 += BATCH) { // (all loads of a batch on their way together)
+		T8 v[BATCH];
+#pragma unroll
+		for (int b = 0; b < BATCH; ++b) {
+			const int q = (q0 + b) * 512 + threadIdx.x, l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3), c = k * 32 + (l >> 4) * 8;
+			const T* line = g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb;
+			v[b] = steps < 8 ? load8(line + c, steps - c) : load8(line + min(c, steps - 8));
+		}
+#pragma unroll
+		for (int b = 0; b < BATCH; ++b) {
+			const int q = (q0 + b) * 512 + threadIdx.x, c = ((q >> 6) % KS) * 32 + ((q & 63) >> 4) * 8;
+			*(T8*)(w + q * 8) = steps < 8 ? v[b] : shift8(v[b], c, steps);
+		}
 	}
 	__syncthreads();
 	for (; slab < slabs; slab += stride) {
@@ -651,20 +662,20 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 	}
 }
 // Backward in one pass: a block takes 32 samples at a time (the next 32 on their way), forms G = dY * act'(Z) and lays it and X into LDS; its 8 wavefronts multiply G with the weights
-// (in LDS as fragments) to dX, and G^T with X into their parts of dW, which stay in registers to the end: one partial sum a block, joined by a second launch.  Every sample's
+// (in LDS too) to dX, and G^T with X into their parts of dW, which stay in registers to the end: one partial sum a block, joined by a second launch.  Every sample's
 // dY, Z, X is read once, dX written once.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
 struct NarrowArgs {
 	uint32_t rows, n, k; int act; const T* x; uint64_t ld_x; const T* w[2]; uint64_t ld_w; const T* pre[2]; uint64_t ld_pre; const T* dy; uint64_t ld_dy; T* dx; uint64_t ld_dx;
 	float* partial; float* bias_partial;
 };
-template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void k_narrow_backward(NarrowArgs g) {
+template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 && KF <= 8 ? 4 : 2) void k_narrow_backward(NarrowArgs g) {
 	constexpr int GC = NF * 16, XC = KF * 16, HALF = GC / 2, NS = NF / 2; // columns of G and X in LDS, first column of the up projection, steps of 32 outputs
 	constexpr int CG = (GATED ? HALF : GC) / 8, CX = XC / 8, RG = 512 / CG, RX = 512 / CX, LG = RG >= 32 ? 1 : 32 / RG, LX = RX >= 32 ? 1 : 32 / RX; // chunks a line, lines at once, chunks a thread
 	constexpr int UNITS = KF * 2 / 8, WN = NF / 4, WK = KF / 2; // 16 x 16 pieces of dX a wavefront has, fragments of dW (4 x 2 wavefronts)
 	static_assert(NF >= 4 && KF >= 4, "");
 	constexpr int RL = RG < 32 ? RG : 32, SLABS = 32 * (GC + XC) * 2, RED = RL * GC * 4; // (the bias's sums take the slabs' place at the end)
-	__shared__ __attribute__((aligned(16))) char shared[KF * NS * 1024 + (SLABS > RED ? SLABS : RED)];
-	T* wf = (T*)shared; T* lg = wf + KF * NS * 512; T* lx = lg + 32 * GC;
+	__shared__ __attribute__((aligned(16))) char shared[GC * XC * 2 + (SLABS > RED ? SLABS : RED)];
+	T* lw = (T*)shared; T* lg = lw + GC * XC; T* lx = lg + 32 * GC; // weights, G, X
 	const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), gq = lane >> 4, li = lane & 15, l4 = li >> 2;
 	const int gc = (tid % CG) * 8, gr = tid / CG, xc = (tid % CX) * 8, xr = tid / CX;
 	const uint32_t slabs = (g.rows + 31) / 32;
@@ -685,17 +696,29 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void 
 	};
 	uint32_t s = blockIdx.x;
 	if (s < slabs) load(s);
-	// the weights as fragments: 16 inputs, 32 outputs (8 a lane)
-	if (g.dx) {
-		for (int q = tid; q < KF * NS * 64; q += 512) {
-			const int l = q & 63, n0 = ((q >> 6) % NS) * 32 + (l >> 4) * 8, k = ((q >> 6) / NS) * 16 + (l & 15);
-			T8 v{};
+	auto tr8 = [&](const T* base, int cols, int line0, int f) -> T8 { // 8 of the 32 lines from line0 on, of column 16 f + li
+		const int line = line0 + gq * 8 + l4, e = f * 16 + (li & 3) * 4;
+		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + line * cols + slot(line, e >> 3, cols / 8) * 8 + (e & 7)));
+		const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + (line + 4) * cols + slot(line + 4, e >> 3, cols / 8) * 8 + (e & 7)));
+		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+	};
+	if (g.dx) { // the weights: lines behind the last output meet zeros of G, but must not be NaN
+		constexpr int EACH_THREAD = GC * XC / 8 / 512, BATCH = EACH_THREAD < 8 ? EACH_THREAD : 8;
 #pragma unroll
-			for (int e = 0; e < 8; ++e) {
-				const int c = n0 + e, n = GATED && c >= HALF ? c - HALF : c;
-				if (n < (int)g.n && k < (int)g.k) v[e] = g.w[GATED && c >= HALF][(uint64_t)n * g.ld_w + k];
+		for (int q0 = 0; q0 < EACH_THREAD; q0 += BATCH) {
+			T8 v[BATCH];
+#pragma unroll
+			for (int b = 0; b < BATCH; ++b) {
+				const int q = (q0 + b) * 512 + tid, line = q / CX, c = (q % CX) * 8, up = GATED && line >= HALF, n = line - up * HALF;
+				const T* p = g.w[up] + (uint64_t)min((uint32_t)n, g.n - 1) * g.ld_w;
+				v[b] = g.k < 8 ? load8(p + c, (int)g.k - c) : load8(p + min(c, (int)g.k - 8));
 			}
-			*(T8*)(wf + q * 8) = v;
+#pragma unroll
+			for (int b = 0; b < BATCH; ++b) {
+				const int q = (q0 + b) * 512 + tid, line = q / CX, c = (q % CX) * 8, n = line - (GATED && line >= HALF) * HALF;
+				const T8 w = ragged_k && g.k >= 8 ? shift8(v[b], c, g.k) : v[b];
+				*(T8*)(lw + line * XC + slot(line, c / 8, CX) * 8) = n < (int)g.n ? w : T8{};
+			}
 		}
 	}
 	float sum[GATED ? 2 : 1][8] = {};
@@ -739,7 +762,7 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void 
 			for (int q = 0; q < UNITS; ++q) d[q] = f4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 			for (int ns = 0; ns < NS; ++ns) {
-				T8 a[2];
+				T8 a[2], b;
 #pragma unroll
 				for (int h = 0; h < (UNITS == 1 ? 1 : 2); ++h) {
 					const int line = (UNITS == 1 ? (int)(wave & 1) : h) * 16 + li;
@@ -748,7 +771,8 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void 
 #pragma unroll
 				for (int q = 0; q < UNITS; ++q) {
 					const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q / 2;
-					d[q] = mfma(*(const T8*)(wf + ((kf * NS + ns) * 64 + lane) * 8), a[UNITS == 1 ? 0 : q & 1], d[q]);
+					if (UNITS == 1 || !(q & 1)) b = tr8(lw, XC, ns * 32, kf);
+					d[q] = mfma(b, a[UNITS == 1 ? 0 : q & 1], d[q]);
 				}
 			}
 #pragma unroll
@@ -767,18 +791,12 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, 2) void 
 			}
 		}
 		if (g.partial) {
-			auto tr8 = [&](const T* base, int cols, int f) -> T8 { // 8 samples (of 32) of column 16 f + li
-				const int line = gq * 8 + l4, e = f * 16 + (li & 3) * 4;
-				const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + line * cols + slot(line, e >> 3, cols / 8) * 8 + (e & 7)));
-				const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + (line + 4) * cols + slot(line + 4, e >> 3, cols / 8) * 8 + (e & 7)));
-				return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-			};
 			T8 a[WN];
 #pragma unroll
-			for (int i = 0; i < WN; ++i) a[i] = tr8(lg, GC, (wave >> 1) * WN + i);
+			for (int i = 0; i < WN; ++i) a[i] = tr8(lg, GC, 0, (wave >> 1) * WN + i);
 #pragma unroll
 			for (int j = 0; j < WK; ++j) {
-				const T8 b = tr8(lx, XC, (wave & 1) * WK + j);
+				const T8 b = tr8(lx, XC, 0, (wave & 1) * WK + j);
 #pragma unroll
 				for (int i = 0; i < WN; ++i) acc[i][j] = mfma(b, a[i], acc[i][j]);
 			}
@@ -874,33 +892,49 @@ __global__ __launch_bounds__(1024) void k_bias_grad(const float* partial, uint32
 		if (out) out[c] = (T)t;
 	}
 }
-// the splits' sums in their order, then the product's own epilogue (EPI_GATED: partial sums of both projections)
-template <int EPI> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs g) {
-	const uint32_t cc = up8(g.cols) / 8, problem = blockIdx.y, parts = EPI == EPI_GATED ? 2 : g.problems;
-	const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-	if (id >= (uint64_t)g.rows * cc) return;
-	const uint32_t r = (uint32_t)(id / cc), c = (uint32_t)(id % cc) * 8;
+// the splits' sums, GROUPS threads sharing them out (in a fixed order), then the product's own epilogue (EPI_GATED: partial sums of both projections)
+template <int EPI, int GROUPS> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs g) {
+	constexpr int P = EPI == EPI_GATED ? 2 : 1, ITEMS = 256 / GROUPS;
+	__shared__ float red[GROUPS > 1 ? GROUPS : 1][P][GROUPS > 1 ? ITEMS : 1][9];
+	const uint32_t cc = up8(g.cols) / 8, problem = blockIdx.y, parts = P == 2 ? 2 : g.problems, item = threadIdx.x % ITEMS, group = threadIdx.x / ITEMS;
+	const uint64_t id = (uint64_t)blockIdx.x * ITEMS + item;
+	const bool in = id < (uint64_t)g.rows * cc;
+	if (GROUPS == 1 && !in) return;
+	const uint32_t r = in ? (uint32_t)(id / cc) : 0, c = in ? (uint32_t)(id % cc) * 8 : 0;
 	const uint64_t part = (uint64_t)g.rows * cc * 8;
 	const int n = (int)min(8u, g.cols - c);
-	const T8 bias0 = bias8<EPI>(g, 0, c, n), bias1 = bias8<EPI>(g, 1, c, n), residual = residual8<EPI>(g, r, c, n);
+	T8 bias0{}, bias1{}, residual{};
+	if (group == 0) { bias0 = bias8<EPI>(g, 0, c, n); bias1 = bias8<EPI>(g, 1, c, n); residual = residual8<EPI>(g, r, c, in ? n : 0); }
 	float z[8] = {}, u[8] = {};
-	const float* p = g.partial + problem * part + (uint64_t)r * cc * 8 + c;
+	const float* p = g.partial + problem * part + (uint64_t)r * cc * 8 + c + (uint64_t)group * parts * part;
 #pragma unroll 4
-	for (uint32_t k = 0; k < g.splits; ++k, p += parts * part) {
+	for (uint32_t k = group; k < g.splits; k += GROUPS, p += (uint64_t)GROUPS * parts * part) {
 		const f4v a = *(const f4v*)p, b = *(const f4v*)(p + 4);
 #pragma unroll
 		for (int e = 0; e < 4; ++e) { z[e] += a[e]; z[e + 4] += b[e]; }
-		if constexpr (EPI == EPI_GATED) {
+		if constexpr (P == 2) {
 			const f4v d = *(const f4v*)(p + part), f = *(const f4v*)(p + part + 4);
 #pragma unroll
 			for (int e = 0; e < 4; ++e) { u[e] += d[e]; u[e + 4] += f[e]; }
 		}
+	}
+	if constexpr (GROUPS > 1) {
+		EACH { red[group][0][item][e] = z[e]; if (P == 2) red[group][P - 1][item][e] = u[e]; }
+		__syncthreads();
+		if (group || !in) return;
+#pragma unroll
+		for (int q = 1; q < GROUPS; ++q) EACH { z[e] += red[q][0][item][e]; if (P == 2) u[e] += red[q][P - 1][item][e]; }
 	}
 	epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual);
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
+template <int EPI> void launch_join(hipStream_t s, const GemmArgs& g) {
+	const uint64_t items = (uint64_t)g.rows * (up8(g.cols) / 8);
+	if (g.splits >= 16) hipLaunchKernelGGL((k_join_splits<EPI, 8>), dim3(div_up(items, 32), g.problems), dim3(256), 0, s, g);
+	else hipLaunchKernelGGL((k_join_splits<EPI, 1>), dim3(div_up(items, 256), g.problems), dim3(256), 0, s, g);
+}
 // `wholes`: both operands come in whole 16-byte pieces
 template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs& g, bool wholes, bool large) {
 	constexpr int K = GATED_TILE<EPI> ? 2 : 1; // weight columns per column of C
@@ -919,7 +953,7 @@ template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs&
 	if (d.splits > 1) {
 		g.splits = d.splits; g.partial = partial;
 		launch_tiles<A_T, B_T, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>(s, g, wholes, wholes && d.large);
-		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), g.problems), dim3(256), 0, s, g);
+		launch_join<EPI>(s, g);
 	} else launch_tiles<A_T, B_T, EPI>(s, g, wholes, wholes && d.large);
 }
 template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, float* partial) {
@@ -929,7 +963,7 @@ template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, floa
 	g.splits = f.splits; g.partial = partial;
 	if (f.splits > 1) {
 		hipLaunchKernelGGL((k_few_rows<MT, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>), grid, dim3(512), 0, s, g, f.slices, per);
-		hipLaunchKernelGGL((k_join_splits<EPI>), dim3(div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256), 1), dim3(256), 0, s, g);
+		launch_join<EPI>(s, g);
 	} else hipLaunchKernelGGL((k_few_rows<MT, EPI>), grid, dim3(512), 0, s, g, f.slices, per);
 }
 template <int NF, int EPI> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
@@ -992,7 +1026,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		if (a.partial) {
 			GemmArgs g{};
 			g.rows = d.n; g.cols = d.k; g.problems = problems; g.splits = p.row_blocks; g.partial = a.partial; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
-			hipLaunchKernelGGL((k_join_splits<EPI_STORE>), dim3(div_up((uint64_t)d.n * (up8(d.k) / 8), 256), problems), dim3(256), 0, s, g);
+			launch_join<EPI_STORE>(s, g);
 		}
 		return;
 	}

@@ -398,7 +398,8 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
 	if (dense_narrow(m, n, k, gated)) { // one pass, a partial sum a block
 		const uint32_t slabs = (m + 31) / 32;
-		p.rows_per_block = 0; p.row_blocks = slabs < 256 ? slabs : 256;
+		const uint32_t most = (gated ? 2 * n : n) <= 128 && k <= 128 ? 512 : 256; // two blocks a compute unit where their registers and LDS allow it
+		p.rows_per_block = 0; p.row_blocks = slabs < most ? slabs : most;
 		p.grad = p.bias = 0; p.partial = up((uint64_t)problems * p.row_blocks * n * 4);
 		p.bytes = p.partial + up((uint64_t)problems * p.row_blocks * n * (((uint64_t)k + 7) & ~7ull) * 4);
 		return p;
