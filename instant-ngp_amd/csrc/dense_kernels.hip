@@ -79,11 +79,25 @@ __device__ inline T8 shift8(T8 raw, int c, int width) {
 	__builtin_memcpy(&r, t, 16);
 	return r;
 }
+// COUNT chunks of 8 elements of lines of one width, all on their way together: at(q, line) gives the line and returns the column.  Lines of 8 elements and more are read in whole chunks
+// (at min(column, width - 8): shift8 puts them right later), shorter ones element by element.
+template <int COUNT, typename F> __device__ inline void load_chunks(T8* out, int width, F&& at) {
+	if (width >= 8) {
+#pragma unroll
+		for (int q = 0; q < COUNT; ++q) { const T* line; const int c = at(q, line); out[q] = load8(line + min(c, width - 8)); }
+	} else {
+#pragma unroll
+		for (int q = 0; q < COUNT; ++q) { const T* line; const int c = at(q, line); out[q] = load8(line + c, width - c); }
+	}
+}
 __device__ inline void store8(T* p, T8 v, int n) {
 	if (n >= 8) { __builtin_memcpy(p, &v, 16); return; }
 #pragma unroll
 	for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
 }
+
+// a barrier that waits for LDS alone: loads and stores stay on their way
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // ---- activations: values and derivatives in 32 bits.  1 / (1 + e^-z) through v_exp_f32 / v_rcp_f32 (1 ulp each): far below the 16-bit rounding of the result
 __device__ inline float logistic(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
@@ -109,14 +123,17 @@ __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 va
 		default: break;
 	}
 }
-__device__ inline void act_value_slope8(int act, const float z[8], float value[8], float slope[8]) {
+// G of 8 outputs: dY act'(Z); gated: dY Zu act'(Zg) and dY act(Zg).  Zeros give zeros.
+template <bool GATED> __device__ inline void output_grad8(int act, const T8& dy, const T8& zt, const T8& ut, float g[8], float g2[8]) {
+	float d[8], m[8], z[8];
+	EACH { d[e] = (float)dy[e]; z[e] = (float)zt[e]; m[e] = GATED ? d[e] * (float)ut[e] : d[e]; }
 	switch (act) {
-		case NGP_ACT_RELU: EACH { value[e] = z[e] < 0.f ? 0.f : z[e]; slope[e] = z[e] > 0.f ? 1.f : 0.f; } break;
-		case NGP_ACT_LOGISTIC: EACH { const float p = logistic(z[e]); value[e] = p; slope[e] = p * (1.f - p); } break;
-		case NGP_ACT_EXPONENTIAL: EACH value[e] = slope[e] = __expf(z[e]); break;
-		case NGP_ACT_SILU: EACH { const float p = logistic(z[e]); value[e] = z[e] * p; slope[e] = p * (1.f + z[e] * (1.f - p)); } break;
-		case NGP_ACT_GELU: EACH { float x; const float c = normal_cdf(z[e], x); value[e] = z[e] * c; slope[e] = fmaf(z[e] * 0.39894228f, x, c); } break;
-		default: EACH { value[e] = z[e]; slope[e] = 1.f; } break;
+		case NGP_ACT_RELU: EACH { g[e] = z[e] > 0.f ? m[e] : 0.f; if (GATED) g2[e] = z[e] > 0.f ? d[e] * z[e] : 0.f; } break; // (a closed unit passes nothing, whatever arrives)
+		case NGP_ACT_LOGISTIC: EACH { const float p = logistic(z[e]); g[e] = m[e] * (p * (1.f - p)); if (GATED) g2[e] = d[e] * p; } break;
+		case NGP_ACT_EXPONENTIAL: EACH { const float p = __expf(z[e]); g[e] = m[e] * p; if (GATED) g2[e] = d[e] * p; } break;
+		case NGP_ACT_SILU: EACH { const float p = logistic(z[e]); g[e] = m[e] * (p * fmaf(z[e], 1.f - p, 1.f)); if (GATED) g2[e] = d[e] * (z[e] * p); } break;
+		case NGP_ACT_GELU: EACH { float x; const float c = normal_cdf(z[e], x); g[e] = m[e] * fmaf(z[e] * 0.39894228f, x, c); if (GATED) g2[e] = d[e] * (z[e] * c); } break;
+		default: EACH { g[e] = m[e]; if (GATED) g2[e] = d[e] * z[e]; } break;
 	}
 }
 
@@ -234,16 +251,13 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	// there; beyond the sum's last step both operands are zero (put right on the way to LDS, when the loads have arrived).
 	auto load_operand = [&](auto tile_c, auto contig_c, T8* out, auto count_c, auto&& matrix, uint64_t ld, uint32_t e0, uint32_t extent, uint32_t t0, int left) {
 		typedef decltype(tile_c) TX; constexpr bool CONTIG = decltype(contig_c)::value; constexpr int COUNT = decltype(count_c)::value;
-		const int width = CONTIG ? (int)g.steps : (int)extent;
-#pragma unroll
-		for (int q = 0; q < COUNT; ++q) {
+		load_chunks<COUNT>(out, CONTIG ? (int)g.steps : (int)extent, [&](int q, const T*& p) -> int {
 			const int slot = q * THREADS + tid, line = slot / TX::SLOTS, chunk = TX::source(line, slot % TX::SLOTS);
 			uint32_t in_tile = line; // (CONTIG)
 			const T* base = matrix(in_tile);
-			const T* p = CONTIG ? base + (uint64_t)min(e0 + in_tile, extent - 1) * ld : base + (uint64_t)(t0 + min(line, left - 1)) * ld;
-			const int c = (CONTIG ? (int)t0 : (int)e0) + chunk * 8;
-			if (width < 8) out[q] = load8(p + c, width - c); else out[q] = load8(p + min(c, width - 8));
-		}
+			p = CONTIG ? base + (uint64_t)min(e0 + in_tile, extent - 1) * ld : base + (uint64_t)(t0 + min(line, left - 1)) * ld;
+			return (CONTIG ? (int)t0 : (int)e0) + chunk * 8;
+		});
 	};
 	auto to_lds = [&](auto tile_c, auto contig_c, T8* in, auto count_c, T* lds, uint32_t e0, uint32_t extent, uint32_t t0, int left) {
 		typedef decltype(tile_c) TX; constexpr bool CONTIG = decltype(contig_c)::value; constexpr int COUNT = decltype(count_c)::value;
@@ -601,10 +615,6 @@ template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(Gem
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
-__device__ inline T8 line8(const T* line, int c, int width, bool ragged /* uniform: c + 8 may pass the line's end */) { // zeros behind the end
-	if (!ragged) return load8(line + c);
-	return width < 8 ? load8(line + c, width - c) : shift8(load8(line + min(c, width - 8)), c, width);
-}
 template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int OF = GATED ? NF / 2 : NF; // fragments of outputs
@@ -617,7 +627,12 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 	auto load_x = [&](uint32_t s) {
 		const T* line = g.a + (uint64_t)min(s * 16 + li, g.rows - 1) * g.lda; // (samples behind the last one repeat it and are dropped)
 #pragma unroll
-		for (int k = 0; k < KS; ++k) x[k] = line8(line, k * 32 + gq * 8, steps, k >= whole_ks);
+		for (int k = 0; k < KS; ++k) x[k] = load8(line + min(k * 32 + (int)gq * 8, steps - 8));
+	};
+	auto tail_x = [&]() { // the line's end
+		if (whole_ks == KS) return;
+#pragma unroll
+		for (int k = 0; k < KS; ++k) if (k >= whole_ks) x[k] = shift8(x[k], k * 32 + gq * 8, steps);
 	};
 	if (slab < slabs) load_x(slab);
 	constexpr int EACH_THREAD = NF * KS / 8, BATCH = EACH_THREAD < 8 ? EACH_THREAD : 8;
@@ -626,14 +641,13 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 		T8 v[BATCH];
 #pragma unroll
 		for (int b = 0; b < BATCH; ++b) {
-			const int q = (q0 + b) * 512 + threadIdx.x, l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3), c = k * 32 + (l >> 4) * 8;
-			const T* line = g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb;
-			v[b] = steps < 8 ? load8(line + c, steps - c) : load8(line + min(c, steps - 8));
+			const int q = (q0 + b) * 512 + threadIdx.x, l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3);
+			v[b] = load8(g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb + min(k * 32 + (l >> 4) * 8, steps - 8));
 		}
 #pragma unroll
 		for (int b = 0; b < BATCH; ++b) {
 			const int q = (q0 + b) * 512 + threadIdx.x, c = ((q >> 6) % KS) * 32 + ((q & 63) >> 4) * 8;
-			*(T8*)(w + q * 8) = steps < 8 ? v[b] : shift8(v[b], c, steps);
+			*(T8*)(w + q * 8) = steps == KS * 32 ? v[b] : shift8(v[b], c, steps);
 		}
 	}
 	__syncthreads();
@@ -642,6 +656,7 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 		f4v acc[NF];
 #pragma unroll
 		for (int f = 0; f < NF; ++f) acc[f] = f4v{0.f, 0.f, 0.f, 0.f};
+		tail_x();
 #pragma unroll
 		for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -684,15 +699,30 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 	auto slot = [](int line, int s, int slots) -> int { return s ^ ((((line & 3) << 1) | (line & 8) | ((line >> 2) & 1)) & (slots >= 16 ? 15 : slots - 1)); };
 	T8 dy[LG], z[LG], u[GATED ? LG : 1], x[LX];
 	auto load = [&](uint32_t s) {
+		if (RG < 32 || gr < 32) {
 #pragma unroll
-		for (int q = 0; q < LG; ++q) if (RG < 32 || gr < 32) {
-			const uint64_t r = min(s * 32 + gr + q * RG, g.rows - 1);
-			dy[q] = line8(g.dy + r * g.ld_dy, gc, g.n, ragged_n);
-			if (g.pre[0]) z[q] = line8(g.pre[0] + r * g.ld_pre, gc, g.n, ragged_n); else z[q] = T8{};
-			if (GATED) u[GATED ? q : 0] = line8(g.pre[1] + r * g.ld_pre, gc, g.n, ragged_n);
+			for (int q = 0; q < LG; ++q) {
+				const uint64_t r = min(s * 32 + gr + q * RG, g.rows - 1);
+				const int c = min(gc, (int)g.n - 8);
+				dy[q] = load8(g.dy + r * g.ld_dy + c);
+				z[q] = load8(g.pre[0] + r * g.ld_pre + c);
+				if (GATED) u[GATED ? q : 0] = load8(g.pre[1] + r * g.ld_pre + c);
+			}
 		}
+		if (RX < 32 || xr < 32) {
 #pragma unroll
-		for (int q = 0; q < LX; ++q) if (RX < 32 || xr < 32) x[q] = line8(g.x + (uint64_t)min(s * 32 + xr + q * RX, g.rows - 1) * g.ld_x, xc, g.k, ragged_k);
+			for (int q = 0; q < LX; ++q) x[q] = load8(g.x + (uint64_t)min(s * 32 + xr + q * RX, g.rows - 1) * g.ld_x + min(xc, (int)g.k - 8));
+		}
+	};
+	auto tails = [&]() { // the lines' ends
+		if (ragged_n) {
+#pragma unroll
+			for (int q = 0; q < LG; ++q) { dy[q] = shift8(dy[q], gc, g.n); z[q] = shift8(z[q], gc, g.n); if (GATED) u[GATED ? q : 0] = shift8(u[GATED ? q : 0], gc, g.n); }
+		}
+		if (ragged_k) {
+#pragma unroll
+			for (int q = 0; q < LX; ++q) x[q] = shift8(x[q], xc, g.k);
+		}
 	};
 	uint32_t s = blockIdx.x;
 	if (s < slabs) load(s);
@@ -709,14 +739,13 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 			T8 v[BATCH];
 #pragma unroll
 			for (int b = 0; b < BATCH; ++b) {
-				const int q = (q0 + b) * 512 + tid, line = q / CX, c = (q % CX) * 8, up = GATED && line >= HALF, n = line - up * HALF;
-				const T* p = g.w[up] + (uint64_t)min((uint32_t)n, g.n - 1) * g.ld_w;
-				v[b] = g.k < 8 ? load8(p + c, (int)g.k - c) : load8(p + min(c, (int)g.k - 8));
+				const int q = (q0 + b) * 512 + tid, l = q / CX, up = GATED && l >= HALF, n = l - up * HALF;
+				v[b] = load8(g.w[up] + (uint64_t)min((uint32_t)n, g.n - 1) * g.ld_w + min((q % CX) * 8, (int)g.k - 8));
 			}
 #pragma unroll
 			for (int b = 0; b < BATCH; ++b) {
 				const int q = (q0 + b) * 512 + tid, line = q / CX, c = (q % CX) * 8, n = line - (GATED && line >= HALF) * HALF;
-				const T8 w = ragged_k && g.k >= 8 ? shift8(v[b], c, g.k) : v[b];
+				const T8 w = ragged_k ? shift8(v[b], c, g.k) : v[b];
 				*(T8*)(lw + line * XC + slot(line, c / 8, CX) * 8) = n < (int)g.n ? w : T8{};
 			}
 		}
@@ -729,63 +758,56 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 		for (int j = 0; j < WK; ++j) acc[i][j] = f4v{0.f, 0.f, 0.f, 0.f};
 	for (; s < slabs; s += gridDim.x) {
 		// G and X into LDS; samples behind the last one are zero
+		const bool last = s * 32 + 32 > g.rows;
+		tails();
 #pragma unroll
 		for (int q = 0; q < LG; ++q) if (RG < 32 || gr < 32) {
 			const int line = gr + q * RG;
-			const bool in = s * 32 + line < g.rows;
-			float zf[8], value[8], slope[8];
+			if (last && s * 32 + line >= g.rows) { dy[q] = z[q] = T8{}; u[GATED ? q : 0] = T8{}; }
+			float v[8], v2[8];
 			T8 o, o2;
-			EACH zf[e] = (float)z[q][e];
-			act_value_slope8(g.act, zf, value, slope);
-#pragma unroll
-			for (int e = 0; e < 8; ++e) {
-				const bool live = in && gc + e < (int)g.n;
-				const float v = live && slope[e] != 0.f ? (GATED ? (float)dy[q][e] * (float)u[GATED ? q : 0][e] * slope[e] : (float)dy[q][e] * slope[e]) : 0.f; // (a closed unit passes nothing, whatever arrives)
-				sum[0][e] += v; o[e] = (T)v;
-				if (GATED) { const float v2 = live ? (float)dy[q][e] * value[e] : 0.f; sum[GATED ? 1 : 0][e] += v2; o2[e] = (T)v2; }
-			}
+			output_grad8<GATED>(g.act, dy[q], z[q], u[GATED ? q : 0], v, v2);
+			EACH { sum[0][e] += v[e]; o[e] = (T)v[e]; if (GATED) { sum[GATED ? 1 : 0][e] += v2[e]; o2[e] = (T)v2[e]; } }
 			*(T8*)(lg + line * GC + slot(line, gc / 8, GC / 8) * 8) = o;
 			if (GATED) *(T8*)(lg + line * GC + slot(line, (HALF + gc) / 8, GC / 8) * 8) = o2;
 		}
 #pragma unroll
 		for (int q = 0; q < LX; ++q) if (RX < 32 || xr < 32) {
 			const int line = xr + q * RX;
-			*(T8*)(lx + line * XC + slot(line, xc / 8, XC / 8) * 8) = s * 32 + line < g.rows ? x[q] : T8{};
+			*(T8*)(lx + line * XC + slot(line, xc / 8, XC / 8) * 8) = last && s * 32 + line >= g.rows ? T8{} : x[q];
 		}
-		__syncthreads();
 		const uint32_t here = s;
 		if (s + gridDim.x < slabs) load(s + gridDim.x);
+		lds_barrier();
 		if (g.dx) {
-			f4v d[UNITS];
-			// pieces of 16 samples x 16 inputs: the wavefronts share out the inputs first
+			// pieces of 16 samples x 16 inputs: the wavefronts share out the inputs first, two pieces (both halves of the samples) at a time
+			constexpr int PAIR = UNITS == 1 ? 1 : 2;
+#pragma unroll 1
+			for (int q = 0; q < UNITS / PAIR; ++q) {
+				const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q;
+				f4v d[PAIR];
 #pragma unroll
-			for (int q = 0; q < UNITS; ++q) d[q] = f4v{0.f, 0.f, 0.f, 0.f};
+				for (int h = 0; h < PAIR; ++h) d[h] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+				for (int ns = 0; ns < NS; ++ns) {
+					const T8 b = tr8(lw, XC, ns * 32, kf);
 #pragma unroll
-			for (int ns = 0; ns < NS; ++ns) {
-				T8 a[2], b;
-#pragma unroll
-				for (int h = 0; h < (UNITS == 1 ? 1 : 2); ++h) {
-					const int line = (UNITS == 1 ? (int)(wave & 1) : h) * 16 + li;
-					a[h] = *(const T8*)(lg + line * GC + slot(line, ns * 4 + gq, GC / 8) * 8);
+					for (int h = 0; h < PAIR; ++h) {
+						const int line = (UNITS == 1 ? (int)(wave & 1) : h) * 16 + li;
+						d[h] = mfma(b, *(const T8*)(lg + line * GC + slot(line, ns * 4 + gq, GC / 8) * 8), d[h]);
+					}
 				}
 #pragma unroll
-				for (int q = 0; q < UNITS; ++q) {
-					const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q / 2;
-					if (UNITS == 1 || !(q & 1)) b = tr8(lw, XC, ns * 32, kf);
-					d[q] = mfma(b, a[UNITS == 1 ? 0 : q & 1], d[q]);
-				}
-			}
+				for (int h = 0; h < PAIR; ++h) {
+					const uint32_t r = here * 32 + (UNITS == 1 ? wave & 1 : h) * 16 + li, c = kf * 16 + gq * 4;
+					if (r < g.rows && c < g.k) {
+						T* o = g.dx + (uint64_t)r * g.ld_dx + c;
+						T v[4] = {(T)d[h][0], (T)d[h][1], (T)d[h][2], (T)d[h][3]};
+						if (c + 4 <= g.k) __builtin_memcpy(o, v, 8);
+						else {
 #pragma unroll
-			for (int q = 0; q < UNITS; ++q) {
-				const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q / 2;
-				const uint32_t r = here * 32 + (UNITS == 1 ? wave & 1 : q & 1) * 16 + li, c = kf * 16 + gq * 4;
-				if (r < g.rows && c < g.k) {
-					T* o = g.dx + (uint64_t)r * g.ld_dx + c;
-					T v[4] = {(T)d[q][0], (T)d[q][1], (T)d[q][2], (T)d[q][3]};
-					if (c + 4 <= g.k) __builtin_memcpy(o, v, 8);
-					else {
-#pragma unroll
-						for (int e = 0; e < 3; ++e) if (c + e < g.k) o[e] = v[e];
+							for (int e = 0; e < 3; ++e) if (c + e < g.k) o[e] = v[e];
+						}
 					}
 				}
 			}
@@ -801,7 +823,7 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 				for (int i = 0; i < WN; ++i) acc[i][j] = mfma(b, a[i], acc[i][j]);
 			}
 		}
-		__syncthreads();
+		lds_barrier();
 	}
 	if (g.partial) {
 		const uint32_t k8 = up8(g.k);
@@ -843,15 +865,9 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 			T8 z{}, u{}, o, o2;
 			if (g.pre[0]) z = load8(g.pre[0] + (uint64_t)r * g.ld_pre + c, n);
 			if (GATED) u = load8(g.pre[1] + (uint64_t)r * g.ld_pre + c, n);
-			float zf[8], value[8], slope[8];
-			EACH zf[e] = (float)z[e];
-			act_value_slope8(g.act, zf, value, slope);
-#pragma unroll
-			for (int e = 0; e < 8; ++e) {
-				const float v = e < n && slope[e] != 0.f ? (GATED ? (float)dy[e] * (float)u[e] * slope[e] : (float)dy[e] * slope[e]) : 0.f; // (a closed unit passes nothing, whatever arrives)
-				sum[0][e] += v; o[e] = (T)v;
-				if (GATED) { const float w = e < n ? (float)dy[e] * value[e] : 0.f; sum[GATED ? 1 : 0][e] += w; o2[e] = (T)w; }
-			}
+			float v[8], v2[8];
+			output_grad8<GATED>(g.act, dy, z, u, v, v2);
+			EACH { sum[0][e] += v[e]; o[e] = (T)v[e]; if (GATED) { sum[GATED ? 1 : 0][e] += v2[e]; o2[e] = (T)v2[e]; } }
 			if (g.out) {
 				*(T8*)(g.out + (uint64_t)r * g.ld_out + c) = o;
 				if (GATED) *(T8*)(g.out + (uint64_t)r * g.ld_out + pc + c) = o2;
@@ -1018,8 +1034,8 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		NarrowArgs a{};
 		a.rows = d.m; a.n = d.n; a.k = d.k; a.act = d.act; a.x = (const T*)d.x; a.ld_x = d.x_stride; a.ld_w = d.w_stride; a.ld_pre = d.pre_stride; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride;
 		for (int i = 0; i < 2; ++i) { a.w[i] = (const T*)d.w[i]; a.pre[i] = (const T*)d.pre[i]; }
-		if (identity) a.pre[0] = nullptr;
-		if (!a.x) { a.x = a.dy; a.ld_x = 0; } // (dW is not wanted: nothing reads X's place)
+		if (identity) { a.pre[0] = a.dy; a.ld_pre = a.ld_dy; } // (read, not used)
+		if (!a.x) { a.x = a.dy; a.ld_x = 0; }                  // (dW is not wanted: nothing reads X's place)
 		a.dx = (T*)d.dx; a.ld_dx = d.dx_stride; a.partial = d.dw[0] ? (float*)(ws + p.partial) : nullptr; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr;
 		if (d.gated) launch_narrow_backward<true>(s, a, p.row_blocks); else launch_narrow_backward<false>(s, a, p.row_blocks);
 		if (bias) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, a.bias_partial, p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);

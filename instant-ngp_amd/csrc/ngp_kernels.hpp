@@ -383,7 +383,7 @@ inline uint64_t dense_split_bytes(uint64_t rows, uint64_t cols, uint64_t steps, 
 	return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0;
 }
 // layers that k_narrow_forward / k_narrow_backward take: all weights in one compute unit
-inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) { return m >= 2048 && k <= 256 && (gated ? 2 * (uint64_t)n : n) <= 256; }
+inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) { return m >= 2048 && n >= 8 && k >= 8 && k <= 256 && (gated ? 2 * (uint64_t)n : n) <= 256; }
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
