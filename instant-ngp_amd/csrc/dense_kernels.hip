@@ -726,12 +726,13 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 	};
 	uint32_t s = blockIdx.x;
 	if (s < slabs) load(s);
-	auto tr8 = [&](const T* base, int cols, int line0, int f) -> T8 { // 8 of the 32 lines from line0 on, of column 16 f + li
-		const int line = line0 + gq * 8 + l4, e = f * 16 + (li & 3) * 4;
+	auto tr8_at = [&](const T* base, int cols, int line0, int e) -> T8 { // 8 of the 32 lines from line0 on, of the column whose group of 4 the lane reads at e
+		const int line = line0 + gq * 8 + l4;
 		const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + line * cols + slot(line, e >> 3, cols / 8) * 8 + (e & 7)));
 		const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + (line + 4) * cols + slot(line + 4, e >> 3, cols / 8) * 8 + (e & 7)));
 		return __builtin_bit_cast(T8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 	};
+	auto tr8 = [&](const T* base, int cols, int line0, int f) -> T8 { return tr8_at(base, cols, line0, f * 16 + (li & 3) * 4); }; // of column 16 f + li
 	if (g.dx) { // the weights: lines behind the last output meet zeros of G, but must not be NaN
 		constexpr int EACH_THREAD = GC * XC / 8 / 512, BATCH = EACH_THREAD < 8 ? EACH_THREAD : 8;
 #pragma unroll
@@ -780,33 +781,44 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 		if (s + gridDim.x < slabs) load(s + gridDim.x);
 		lds_barrier();
 		if (g.dx) {
-			// pieces of 16 samples x 16 inputs: the wavefronts share out the inputs first, two pieces (both halves of the samples) at a time
+			// pieces of 16 samples x 16 inputs, two at a time: with 256 inputs a wavefront has 32 of them, dealt to two fragments so that a lane owns 8 consecutive ones; with 128 it has 16, of both
+			// halves of the samples; with 64 one piece
+			constexpr bool WIDE = UNITS == 4;
 			constexpr int PAIR = UNITS == 1 ? 1 : 2;
 #pragma unroll 1
 			for (int q = 0; q < UNITS / PAIR; ++q) {
-				const int kf = UNITS == 1 ? wave >> 1 : wave * (UNITS / 2) + q;
+				const int kf = UNITS == 1 ? wave >> 1 : WIDE ? wave * 2 : wave;
 				f4v d[PAIR];
 #pragma unroll
 				for (int h = 0; h < PAIR; ++h) d[h] = f4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+				auto rows_at = [&](int h) -> int { return UNITS == 1 ? (int)(wave & 1) * 16 : WIDE ? q * 16 : h * 16; };
+#pragma unroll 4
 				for (int ns = 0; ns < NS; ++ns) {
-					const T8 b = tr8(lw, XC, ns * 32, kf);
+					T8 a, b;
 #pragma unroll
 					for (int h = 0; h < PAIR; ++h) {
-						const int line = (UNITS == 1 ? (int)(wave & 1) : h) * 16 + li;
-						d[h] = mfma(b, *(const T8*)(lg + line * GC + slot(line, ns * 4 + gq, GC / 8) * 8), d[h]);
+						if (!WIDE || h == 0) { const int line = rows_at(h) + li; a = *(const T8*)(lg + line * GC + slot(line, ns * 4 + gq, GC / 8) * 8); }
+						if (WIDE) b = tr8_at(lw, XC, ns * 32, kf * 16 + (li & 3) * 8 + h * 4); else if (h == 0) b = tr8(lw, XC, ns * 32, kf);
+						d[h] = mfma(b, a, d[h]);
 					}
 				}
+				if constexpr (WIDE) {
+					const uint32_t r = here * 32 + rows_at(0) + li, c = kf * 16 + gq * 8;
+					T8 o;
+					EACH o[e] = (T)d[e / 4][e & 3];
+					if (r < g.rows && c < g.k) store8(g.dx + (uint64_t)r * g.ld_dx + c, o, (int)min(8u, g.k - c));
+				} else {
 #pragma unroll
-				for (int h = 0; h < PAIR; ++h) {
-					const uint32_t r = here * 32 + (UNITS == 1 ? wave & 1 : h) * 16 + li, c = kf * 16 + gq * 4;
-					if (r < g.rows && c < g.k) {
-						T* o = g.dx + (uint64_t)r * g.ld_dx + c;
-						T v[4] = {(T)d[h][0], (T)d[h][1], (T)d[h][2], (T)d[h][3]};
-						if (c + 4 <= g.k) __builtin_memcpy(o, v, 8);
-						else {
+					for (int h = 0; h < PAIR; ++h) {
+						const uint32_t r = here * 32 + rows_at(h) + li, c = kf * 16 + gq * 4;
+						if (r < g.rows && c < g.k) {
+							T* o = g.dx + (uint64_t)r * g.ld_dx + c;
+							T v[4] = {(T)d[h][0], (T)d[h][1], (T)d[h][2], (T)d[h][3]};
+							if (c + 4 <= g.k) __builtin_memcpy(o, v, 8);
+							else {
 #pragma unroll
-							for (int e = 0; e < 3; ++e) if (c + e < g.k) o[e] = v[e];
+								for (int e = 0; e < 3; ++e) if (c + e < g.k) o[e] = v[e];
+							}
 						}
 					}
 				}
