@@ -2,16 +2,17 @@
 //   norm = sqrt(sum of g^2 over all tensors) / loss_scale;   c = max_norm / norm where norm > max_norm, else 1;   clipped = c g
 // Memory bound: one pass reads every gradient for the sum, one reads and writes it (nothing is written in place where c = 1).  The tensors' table travels in the
 // kernel arguments (no upload that a captured graph would have to keep alive), TABLE tensors a launch.  Every block owns a contiguous range of the tensors' chunks;
-// the second pass walks the ranges backwards, so that it begins with what the first one left in the caches.  Sums are double, in a fixed order: the result
+// the second pass takes launches and ranges backwards, so that it begins with what the first one left in the caches.  Up to SMALL elements one block does it all, in one launch.  Sums are double, in a fixed order: the result
 // does not depend on timing, and squares of any bfloat16 / float fit.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <algorithm>
+#include <vector>
 #include "ngp_kernels.hpp"
 
 namespace ngp {
 namespace {
-constexpr uint32_t TABLE = 112, CHUNK = 8192, THREADS = 256;
+constexpr uint32_t TABLE = 112, CHUNK = 8192, THREADS = 256, SMALL = 65536;
 struct ClipTable { const void* grad[TABLE]; void* clipped[TABLE]; uint64_t size[TABLE]; uint32_t first[TABLE + 1]; uint8_t type[TABLE]; uint32_t n; };
 struct Range { uint32_t begin, end; };
 __device__ inline Range block_range(uint32_t chunks) {
@@ -23,7 +24,7 @@ __device__ inline uint32_t tensor_of(const ClipTable& t, uint32_t chunk) { // la
 	return lo;
 }
 template <typename T, int N> struct Vec { T v[N]; };
-template <typename T> __device__ inline double sum_squares(const T* p, uint32_t n) { // n <= CHUNK elements
+template <uint32_t THREADS, typename T> __device__ inline double sum_squares(const T* p, uint32_t n) {
 	constexpr int N = 16 / sizeof(T);
 	double s = 0;
 	uint32_t i = threadIdx.x * N;
@@ -37,7 +38,7 @@ template <typename T> __device__ inline double sum_squares(const T* p, uint32_t 
 	for (; i < n; ++i) { const double d = (double)(float)p[i]; s = fma(d, d, s); }
 	return s;
 }
-template <typename T> __device__ inline void scale(const T* p, T* q, uint32_t n, float c) {
+template <uint32_t THREADS, typename T> __device__ inline void scale(const T* p, T* q, uint32_t n, float c) {
 	constexpr int N = 16 / sizeof(T);
 	uint32_t i = threadIdx.x * N;
 #pragma unroll 4
@@ -50,15 +51,34 @@ template <typename T> __device__ inline void scale(const T* p, T* q, uint32_t n,
 	}
 	for (; i < n; ++i) q[i] = (T)((float)p[i] * c);
 }
-__device__ inline double block_sum(double s) { // the sum over the block, in every thread
+template <uint32_t THREADS> __device__ inline double sum_tensor(int type, const void* p, uint64_t at, uint32_t n) {
+	switch (type) {
+		case NGP_TYPE_HALF: return sum_squares<THREADS>((const _Float16*)p + at, n);
+		case NGP_TYPE_BFLOAT16: return sum_squares<THREADS>((const __bf16*)p + at, n);
+		default: return sum_squares<THREADS>((const float*)p + at, n);
+	}
+}
+template <uint32_t THREADS> __device__ inline void scale_tensor(int type, const void* p, void* q, uint64_t at, uint32_t n, float c) {
+	switch (type) {
+		case NGP_TYPE_HALF: scale<THREADS>((const _Float16*)p + at, (_Float16*)q + at, n, c); break;
+		case NGP_TYPE_BFLOAT16: scale<THREADS>((const __bf16*)p + at, (__bf16*)q + at, n, c); break;
+		default: scale<THREADS>((const float*)p + at, (float*)q + at, n, c); break;
+	}
+}
+template <uint32_t THREADS = 256> __device__ inline double block_sum(double s) { // the sum over the block, in every thread
 	__shared__ double red[THREADS / 64];
 #pragma unroll
 	for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
 	__syncthreads();
 	if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
 	__syncthreads();
-	return red[0] + red[1] + red[2] + red[3];
+	s = 0;
+#pragma unroll
+	for (uint32_t i = 0; i < THREADS / 64; ++i) s += red[i];
+	return s;
 }
+// max_norm / norm where the norm is finite and beyond it
+__device__ inline float clip_factor(double norm, float max_norm) { return norm <= 1.7976931348623157e308 && norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f; }
 __global__ __launch_bounds__(THREADS) void k_norm_partial(ClipTable t, double* slots, uint32_t written) {
 	const Range r = block_range(t.first[t.n]);
 	double s = 0;
@@ -67,11 +87,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_partial(ClipTable t, double* s
 		while (t.first[i + 1] <= k) ++i;
 		const uint64_t at = (uint64_t)(k - t.first[i]) * CHUNK, left = t.size[i] - at;
 		const uint32_t n = left < CHUNK ? (uint32_t)left : CHUNK;
-		switch (t.type[i]) {
-			case NGP_TYPE_HALF: s += sum_squares((const _Float16*)t.grad[i] + at, n); break;
-			case NGP_TYPE_BFLOAT16: s += sum_squares((const __bf16*)t.grad[i] + at, n); break;
-			default: s += sum_squares((const float*)t.grad[i] + at, n); break;
-		}
+		s += sum_tensor<THREADS>(t.type[i], t.grad[i], at, n);
 	}
 	s = block_sum(s);
 	if (threadIdx.x == 0) slots[blockIdx.x] = (blockIdx.x < written ? slots[blockIdx.x] : 0.0) + s;
@@ -88,8 +104,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_finish(const double* slots, ui
 __global__ __launch_bounds__(THREADS) void k_clip(ClipTable t, const double* slots, uint32_t n_slots, float loss_scale, float max_norm, float* norm) {
 	const double v = norm_of(slots, n_slots, loss_scale);
 	if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-	const bool finite = v <= 1.7976931348623157e308; // (false for NaN): a norm that is not finite leaves the gradients as they are
-	const float c = finite && v > (double)max_norm ? (float)((double)max_norm / v) : 1.f;
+	const float c = clip_factor(v, max_norm);
 	const Range r = block_range(t.first[t.n]);
 	if (r.begin >= r.end) return;
 	uint32_t i = tensor_of(t, r.end - 1);
@@ -98,40 +113,58 @@ __global__ __launch_bounds__(THREADS) void k_clip(ClipTable t, const double* slo
 		if (!t.clipped[i] || (c == 1.f && t.clipped[i] == t.grad[i])) continue;
 		const uint64_t at = (uint64_t)(k - t.first[i]) * CHUNK, left = t.size[i] - at;
 		const uint32_t n = left < CHUNK ? (uint32_t)left : CHUNK;
-		switch (t.type[i]) {
-			case NGP_TYPE_HALF: scale((const _Float16*)t.grad[i] + at, (_Float16*)t.clipped[i] + at, n, c); break;
-			case NGP_TYPE_BFLOAT16: scale((const __bf16*)t.grad[i] + at, (__bf16*)t.clipped[i] + at, n, c); break;
-			default: scale((const float*)t.grad[i] + at, (float*)t.clipped[i] + at, n, c); break;
-		}
+		scale_tensor<THREADS>(t.type[i], t.grad[i], t.clipped[i], at, n, c);
 	}
+}
+// all of it by one block
+__global__ __launch_bounds__(1024) void k_clip_small(ClipTable t, float loss_scale, float max_norm, float* norm) {
+	double s = 0;
+	for (uint32_t i = 0; i < t.n; ++i) s += sum_tensor<1024>(t.type[i], t.grad[i], 0, (uint32_t)t.size[i]);
+	const double v = sqrt(block_sum<1024>(s)) / (double)loss_scale;
+	if (threadIdx.x == 0) *norm = (float)v;
+	const float c = clip_factor(v, max_norm);
+	for (uint32_t i = 0; i < t.n; ++i)
+		if (t.clipped[i] && !(c == 1.f && t.clipped[i] == t.grad[i])) scale_tensor<1024>(t.type[i], t.grad[i], t.clipped[i], 0, (uint32_t)t.size[i], c);
 }
 } // namespace
 
 void launch_gradient_norm(hipStream_t s, uint32_t n, const ngp_gradient* tensors, float loss_scale, bool clip, float max_norm, float* norm, double* slots) {
-	uint32_t written = 0, last_blocks = 0;
-	bool norm_written = false;
-	auto walk = [&](auto&& launch) {
-		for (uint32_t i = 0; i < n;) {
-			ClipTable t;
-			t.n = 0; t.first[0] = 0;
-			for (; i < n && t.n < TABLE; ++i) {
-				if (!tensors[i].size) continue;
-				const uint64_t chunks = (tensors[i].size + CHUNK - 1) / CHUNK;
-				if (t.n && t.first[t.n] + chunks > 0x7fffffffull) break; // (a launch's chunks fit 31 bits; one tensor alone does: checked at the entry point)
-				t.grad[t.n] = tensors[i].grad; t.clipped[t.n] = clip ? tensors[i].clipped : nullptr; t.size[t.n] = tensors[i].size; t.type[t.n] = (uint8_t)tensors[i].type;
-				t.first[t.n + 1] = t.first[t.n] + (uint32_t)chunks; ++t.n;
-			}
-			if (t.n) { last_blocks = std::min(t.first[t.n], CLIP_SLOTS); launch(t); }
+	// the tensors in tables of at most TABLE (a table's chunks fit 31 bits; one tensor alone does: checked at the entry point)
+	auto table = [&](uint32_t& i, ClipTable& t) { // from tensor i on; i: the first one that is left
+		t.n = 0; t.first[0] = 0;
+		for (; i < n && t.n < TABLE; ++i) {
+			if (!tensors[i].size) continue;
+			const uint64_t chunks = (tensors[i].size + CHUNK - 1) / CHUNK;
+			if (t.n && t.first[t.n] + chunks > 0x7fffffffull) break;
+			t.grad[t.n] = tensors[i].grad; t.clipped[t.n] = clip ? tensors[i].clipped : nullptr; t.size[t.n] = tensors[i].size; t.type[t.n] = (uint8_t)tensors[i].type;
+			t.first[t.n + 1] = t.first[t.n] + (uint32_t)chunks; ++t.n;
 		}
 	};
-	walk([&](const ClipTable& t) {
-		hipLaunchKernelGGL(k_norm_partial, dim3(last_blocks), dim3(THREADS), 0, s, t, slots, written);
-		written = std::max(written, last_blocks);
-	});
-	if (clip) walk([&](const ClipTable& t) {
-		hipLaunchKernelGGL(k_clip, dim3(last_blocks), dim3(THREADS), 0, s, t, slots, written, loss_scale, max_norm, norm_written ? nullptr : norm);
-		norm_written = true;
-	});
-	if (!norm_written) hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(THREADS), 0, s, slots, written, loss_scale, norm);
+	ClipTable t;
+	uint64_t total = 0;
+	for (uint32_t i = 0; i < n && total <= SMALL; ++i) total += tensors[i].size;
+	uint32_t i = 0;
+	if (total <= SMALL) {
+		table(i, t);
+		if (i >= n) { hipLaunchKernelGGL(k_clip_small, dim3(1), dim3(1024), 0, s, t, loss_scale, max_norm, norm); return; }
+		i = 0;
+	}
+	std::vector<uint32_t> starts; // first tensor of each table
+	uint32_t written = 0;         // slots
+	while (i < n) {
+		const uint32_t from = i;
+		table(i, t);
+		if (!t.n) { table(i = starts.back(), t); break; } // (only empty ones were left)
+		starts.push_back(from);
+		const uint32_t blocks = std::min(t.first[t.n], CLIP_SLOTS);
+		hipLaunchKernelGGL(k_norm_partial, dim3(blocks), dim3(THREADS), 0, s, t, slots, written);
+		written = std::max(written, blocks);
+	}
+	if (!clip) { hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(THREADS), 0, s, slots, written, loss_scale, norm); return; }
+	for (size_t k = starts.size(); k-- > 0;) { // the last table first (it is still there)
+		i = starts[k];
+		if (k + 1 < starts.size()) table(i, t);
+		hipLaunchKernelGGL(k_clip, dim3(std::min(t.first[t.n], CLIP_SLOTS)), dim3(THREADS), 0, s, t, slots, written, loss_scale, max_norm, k + 1 == starts.size() ? norm : nullptr);
+	}
 }
 } // namespace ngp

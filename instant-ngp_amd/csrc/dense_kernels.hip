@@ -1028,7 +1028,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		else { if (d.gated) launch_few_rows<2, EPI_GATED>(s, g, partial); else launch_few_rows<2, EPI_LINEAR>(s, g, partial); }
 		return;
 	}
-	if (dense_narrow(d.m, d.n, d.k, d.gated) && d.k) {
+	if (dense_narrow(d.m, d.n, d.k, d.gated)) {
 		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
 		return;
 	}
@@ -1042,12 +1042,12 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const bool bias = d.dbias[0] || d.dbias[1];
 	const bool identity = !d.gated && d.act == NGP_ACT_NONE; // G is dY as it stands
 	const bool products = d.dx || d.dw[0] || d.dw[1];
-	if (products && dense_narrow(d.m, d.n, d.k, d.gated) && d.n && d.k) {
+	if ((products || bias) && dense_narrow(d.m, d.n, d.k, d.gated)) {
 		NarrowArgs a{};
 		a.rows = d.m; a.n = d.n; a.k = d.k; a.act = d.act; a.x = (const T*)d.x; a.ld_x = d.x_stride; a.ld_w = d.w_stride; a.ld_pre = d.pre_stride; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride;
 		for (int i = 0; i < 2; ++i) { a.w[i] = (const T*)d.w[i]; a.pre[i] = (const T*)d.pre[i]; }
 		if (identity) { a.pre[0] = a.dy; a.ld_pre = a.ld_dy; } // (read, not used)
-		if (!a.x) { a.x = a.dy; a.ld_x = 0; }                  // (dW is not wanted: nothing reads X's place)
+		if (!d.dw[0]) { a.x = a.dy; a.ld_x = 0; }              // (dW is not wanted: something to read in the place of X, where nothing looks)
 		a.dx = (T*)d.dx; a.ld_dx = d.dx_stride; a.partial = d.dw[0] ? (float*)(ws + p.partial) : nullptr; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr;
 		if (d.gated) launch_narrow_backward<true>(s, a, p.row_blocks); else launch_narrow_backward<false>(s, a, p.row_blocks);
 		if (bias) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, a.bias_partial, p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);

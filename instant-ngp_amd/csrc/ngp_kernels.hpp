@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <cmath>
 #include "../../include/ngp_hip.h"
 
 namespace ngp {
@@ -382,8 +383,12 @@ inline uint64_t dense_split_bytes(uint64_t rows, uint64_t cols, uint64_t steps, 
 	const DenseSplit d = dense_split(rows, cols, steps, segments, parts);
 	return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0;
 }
-// layers that k_narrow_forward / k_narrow_backward take: all weights in one compute unit
-inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) { return m >= 2048 && n >= 8 && k >= 8 && k <= 256 && (gated ? 2 * (uint64_t)n : n) <= 256; }
+// Layers that k_narrow_forward / k_narrow_backward take: all weights in one compute unit.  Every block stages them, which pays from few samples on where they are small (64 x 64, 2048
+// samples: forward + backward 5.0 + 11 us against 8.9 + 20 us by tiles) and from many where they fill LDS (256 x 256, 65536 samples: 28 + 58 us against 30 + 66 us).
+inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) {
+	const uint64_t cols = (gated ? 2 * (uint64_t)n : n);
+	return n >= 8 && k >= 8 && k <= 256 && cols <= 256 && m > FEW_ROWS && (cols * k <= 32768 || m >= 32768);
+}
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
@@ -398,8 +403,11 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
 	if (dense_narrow(m, n, k, gated)) { // one pass, a partial sum a block
 		const uint32_t slabs = (m + 31) / 32;
-		const uint32_t most = (gated ? 2 * n : n) <= 128 && k <= 128 ? 512 : 256; // two blocks a compute unit where their registers and LDS allow it
+		// two blocks a compute unit where their registers and LDS allow it; fewer where the partial sums (written and read at 4 TB/s) would cost more than the blocks save (2 us a slab)
+		const uint32_t most = (gated ? 2 * n : n) <= 128 && k <= 128 ? 512 : 256;
+		const double even = std::sqrt((double)slabs * 2.0 * 4e6 / ((double)problems * n * k * 8.0));
 		p.rows_per_block = 0; p.row_blocks = slabs < most ? slabs : most;
+		if (even < p.row_blocks) p.row_blocks = even < 1.0 ? 1 : (uint32_t)even;
 		p.grad = p.bias = 0; p.partial = up((uint64_t)problems * p.row_blocks * n * 4);
 		p.bytes = p.partial + up((uint64_t)problems * p.row_blocks * n * (((uint64_t)k + 7) & ~7ull) * 4);
 		return p;
