@@ -24,32 +24,41 @@ __device__ inline uint32_t tensor_of(const ClipTable& t, uint32_t chunk) { // la
 	return lo;
 }
 template <typename T, int N> struct Vec { T v[N]; };
+// elements in front of the first 16-byte boundary of p, n at most (a tensor begins wherever its elements allow)
+template <typename T> __device__ inline uint32_t head_of(const T* p, uint32_t n) { return min(n, (uint32_t)(-(uintptr_t)p & 15) / (uint32_t)sizeof(T)); }
 template <uint32_t THREADS, typename T> __device__ inline double sum_squares(const T* p, uint32_t n) {
 	constexpr int N = 16 / sizeof(T);
+	const uint32_t head = head_of(p, n);
 	double s = 0;
-	uint32_t i = threadIdx.x * N;
+	if (threadIdx.x < head) { const double d = (double)(float)p[threadIdx.x]; s = d * d; }
+	p += head; n -= head;
+	const uint32_t tail = n % N;
+	if (threadIdx.x >= THREADS - tail) { const double d = (double)(float)p[n - (THREADS - threadIdx.x)]; s = fma(d, d, s); } // (one element a thread: a loop waits for every load)
 #pragma unroll 4
-	for (; i + N <= n; i += THREADS * N) {
+	for (uint32_t i = threadIdx.x * N; i + N <= n; i += THREADS * N) {
 		Vec<T, N> v;
-		__builtin_memcpy(&v, p + i, 16);
+		__builtin_memcpy(&v, __builtin_assume_aligned(p + i, 16), 16);
 #pragma unroll
 		for (int e = 0; e < N; ++e) { const double d = (double)(float)v.v[e]; s = fma(d, d, s); }
 	}
-	for (; i < n; ++i) { const double d = (double)(float)p[i]; s = fma(d, d, s); }
 	return s;
 }
 template <uint32_t THREADS, typename T> __device__ inline void scale(const T* p, T* q, uint32_t n, float c) {
 	constexpr int N = 16 / sizeof(T);
-	uint32_t i = threadIdx.x * N;
+	const uint32_t head = head_of(q, n); // (whole lines are written; p has the same alignment or is read across it)
+	if (threadIdx.x < head) q[threadIdx.x] = (T)((float)p[threadIdx.x] * c);
+	p += head; q += head; n -= head;
+	const uint32_t tail = n % N;
+	if (threadIdx.x >= THREADS - tail) { const uint32_t i = n - (THREADS - threadIdx.x); q[i] = (T)((float)p[i] * c); }
 #pragma unroll 4
-	for (; i + N <= n; i += THREADS * N) {
+	for (uint32_t i = threadIdx.x * N; i + N <= n; i += THREADS * N) {
 		Vec<T, N> v;
 		__builtin_memcpy(&v, p + i, 16);
 #pragma unroll
 		for (int e = 0; e < N; ++e) v.v[e] = (T)((float)v.v[e] * c); // rounded once, to the gradient's own type
-		__builtin_memcpy(q + i, &v, 16);
+		typedef float f4 __attribute__((ext_vector_type(4)));
+		__builtin_nontemporal_store(__builtin_bit_cast(f4, v), (f4*)(q + i)); // (not wanted again: the caches keep gradients that are still to be read)
 	}
-	for (; i < n; ++i) q[i] = (T)((float)p[i] * c);
 }
 template <uint32_t THREADS> __device__ inline double sum_tensor(int type, const void* p, uint64_t at, uint32_t n) {
 	switch (type) {
