@@ -123,6 +123,17 @@ __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 va
 		default: break;
 	}
 }
+// f(activation as a constant): one branch for a whole loop, whose code then stays small (an epilogue with the branch in every row ran 2.5 times longer, waiting for instructions)
+template <typename F> __device__ inline void with_act(int act, F&& f) {
+	switch (act) {
+		case NGP_ACT_RELU: f(std::integral_constant<int, NGP_ACT_RELU>()); break;
+		case NGP_ACT_LOGISTIC: f(std::integral_constant<int, NGP_ACT_LOGISTIC>()); break;
+		case NGP_ACT_EXPONENTIAL: f(std::integral_constant<int, NGP_ACT_EXPONENTIAL>()); break;
+		case NGP_ACT_SILU: f(std::integral_constant<int, NGP_ACT_SILU>()); break;
+		case NGP_ACT_GELU: f(std::integral_constant<int, NGP_ACT_GELU>()); break;
+		default: f(std::integral_constant<int, NGP_ACT_NONE>()); break;
+	}
+}
 // G of 8 outputs: dY act'(Z); gated: dY Zu act'(Zg) and dY act(Zg).  Zeros give zeros.
 template <bool GATED> __device__ inline void output_grad8(int act, const T8& dy, const T8& zt, const T8& ut, float g[8], float g2[8]) {
 	float d[8], m[8], z[8];
@@ -183,7 +194,7 @@ __host__ __device__ inline uint32_t up8(uint32_t v) { return (v + 7) & ~7u; }
 
 // What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C.  Biases and the residual come as values: a caller
 // with several rows loads them ahead.
-template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual) {
+template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual, int act) {
 	T8 o, s;
 	if constexpr (EPI == EPI_PARTIAL || EPI == EPI_PARTIAL2) {
 		const uint32_t parts = EPI == EPI_PARTIAL2 ? 2 : g.problems;
@@ -199,7 +210,7 @@ template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t 
 	}
 	EACH z[e] += (float)bias0[e];
 	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n); }
-	act_value8(g.act, z);
+	act_value8(act, z);
 	if constexpr (EPI == EPI_LINEAR) {
 		EACH o[e] = (T)(z[e] + (float)residual[e]);
 	} else {
@@ -321,7 +332,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 			const int n = (int)min(8u, g.cols - c);
 			float z[8], u[8];
 			EACH { z[e] = acc[i][2 * p + e / 4][e & 3]; u[e] = GATED_TILE<EPI> ? acc[i][(GATED_TILE<EPI> ? FC / 2 : 0) + 2 * p + e / 4][e & 3] : 0.f; }
-			epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+			epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), g.act);
 		}
 	}
 }
@@ -507,35 +518,50 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 || UNITS > 2 ? 1 : 2) void 
 		settle(acc);
 		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is under way to LDS any more
 	}
-	// epilogue through the wavefront's own strip of LDS: 8 consecutive columns a lane, whole lines a store, the residual of 8 rows on its way at a time
+	// epilogue through the wavefront's own strip of LDS: 8 consecutive columns a lane, whole lines a store, the residual of the next rows on its way
 	float* strip = (float*)lds + wave * PASS * 16 * STRIP;
-	constexpr int LANES = OUT / WC / 8, ROWS = 64 / LANES, AT_ONCE = PASS * 16 / ROWS < 8 ? PASS * 16 / ROWS : 8; // lanes a row, rows at a time
+	constexpr int LANES = OUT / WC / 8, ROWS = 64 / LANES, AT_ONCE = 4; // lanes a row, rows at a time, such groups a turn
+	static_assert(PASS * 16 % (ROWS * AT_ONCE) == 0, "");
 	const uint32_t er = lane / LANES, ec = (lane % LANES) * 8, c = c0 + wc * (OUT / WC) + ec;
 	const int n = (int)min(8u, g.cols > c ? g.cols - c : 0u);
 	const T8 bias0 = bias8<EPI>(g, 0, c, n), bias1 = bias8<EPI>(g, 1, c, n);
-#pragma unroll
+#pragma unroll 1
 	for (int pass = 0; pass < FR / PASS; ++pass) {
 #pragma unroll
-		for (int i = 0; i < PASS; ++i)
+		for (int k = 0; k < FR / PASS; ++k)
+			if (k == pass) {
 #pragma unroll
-			for (int j = 0; j < FC; ++j) *(f4v*)(strip + (i * 16 + li) * STRIP + j * 16 + gq * 4) = acc[pass * PASS + i][j];
+				for (int i = 0; i < PASS; ++i)
+#pragma unroll
+					for (int j = 0; j < FC; ++j) *(f4v*)(strip + (i * 16 + li) * STRIP + j * 16 + gq * 4) = acc[k * PASS + i][j];
+			}
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the strip is this wavefront's alone)
 		const uint32_t r_pass = r0 + wr * (BR / WR) + pass * PASS * 16 + er;
+		auto rows = [&](auto act_c) {
+			T8 next[AT_ONCE];
+			auto load_residual = [&](int k) {
+#pragma unroll
+				for (int q = 0; q < AT_ONCE; ++q) next[q] = residual8<EPI>(g, min(r_pass + k + q * ROWS, g.rows - 1), c, n);
+			};
+			load_residual(0);
 #pragma unroll 1
-		for (int k = 0; k < PASS * 16; k += ROWS * AT_ONCE) {
-			T8 residual[AT_ONCE];
+			for (int k = 0; k < PASS * 16; k += ROWS * AT_ONCE) {
+				T8 residual[AT_ONCE];
 #pragma unroll
-			for (int q = 0; q < AT_ONCE; ++q) residual[q] = residual8<EPI>(g, r_pass + k + q * ROWS, c, r_pass + k + q * ROWS < g.rows ? n : 0);
+				for (int q = 0; q < AT_ONCE; ++q) residual[q] = next[q];
+				if (k + ROWS * AT_ONCE < PASS * 16) load_residual(k + ROWS * AT_ONCE);
 #pragma unroll
-			for (int q = 0; q < AT_ONCE; ++q) {
-				const uint32_t r = r_pass + k + q * ROWS;
-				float z[8], u[8];
-				const float* p = strip + (k + q * ROWS + er) * STRIP + ec;
-				*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
-				if constexpr (GATED_TILE<EPI>) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
-				if (r < g.rows && n > 0) epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias0, bias1, residual[q]);
+				for (int q = 0; q < AT_ONCE; ++q) {
+					const uint32_t r = r_pass + k + q * ROWS;
+					float z[8], u[8];
+					const float* p = strip + (k + q * ROWS + er) * STRIP + ec;
+					*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
+					if constexpr (GATED_TILE<EPI>) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
+					if (r < g.rows && n > 0) epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias0, bias1, residual[q], decltype(act_c)::value);
+				}
 			}
-		}
+		};
+		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) with_act(g.act, rows); else rows(std::integral_constant<int, NGP_ACT_NONE>());
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
 }
@@ -607,7 +633,7 @@ template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(Gem
 			EACH z[e] += sums[k * slices + q][0][r][half * 8 + e];
 			if (GATED) EACH u[e] += sums[k * slices + q][P - 1][r][half * 8 + e];
 		}
-		epilogue8<EPI>(g, 0, blockIdx.y, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+		epilogue8<EPI>(g, 0, blockIdx.y, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), g.act);
 	}
 }
 
@@ -663,7 +689,7 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 			for (int f = 0; f < NF; ++f) acc[f] = mfma(*(const T8*)(w + ((f * KS + k) * 64 + lane) * 8), x[k], acc[f]);
 		if (slab + stride < slabs) load_x(slab + stride);
 		const uint32_t r = slab * 16 + li;
-		if (r < g.rows) {
+		if (r < g.rows) with_act(g.act, [&](auto act_c) {
 #pragma unroll
 			for (int p = 0; p < OF / 2; ++p) {
 				const uint32_t c = p * 32 + gq * 8;
@@ -671,9 +697,9 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 				const int n = (int)min(8u, g.cols - c);
 				float z[8], u[8];
 				EACH { z[e] = acc[2 * p + e / 4][e & 3]; u[e] = GATED ? acc[(GATED ? OF : 0) + 2 * p + e / 4][e & 3] : 0.f; }
-				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n));
+				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), decltype(act_c)::value);
 			}
-		}
+		});
 	}
 }
 // Backward in one pass: a block takes 32 samples at a time (the next 32 on their way), forms G = dY * act'(Z) and lays it and X into LDS; its 8 wavefronts multiply G with the weights
@@ -953,7 +979,7 @@ template <int EPI, int GROUPS> __global__ __launch_bounds__(256) void k_join_spl
 #pragma unroll
 		for (int q = 1; q < GROUPS; ++q) EACH { z[e] += red[q][0][item][e]; if (P == 2) u[e] += red[q][P - 1][item][e]; }
 	}
-	epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual);
+	epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual, g.act);
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -971,8 +997,9 @@ template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs
 	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
 	static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
 	if (!wholes) hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
-	else if (large) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
-	else if (grid.x <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
+	else if (large) {
+		if constexpr (EPI != EPI_PARTIAL && EPI != EPI_PARTIAL2) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g); // (large tiles are many: their sums are not split)
+	} else if (grid.x <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
 	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
 }
 template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
