@@ -179,7 +179,7 @@ template <int EXTENT, bool T_CONTIG, bool IS_B> struct Tile {
 	}
 };
 
-enum { EPI_LINEAR, EPI_GATED, EPI_STORE, EPI_PARTIAL, EPI_PARTIAL2 /* of both projections */ };
+enum { EPI_LINEAR, EPI_GATED, EPI_STORE /* as it is; partial sums where they are split */, EPI_PARTIAL, EPI_PARTIAL2 /* of both projections */ };
 struct GemmArgs {
 	const T* a; const T* b[2]; uint64_t lda, ldb;
 	uint32_t rows, cols, steps;      // C is rows x cols; the sum runs over `segments` pieces of `steps`
@@ -204,6 +204,7 @@ template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t 
 		return;
 	}
 	if constexpr (EPI == EPI_STORE) {
+		if (g.splits > 1) { epilogue8<EPI_PARTIAL>(g, problem, split, r, c, n, z, u, bias0, bias1, residual, act); return; }
 		EACH o[e] = (T)z[e];
 		store8(g.c[problem] + (uint64_t)r * g.ldc + c, o, n);
 		return;
@@ -212,7 +213,8 @@ template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t 
 	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n); }
 	act_value8(act, z);
 	if constexpr (EPI == EPI_LINEAR) {
-		EACH o[e] = (T)(z[e] + (float)residual[e]);
+		if (g.residual) { EACH z[e] += (float)residual[e]; }
+		EACH o[e] = (T)z[e];
 	} else {
 		EACH u[e] += (float)bias1[e];
 		if (g.pre[1]) { EACH s[e] = (T)u[e]; store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n); }
@@ -227,23 +229,20 @@ template <int EPI> __device__ inline T8 residual8(const GemmArgs& g, uint32_t r,
 // Consecutive blocks go to the 8 dies in turn, each with an L2 of its own: give every die one contiguous run of the work, ordered by piece of the sum, product, strips of 8 row
 // tiles, so that its blocks share operands.  (Tiles of one piece on four dies: every operand line missed four L2s, dW of 2^18 samples 86 instead of 60 us.)
 struct Work { uint32_t row, col, problem, split; };
-__device__ inline Work work_of(const GemmArgs& g, uint32_t row_tiles, uint32_t col_tiles) {
-	const uint32_t n = gridDim.x, die = blockIdx.x & 7, per = n >> 3, rest = n & 7, t = die * per + min(die, rest) + (blockIdx.x >> 3), tiles = row_tiles * col_tiles;
+__device__ inline Work work_of(const GemmArgs& g, uint32_t index, uint32_t n, uint32_t row_tiles, uint32_t col_tiles) { // block `index` of the n that share this product
+	const uint32_t die = index & 7, per = n >> 3, rest = n & 7, t = die * per + min(die, rest) + (index >> 3), tiles = row_tiles * col_tiles;
 	const uint32_t which = t / tiles, in = t - which * tiles, strip = 8 * col_tiles, s = in / strip, k = in - s * strip, rows = min(8u, row_tiles - s * 8);
 	return {s * 8 + k % rows, k / rows, which % g.problems, which / g.problems};
 }
 // C tile BR x BC by WR x WC wavefronts; each owns (BR / WR) x (BC / WC) as 16 x 16 fragments (matrix instruction 16x16x32, C^T: a lane holds one row of C and 4 columns
 // of each fragment).  EPI_GATED: the tile's columns are BC / 2 gate outputs and the same BC / 2 up outputs, every wavefront owns both of its columns.
-template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI>
-__global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
+template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI> __device__ inline void any_tile(const GemmArgs& g, T* lds_a, T* lds_b, uint32_t index, uint32_t count) {
 	typedef Tile<BR, A_T, false> TA; typedef Tile<BC, B_T, true> TB;
 	constexpr int THREADS = 64 * WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, NA = TA::N_SLOTS / THREADS, NB = TB::N_SLOTS / THREADS;
 	constexpr int OUT = GATED_TILE<EPI> ? BC / 2 : BC; // columns of C per tile
 	static_assert(FC % (GATED_TILE<EPI> ? 4 : 2) == 0, "pairs of fragments");
-	__shared__ __attribute__((aligned(16))) T lds_a[TA::ELEMS];
-	__shared__ __attribute__((aligned(16))) T lds_b[TB::ELEMS];
 	const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
-	const Work w = work_of(g, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
+	const Work w = work_of(g, index, count, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
 	const uint32_t r0 = w.row * BR, c0 = w.col * OUT, problem = w.problem, split = w.split;
 	const T* a = g.a + problem * g.a_problem;
 	const uint32_t chunks_per_segment = (g.steps + TK - 1) / TK, n_chunks = chunks_per_segment * g.segments;
@@ -337,6 +336,17 @@ __global__ __launch_bounds__(64 * WR * WC) void k_gemm(GemmArgs g) {
 	}
 }
 
+template <bool A_T, bool B_T, int EPI> __global__ __launch_bounds__(256) void k_gemm(GemmArgs g) {
+	__shared__ __attribute__((aligned(16))) T lds[2][128 * TK];
+	any_tile<128, 128, 2, 2, A_T, B_T, EPI>(g, lds[0], lds[1], blockIdx.x, gridDim.x);
+}
+// dX and dW, which do not wait for each other, side by side: the first `blocks_x` blocks and the others
+__global__ __launch_bounds__(256) void k_products(GemmArgs x, GemmArgs w, uint32_t blocks_x) {
+	__shared__ __attribute__((aligned(16))) T lds[2][128 * TK];
+	if (blockIdx.x < blocks_x) any_tile<128, 128, 2, 2, true, false, EPI_STORE>(x, lds[0], lds[1], blockIdx.x, blocks_x);
+	else any_tile<128, 128, 2, 2, false, false, EPI_STORE>(w, lds[0], lds[1], blockIdx.x - blocks_x, gridDim.x - blocks_x);
+}
+
 // ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero) in units of 64 steps
 // of one operand (whole cache lines: 64-byte pieces ask the L2 twice as often, 65 instead of 70 % of the matrix rate).  UNITS of B and one more of A are in LDS: the one in use, and
 // what is on its way.  At 256 x 256 that is 160 KB with UNITS = 2 (about 2000 clocks ahead); 128 x 128 tiles take a quarter of the time a unit and get UNITS = 4 where a compute
@@ -394,18 +404,18 @@ template <bool T_CONTIG, int UNITS, int BYTES> struct Cursor {
 		}
 	}
 };
-template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS>
-__global__ __launch_bounds__(64 * WR * WC, BR >= 256 || UNITS > 2 ? 1 : 2) void k_gemm_async(GemmArgs g) {
+constexpr int async_lds(int tile, int units) { return tile * AK * 2 * (2 * units + 1); }
+template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS> __device__ inline void async_tile(const GemmArgs& g, char* lds, uint32_t index, uint32_t count) {
 	constexpr int WAVES = WR * WC, FR = BR / WR / 16, FC = BC / WC / 16, OUT = GATED_TILE<EPI> ? BC / 2 : BC;
 	typedef Async<BR, A_T, WAVES> LA; typedef Async<BC, B_T, WAVES> LB;
 	constexpr int UNITS_A = UNITS + 1, UNITS_B = UNITS, LDS = UNITS_A * LA::BYTES + UNITS_B * LB::BYTES;
 	constexpr int STRIP = BC / WC + 4, PASS = FR > 4 ? 4 : FR; // epilogue: floats per row of a wavefront's strip of LDS, fragment rows in it
 	static_assert(WAVES * PASS * 16 * STRIP * 4 <= LDS && FR % PASS == 0, "the epilogue's strips fit");
 	static_assert(FC % (GATED_TILE<EPI> ? 4 : 2) == 0 && FR % A_RING == 0 && LA::LOADS % FR == 0 && LB::LOADS % FR == 0, "");
-	__shared__ __attribute__((aligned(1024))) char lds[LDS];
+	static_assert(LDS == async_lds(BR, UNITS), "");
 	const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 	const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WC, wc = wave % WC, gq = lane >> 4, li = lane & 15;
-	const Work w = work_of(g, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
+	const Work w = work_of(g, index, count, (g.rows + BR - 1) / BR, (g.cols + OUT - 1) / OUT);
 	const uint32_t r0 = w.row * BR, c0 = w.col * OUT, problem = w.problem, split = w.split;
 	const uint32_t units_per_segment = (g.steps + AK - 1) / AK, n_units = units_per_segment * g.segments;
 	const uint32_t t_begin = min(n_units, split * g.chunks_per_split), t_end = min(n_units, t_begin + g.chunks_per_split);
@@ -564,6 +574,16 @@ __global__ __launch_bounds__(64 * WR * WC, BR >= 256 || UNITS > 2 ? 1 : 2) void 
 		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) with_act(g.act, rows); else rows(std::integral_constant<int, NGP_ACT_NONE>());
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
+}
+
+template <int TILE, bool A_T, bool B_T, int EPI, int UNITS> __global__ __launch_bounds__(256, TILE >= 256 || UNITS > 2 ? 1 : 2) void k_gemm_async(GemmArgs g) {
+	__shared__ __attribute__((aligned(1024))) char lds[async_lds(TILE, UNITS)];
+	async_tile<TILE, TILE, 2, 2, A_T, B_T, EPI, UNITS>(g, lds, blockIdx.x, gridDim.x);
+}
+template <int UNITS> __global__ __launch_bounds__(256, UNITS > 2 ? 1 : 2) void k_products_async(GemmArgs x, GemmArgs w, uint32_t blocks_x) { // (k_products)
+	__shared__ __attribute__((aligned(1024))) char lds[async_lds(128, UNITS)];
+	if (blockIdx.x < blocks_x) async_tile<128, 128, 2, 2, true, false, EPI_STORE, UNITS>(x, lds, blockIdx.x, blocks_x);
+	else async_tile<128, 128, 2, 2, false, false, EPI_STORE, UNITS>(w, lds, blockIdx.x - blocks_x, gridDim.x - blocks_x);
 }
 
 // ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
@@ -890,8 +910,8 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
-// one line per block of rows, before the rounding).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
-struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; uint32_t rows_per_block; };
+// one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
+struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; };
 template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
 	const uint32_t cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 256 + cx * 8, pc = up8(g.cols);
 	const uint32_t end = min(g.rows, (blockIdx.y + 1) * g.rows_per_block);
@@ -912,7 +932,7 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 			}
 		}
 	}
-	if (!g.bias_partial) return;
+	if (!g.bias_partial && !g.dbias[0] && !g.dbias[1]) return;
 	__shared__ float red[8][256 + 8];
 #pragma unroll
 	for (int k = 0; k < (GATED ? 2 : 1); ++k) {
@@ -924,34 +944,33 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 #pragma unroll
 		for (int y = 0; y < 8; ++y) s += red[y][threadIdx.x];
 		const uint32_t col = blockIdx.x * 256 + threadIdx.x;
-		if (col < g.cols) g.bias_partial[((uint64_t)blockIdx.y * (GATED ? 2 : 1) + k) * g.cols + col] = s;
+		if (col >= g.cols) continue;
+		if (g.bias_partial) g.bias_partial[((uint64_t)blockIdx.y * (GATED ? 2 : 1) + k) * g.cols + col] = s;
+		else if (g.dbias[k]) g.dbias[k][col] = (T)s; // (one block of rows: the sum is whole)
 	}
 }
-// dbias = sum of the blocks' column sums: 32 columns x 32 shares of the blocks, then the shares in their order
-__global__ __launch_bounds__(1024) void k_bias_grad(const float* partial, uint32_t blocks, uint32_t cols, uint32_t problems, T* out0, T* out1) {
-	__shared__ float red[32][33];
-	const uint32_t cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx, k = blockIdx.y;
+// dbias = sum of the blocks' column sums: a block takes 16 columns, 16 threads each, then adds the shares up in their order
+struct BiasArgs { const float* partial; uint32_t blocks, cols, problems; T* out[2]; };
+__device__ inline void bias_grad(const BiasArgs& a, uint32_t index, float* shared) {
+	const uint32_t cx = threadIdx.x & 15, ry = threadIdx.x >> 4, per = (a.cols + 15) / 16, k = index / per, c = (index % per) * 16 + cx;
 	float s = 0.f;
-	if (c < cols) {
+	if (c < a.cols) {
 #pragma unroll 8
-		for (uint32_t b = ry; b < blocks; b += 32) s += partial[((uint64_t)b * problems + k) * cols + c];
+		for (uint32_t b = ry; b < a.blocks; b += 16) s += a.partial[((uint64_t)b * a.problems + k) * a.cols + c];
 	}
-	red[ry][cx] = s;
+	shared[ry * 17 + cx] = s;
 	__syncthreads();
-	if (ry == 0 && c < cols) {
-		float t = 0.f;
+	if (ry || c >= a.cols || !a.out[k]) return;
+	s = 0.f;
 #pragma unroll
-		for (int y = 0; y < 32; ++y) t += red[y][cx];
-		T* out = k ? out1 : out0;
-		if (out) out[c] = (T)t;
-	}
+	for (int y = 0; y < 16; ++y) s += shared[y * 17 + cx];
+	a.out[k][c] = (T)s;
 }
 // the splits' sums, GROUPS threads sharing them out (in a fixed order), then the product's own epilogue (EPI_GATED: partial sums of both projections)
-template <int EPI, int GROUPS> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs g) {
+template <int EPI, int GROUPS> __device__ inline void join_splits(const GemmArgs& g, uint32_t index, float* shared) {
 	constexpr int P = EPI == EPI_GATED ? 2 : 1, ITEMS = 256 / GROUPS;
-	__shared__ float red[GROUPS > 1 ? GROUPS : 1][P][GROUPS > 1 ? ITEMS : 1][9];
-	const uint32_t cc = up8(g.cols) / 8, problem = blockIdx.y, parts = P == 2 ? 2 : g.problems, item = threadIdx.x % ITEMS, group = threadIdx.x / ITEMS;
-	const uint64_t id = (uint64_t)blockIdx.x * ITEMS + item;
+	const uint32_t cc = up8(g.cols) / 8, per = (uint32_t)(((uint64_t)g.rows * cc + ITEMS - 1) / ITEMS), problem = index / per, parts = P == 2 ? 2 : g.problems, item = threadIdx.x % ITEMS, group = threadIdx.x / ITEMS;
+	const uint64_t id = (uint64_t)(index % per) * ITEMS + item;
 	const bool in = id < (uint64_t)g.rows * cc;
 	if (GROUPS == 1 && !in) return;
 	const uint32_t r = in ? (uint32_t)(id / cc) : 0, c = in ? (uint32_t)(id % cc) * 8 : 0;
@@ -973,43 +992,69 @@ template <int EPI, int GROUPS> __global__ __launch_bounds__(256) void k_join_spl
 		}
 	}
 	if constexpr (GROUPS > 1) {
-		EACH { red[group][0][item][e] = z[e]; if (P == 2) red[group][P - 1][item][e] = u[e]; }
+		float* red = shared + ((group * P) * ITEMS + item) * 9;
+		EACH { red[e] = z[e]; if (P == 2) red[ITEMS * 9 + e] = u[e]; }
 		__syncthreads();
 		if (group || !in) return;
 #pragma unroll
-		for (int q = 1; q < GROUPS; ++q) EACH { z[e] += red[q][0][item][e]; if (P == 2) u[e] += red[q][P - 1][item][e]; }
+		for (int q = 1; q < GROUPS; ++q) EACH { z[e] += red[q * P * ITEMS * 9 + e]; if (P == 2) u[e] += red[(q * P + 1) * ITEMS * 9 + e]; }
 	}
-	epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual, g.act);
+	if constexpr (EPI == EPI_STORE) { // (the sums are whole now)
+		T8 o;
+		EACH o[e] = (T)z[e];
+		store8(g.c[problem] + (uint64_t)r * g.ldc + c, o, n);
+	} else epilogue8<EPI>(g, problem, 0, r, c, n, z, u, bias0, bias1, residual, g.act);
+}
+template <int EPI> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs g, int groups) {
+	__shared__ float shared[8 * (EPI == EPI_GATED ? 2 : 1) * 32 * 9];
+	if (groups > 1) join_splits<EPI, 8>(g, blockIdx.x, shared); else join_splits<EPI, 1>(g, blockIdx.x, shared);
+}
+// what is left of a backward pass in one launch: dX's and dW's split sums, the bias's
+__global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32_t blocks_x, GemmArgs w, int groups_w, uint32_t blocks_w, BiasArgs bias) {
+	__shared__ float shared[8 * 32 * 9];
+	uint32_t b = blockIdx.x;
+	if (b < blocks_x) { if (groups_x > 1) join_splits<EPI_STORE, 8>(x, b, shared); else join_splits<EPI_STORE, 1>(x, b, shared); return; }
+	b -= blocks_x;
+	if (b < blocks_w) { if (groups_w > 1) join_splits<EPI_STORE, 8>(w, b, shared); else join_splits<EPI_STORE, 1>(w, b, shared); return; }
+	bias_grad(bias, b - blocks_w, shared);
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
-template <int EPI> void launch_join(hipStream_t s, const GemmArgs& g) {
-	const uint64_t items = (uint64_t)g.rows * (up8(g.cols) / 8);
-	if (g.splits >= 16) hipLaunchKernelGGL((k_join_splits<EPI, 8>), dim3(div_up(items, 32), g.problems), dim3(256), 0, s, g);
-	else hipLaunchKernelGGL((k_join_splits<EPI, 1>), dim3(div_up(items, 256), g.problems), dim3(256), 0, s, g);
-}
+int join_groups(const GemmArgs& g) { return g.splits >= 16 ? 8 : 1; }
+uint32_t join_blocks(const GemmArgs& g) { return div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256 / join_groups(g)) * g.problems; }
+template <int EPI> void launch_join(hipStream_t s, GemmArgs g) { g.problems = 1; hipLaunchKernelGGL((k_join_splits<EPI>), dim3(join_blocks(g)), dim3(256), 0, s, g, join_groups(g)); }
+template <int EPI> uint32_t tiles(const GemmArgs& g, uint32_t tile) { return div_up(g.rows, tile) * div_up(g.cols, tile / (GATED_TILE<EPI> ? 2 : 1)) * g.problems * g.splits; }
+static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
 // `wholes`: both operands come in whole 16-byte pieces
-template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, GemmArgs& g, bool wholes, bool large) {
-	constexpr int K = GATED_TILE<EPI> ? 2 : 1; // weight columns per column of C
-	const uint32_t tile = large ? 256 : 128;
-	const dim3 grid(div_up(g.rows, tile) * div_up(g.cols, tile / K) * g.problems * g.splits);
-	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
-	static_assert(TK == 64 && AK == 64, "splits are counted in chunks of 64 steps");
-	if (!wholes) hipLaunchKernelGGL((k_gemm<128, 128, 2, 2, A_T, B_T, EPI>), grid, dim3(256), 0, s, g);
+template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, const GemmArgs& g, bool wholes, bool large) {
+	const uint32_t n = tiles<EPI>(g, large ? 256 : 128);
+	if (!wholes) hipLaunchKernelGGL((k_gemm<A_T, B_T, EPI>), dim3(n), dim3(256), 0, s, g);
 	else if (large) {
-		if constexpr (EPI != EPI_PARTIAL && EPI != EPI_PARTIAL2) hipLaunchKernelGGL((k_gemm_async<256, 256, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g); // (large tiles are many: their sums are not split)
-	} else if (grid.x <= 256) hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 4>), grid, dim3(256), 0, s, g);
-	else hipLaunchKernelGGL((k_gemm_async<128, 128, 2, 2, A_T, B_T, EPI, 2>), grid, dim3(256), 0, s, g);
+		if constexpr (EPI != EPI_PARTIAL && EPI != EPI_PARTIAL2) hipLaunchKernelGGL((k_gemm_async<256, A_T, B_T, EPI, 2>), dim3(n), dim3(256), 0, s, g); // (large tiles are many: their sums are not split)
+	} else if (n <= 256) hipLaunchKernelGGL((k_gemm_async<128, A_T, B_T, EPI, 4>), dim3(n), dim3(256), 0, s, g);
+	else hipLaunchKernelGGL((k_gemm_async<128, A_T, B_T, EPI, 2>), dim3(n), dim3(256), 0, s, g);
 }
-template <bool A_T, bool B_T, int EPI> void launch_gemm(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
-	const DenseSplit d = dense_split(g.rows, g.cols, g.steps, g.segments, EPI == EPI_GATED ? 2 : g.problems);
-	g.splits = 1;
-	if (d.splits > 1) {
-		g.splits = d.splits; g.partial = partial;
-		launch_tiles<A_T, B_T, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>(s, g, wholes, wholes && d.large);
+// tile size and splits of a product; true: large tiles
+bool set_split(GemmArgs& g, uint32_t parts, float* partial) {
+	const DenseSplit d = dense_split(g.rows, g.cols, g.steps, g.segments, parts);
+	g.splits = d.splits; g.partial = partial;
+	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
+	return d.large;
+}
+template <int EPI> void launch_forward(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
+	const bool large = set_split(g, EPI == EPI_GATED ? 2 : 1, partial) && wholes;
+	if (g.splits > 1) {
+		launch_tiles<true, true, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>(s, g, wholes, false);
 		launch_join<EPI>(s, g);
-	} else launch_tiles<A_T, B_T, EPI>(s, g, wholes, wholes && d.large);
+	} else launch_tiles<true, true, EPI>(s, g, wholes, large);
+}
+void launch_finish(hipStream_t s, const GemmArgs* x, const GemmArgs* w, const BiasArgs& bias) {
+	static const GemmArgs none{};
+	if (!x) x = &none;
+	if (!w) w = &none;
+	const uint32_t bx = x->splits > 1 ? join_blocks(*x) : 0, bw = w->splits > 1 ? join_blocks(*w) : 0, bb = bias.partial ? div_up(bias.cols, 16) * bias.problems : 0;
+	if (bx + bw + bb) hipLaunchKernelGGL(k_finish, dim3(bx + bw + bb), dim3(256), 0, s, *x, join_groups(*x), bx, *w, join_groups(*w), bw, bias);
 }
 template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, float* partial) {
 	const DenseFewRows f = dense_few_rows(g.cols, g.steps);
@@ -1060,7 +1105,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		return;
 	}
 	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
-	if (d.gated) launch_gemm<true, true, EPI_GATED>(s, g, wholes, partial); else launch_gemm<true, true, EPI_LINEAR>(s, g, wholes, partial);
+	if (d.gated) launch_forward<EPI_GATED>(s, g, wholes, partial); else launch_forward<EPI_LINEAR>(s, g, wholes, partial);
 }
 void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const DensePlan p = dense_plan(d.m, d.n, d.k, d.gated);
@@ -1077,40 +1122,51 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		if (!d.dw[0]) { a.x = a.dy; a.ld_x = 0; }              // (dW is not wanted: something to read in the place of X, where nothing looks)
 		a.dx = (T*)d.dx; a.ld_dx = d.dx_stride; a.partial = d.dw[0] ? (float*)(ws + p.partial) : nullptr; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr;
 		if (d.gated) launch_narrow_backward<true>(s, a, p.row_blocks); else launch_narrow_backward<false>(s, a, p.row_blocks);
-		if (bias) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, a.bias_partial, p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
-		if (a.partial) {
-			GemmArgs g{};
-			g.rows = d.n; g.cols = d.k; g.problems = problems; g.splits = p.row_blocks; g.partial = a.partial; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
-			launch_join<EPI_STORE>(s, g);
-		}
+		GemmArgs w{};
+		w.rows = d.n; w.cols = d.k; w.problems = problems; w.splits = p.row_blocks; w.partial = a.partial; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
+		BiasArgs b{a.bias_partial, p.row_blocks, d.n, problems, {(T*)d.dbias[0], (T*)d.dbias[1]}};
+		launch_finish(s, nullptr, a.partial ? &w : nullptr, b);
 		return;
 	}
 	const T* G = (const T*)d.dy; uint64_t ldg = d.dy_stride;
+	BiasArgs b{nullptr, p.row_blocks, d.n, problems, {(T*)d.dbias[0], (T*)d.dbias[1]}};
 	if ((!identity && products) || bias) {
 		GradArgs a{};
 		a.rows = d.m; a.cols = d.n; a.act = d.act; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride; a.pre[0] = (const T*)d.pre[0]; a.pre[1] = (const T*)d.pre[1]; a.ld_pre = d.pre_stride;
 		if (identity) a.pre[0] = nullptr;
-		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr; a.rows_per_block = p.rows_per_block;
+		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems; a.rows_per_block = p.rows_per_block;
+		if (p.row_blocks > 1) a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr; else for (int k = 0; k < 2; ++k) a.dbias[k] = (T*)d.dbias[k];
 		if (a.out) { G = a.out; ldg = a.ld_out; }
-		const dim3 grid(div_up(d.n, 256), p.row_blocks);
-		if (d.m && d.n) {
+		const dim3 grid(div_up(d.n, 256), std::max(1u, p.row_blocks)); // (no samples: the bias's gradient is zero)
+		if (d.n) {
 			if (d.gated) hipLaunchKernelGGL(k_output_grad<true>, grid, dim3(256), 0, s, a); else hipLaunchKernelGGL(k_output_grad<false>, grid, dim3(256), 0, s, a);
 		}
-		if (bias && d.n) hipLaunchKernelGGL(k_bias_grad, dim3(div_up(d.n, 32), problems), dim3(1024), 0, s, (const float*)(ws + p.bias), p.row_blocks, d.n, problems, (T*)d.dbias[0], (T*)d.dbias[1]);
+		b.partial = a.bias_partial;
 	}
 	const bool g_whole = whole(G, ldg, G == d.dy ? d.n : 8); // (the workspace's lines are padded with zeros)
-	float* partial = (float*)(ws + p.partial); // (the two products use it in turn)
-	if (d.dx && d.m && d.k) {
-		GemmArgs g{};
-		g.a = G; g.lda = ldg; g.a_segment = up8(d.n); g.segments = problems; g.b[0] = (const T*)d.w[0]; g.b[1] = (const T*)d.w[1]; g.ldb = d.w_stride;
-		g.rows = d.m; g.cols = d.k; g.steps = d.n; g.problems = 1; g.c[0] = (T*)d.dx; g.ldc = d.dx_stride;
-		launch_gemm<true, false, EPI_STORE>(s, g, g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k), partial);
+	GemmArgs x{}, w{};
+	bool large_x = false, large_w = false;
+	const bool want_x = d.dx && d.m && d.k, want_w = d.dw[0] && d.n && d.k;
+	const bool whole_x = g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k), whole_w = g_whole && whole(d.x, d.x_stride, d.k);
+	if (want_x) {
+		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = (const T*)d.w[0]; x.b[1] = (const T*)d.w[1]; x.ldb = d.w_stride;
+		x.rows = d.m; x.cols = d.k; x.steps = d.n; x.problems = 1; x.c[0] = (T*)d.dx; x.ldc = d.dx_stride;
+		large_x = set_split(x, 1, (float*)(ws + p.partial_x)) && whole_x;
 	}
-	if ((d.dw[0] || d.dw[1]) && d.n && d.k) {
-		GemmArgs g{};
-		g.a = G; g.lda = ldg; g.a_problem = up8(d.n); g.problems = problems; g.b[0] = g.b[1] = (const T*)d.x; g.ldb = d.x_stride;
-		g.rows = d.n; g.cols = d.k; g.steps = d.m; g.segments = 1; g.c[0] = (T*)d.dw[0]; g.c[1] = (T*)d.dw[1]; g.ldc = d.dw_stride;
-		launch_gemm<false, false, EPI_STORE>(s, g, g_whole && whole(d.x, d.x_stride, d.k), partial);
+	if (want_w) {
+		w.a = G; w.lda = ldg; w.a_problem = up8(d.n); w.problems = problems; w.b[0] = w.b[1] = (const T*)d.x; w.ldb = d.x_stride;
+		w.rows = d.n; w.cols = d.k; w.steps = d.m; w.segments = 1; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
+		large_w = set_split(w, problems, (float*)(ws + p.partial)) && whole_w;
 	}
+	if (want_x && want_w && !large_x && !large_w && whole_x == whole_w) {
+		const uint32_t bx = tiles<EPI_STORE>(x, 128), bw = tiles<EPI_STORE>(w, 128);
+		if (!whole_x) hipLaunchKernelGGL(k_products, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
+		else if (bx + bw <= 256) hipLaunchKernelGGL(k_products_async<4>, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
+		else hipLaunchKernelGGL(k_products_async<2>, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
+	} else {
+		if (want_x) launch_tiles<true, false, EPI_STORE>(s, x, whole_x, large_x);
+		if (want_w) launch_tiles<false, false, EPI_STORE>(s, w, whole_w, large_w);
+	}
+	launch_finish(s, &x, &w, b);
 }
 } // namespace ngp

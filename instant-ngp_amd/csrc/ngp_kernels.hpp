@@ -395,7 +395,7 @@ inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gat
 	return ((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull;
 }
 // Where the pieces of a backward pass lie in the workspace (bytes); from the sizes alone, so that ngp_*_workspace_size and the launch agree.
-struct DensePlan { uint64_t grad, bias, partial, bytes; uint32_t rows_per_block, row_blocks; };
+struct DensePlan { uint64_t grad, bias, partial, partial_x, bytes; uint32_t rows_per_block, row_blocks; };
 inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	DensePlan p;
 	const uint32_t problems = gated ? 2 : 1;
@@ -408,7 +408,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 		const double even = std::sqrt((double)slabs * 2.0 * 4e6 / ((double)problems * n * k * 8.0));
 		p.rows_per_block = 0; p.row_blocks = slabs < most ? slabs : most;
 		if (even < p.row_blocks) p.row_blocks = even < 1.0 ? 1 : (uint32_t)even;
-		p.grad = p.bias = 0; p.partial = up((uint64_t)problems * p.row_blocks * n * 4);
+		p.grad = p.bias = p.partial_x = 0; p.partial = up((uint64_t)problems * p.row_blocks * n * 4);
 		p.bytes = p.partial + up((uint64_t)problems * p.row_blocks * n * (((uint64_t)k + 7) & ~7ull) * 4);
 		return p;
 	}
@@ -419,7 +419,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
 	const uint64_t dx = dense_split_bytes(m, k, n, problems, 1), dw = dense_split_bytes(n, k, m, 1, problems);
 	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
-	p.bytes = p.partial + up(dx > dw ? dx : dw);
+	p.partial_x = p.partial + up(dw); p.bytes = p.partial_x + up(dx); // (the two products run side by side)
 	return p;
 }
 void launch_dense_forward_half(hipStream_t s, const DenseArgs& d);
