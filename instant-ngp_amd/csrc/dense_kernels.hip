@@ -63,6 +63,20 @@ __device__ inline T8 load8(const T* p, int n) {
 	for (int i = 0; i < 8; ++i) if (i < n) v[i] = p[i];
 	return v;
 }
+// The same where p may lie between two dwords: memory answers 16 bytes from an odd element on two to three times slower (1 x 4097 inputs, 8192 outputs: 29.6 us against 13.1), so the dwords
+// that hold them are read, five where p is odd.  (A dword with one element of the matrix in it can be read.)
+__device__ inline T8 load8_odd(const T* p) {
+	const uint32_t* q = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+	const bool odd = (uintptr_t)p & 2;
+	uint32_t v[4];
+	__builtin_memcpy(v, q, 16);
+	const uint32_t t = q[odd ? 4 : 3];
+	const uint32_t r[4] = {odd ? __builtin_amdgcn_alignbit(v[1], v[0], 16) : v[0], odd ? __builtin_amdgcn_alignbit(v[2], v[1], 16) : v[1],
+		odd ? __builtin_amdgcn_alignbit(v[3], v[2], 16) : v[2], odd ? __builtin_amdgcn_alignbit(t, v[3], 16) : v[3]};
+	T8 o;
+	__builtin_memcpy(&o, r, 16);
+	return o;
+}
 // elements c .. c + 7 of a line of `width` >= 8 out of the 16 bytes that were read at min(c, width - 8): moved down, zeros behind the line's end, without a branch
 __device__ inline T8 shift8(T8 raw, int c, int width) {
 	const int by = c - min(c, width - 8), d = by >> 1;
@@ -340,11 +354,18 @@ template <bool A_T, bool B_T, int EPI> __global__ __launch_bounds__(256) void k_
 	__shared__ __attribute__((aligned(16))) T lds[2][128 * TK];
 	any_tile<128, 128, 2, 2, A_T, B_T, EPI>(g, lds[0], lds[1], blockIdx.x, gridDim.x);
 }
-// dX and dW, which do not wait for each other, side by side: the first `blocks_x` blocks and the others
-__global__ __launch_bounds__(256) void k_products(GemmArgs x, GemmArgs w, uint32_t blocks_x) {
+// dX and dW, which do not wait for each other, side by side; the blocks with the longer sums begin
+struct Share { bool x; uint32_t index, count; };
+__device__ inline Share share_of(uint32_t blocks_x, uint32_t blocks_w, bool w_first) {
+	const uint32_t b = blockIdx.x, first = w_first ? blocks_w : blocks_x;
+	const bool x = (b < first) != w_first;
+	return {x, b < first ? b : b - first, x ? blocks_x : blocks_w};
+}
+__global__ __launch_bounds__(256) void k_products(GemmArgs x, GemmArgs w, uint32_t blocks_x, uint32_t blocks_w, bool w_first) {
 	__shared__ __attribute__((aligned(16))) T lds[2][128 * TK];
-	if (blockIdx.x < blocks_x) any_tile<128, 128, 2, 2, true, false, EPI_STORE>(x, lds[0], lds[1], blockIdx.x, blocks_x);
-	else any_tile<128, 128, 2, 2, false, false, EPI_STORE>(w, lds[0], lds[1], blockIdx.x - blocks_x, gridDim.x - blocks_x);
+	const Share s = share_of(blocks_x, blocks_w, w_first);
+	if (s.x) any_tile<128, 128, 2, 2, true, false, EPI_STORE>(x, lds[0], lds[1], s.index, s.count);
+	else any_tile<128, 128, 2, 2, false, false, EPI_STORE>(w, lds[0], lds[1], s.index, s.count);
 }
 
 // ---- operands whose lines are whole 16-byte pieces: straight from memory to LDS (buffer loads with the LDS bit; what lies outside the matrix arrives as zero) in units of 64 steps
@@ -429,7 +450,7 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS
 		const uint32_t seg = units_per_segment ? t_begin / units_per_segment : 0, t0 = (t_begin - seg * units_per_segment) * AK, steps8 = up8(g.steps);
 		ca.ld = g.lda; cb.ld = g.ldb; ca.inc = A_T ? AK : AK * g.lda; cb.inc = B_T ? AK : AK * g.ldb;
 		ca.lds = ca.lds0 = lds0; cb.lds = cb.lds0 = lds0 + UNITS_A * LA::BYTES;
-		ca.width = up8(g.rows) - r0; cb.width = g.cols - c0;
+		ca.width = up8(g.rows) - r0; cb.width = up8(g.cols) - c0;
 		ca.full = A_T ? records((int64_t)(min((uint32_t)BR, g.rows - r0) - 1) * (int64_t)g.lda + steps8) : records((int64_t)(AK - 1) * (int64_t)g.lda + ca.width);
 		cb.full = B_T ? records((int64_t)(min((uint32_t)OUT, g.cols - c0) - 1) * (int64_t)g.ldb + steps8) : records((int64_t)(AK - 1) * (int64_t)g.ldb + cb.width);
 		ca.seg = cb.seg = seg; ca.loaded = cb.loaded = t_begin; ca.end = cb.end = t_end; ca.left = cb.left = (int)(g.steps - t0);
@@ -580,16 +601,17 @@ template <int TILE, bool A_T, bool B_T, int EPI, int UNITS> __global__ __launch_
 	__shared__ __attribute__((aligned(1024))) char lds[async_lds(TILE, UNITS)];
 	async_tile<TILE, TILE, 2, 2, A_T, B_T, EPI, UNITS>(g, lds, blockIdx.x, gridDim.x);
 }
-template <int UNITS> __global__ __launch_bounds__(256, UNITS > 2 ? 1 : 2) void k_products_async(GemmArgs x, GemmArgs w, uint32_t blocks_x) { // (k_products)
+template <int UNITS> __global__ __launch_bounds__(256, UNITS > 2 ? 1 : 2) void k_products_async(GemmArgs x, GemmArgs w, uint32_t blocks_x, uint32_t blocks_w, bool w_first) { // (k_products)
 	__shared__ __attribute__((aligned(1024))) char lds[async_lds(128, UNITS)];
-	if (blockIdx.x < blocks_x) async_tile<128, 128, 2, 2, true, false, EPI_STORE, UNITS>(x, lds, blockIdx.x, blocks_x);
-	else async_tile<128, 128, 2, 2, false, false, EPI_STORE, UNITS>(w, lds, blockIdx.x - blocks_x, gridDim.x - blocks_x);
+	const Share s = share_of(blocks_x, blocks_w, w_first);
+	if (s.x) async_tile<128, 128, 2, 2, true, false, EPI_STORE, UNITS>(x, lds, s.index, s.count);
+	else async_tile<128, 128, 2, 2, false, false, EPI_STORE, UNITS>(w, lds, s.index, s.count);
 }
 
 // ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
 // straight from memory to registers as the matrix instruction's fragments, U loads on the way at a time; the samples (MT x 16 rows, the last one repeated where there are fewer)
 // come out of the caches.  `slices` wavefronts share the sum and add up in LDS, in their order; where there are few outputs blocks share it too (EPI_PARTIAL*).
-template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
+template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4;
 	__shared__ float sums[8][P][MT * 16][20]; // [wavefront][projection][row][output]
@@ -613,11 +635,11 @@ template <int MT, int EPI> __global__ __launch_bounds__(512) void k_few_rows(Gem
 #pragma unroll
 		for (int u = 0; u < U; ++u)
 #pragma unroll
-			for (int p = 0; p < P; ++p) fw[p][u] = load8(w[p] + t + u * 32);
+			for (int p = 0; p < P; ++p) fw[p][u] = ODD ? load8_odd(w[p] + t + u * 32) : load8(w[p] + t + u * 32);
 #pragma unroll
 		for (int u = 0; u < U; ++u)
 #pragma unroll
-			for (int m = 0; m < MT; ++m) fx[m][u] = load8(x[m] + t + u * 32);
+			for (int m = 0; m < MT; ++m) fx[m][u] = ODD ? load8_odd(x[m] + t + u * 32) : load8(x[m] + t + u * 32);
 #pragma unroll
 		for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -682,13 +704,15 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 	};
 	if (slab < slabs) load_x(slab);
 	constexpr int EACH_THREAD = NF * KS / 8, BATCH = EACH_THREAD < 8 ? EACH_THREAD : 8;
+	const bool odd = ((uintptr_t)g.b[0] | (uintptr_t)g.b[GATED ? 1 : 0] | g.ldb * 2) & 3;
 #pragma unroll
 	for (int q0 = 0; q0 < EACH_THREAD; q0 += BATCH) { // (all loads of a batch on their way together)
 		T8 v[BATCH];
 #pragma unroll
 		for (int b = 0; b < BATCH; ++b) {
 			const int q = (q0 + b) * 512 + threadIdx.x, l = q & 63, k = (q >> 6) % KS, f = (q >> 6) / KS, i = l & 15, col = (f / 2 % (OF / 2)) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3);
-			v[b] = load8(g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb + min(k * 32 + (l >> 4) * 8, steps - 8));
+			const T* p = g.b[GATED && f >= OF] + (uint64_t)min((uint32_t)col, g.cols - 1) * g.ldb + min(k * 32 + (l >> 4) * 8, steps - 8);
+			v[b] = odd ? load8_odd(p) : load8(p);
 		}
 #pragma unroll
 		for (int b = 0; b < BATCH; ++b) {
@@ -1021,6 +1045,46 @@ __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
+// X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else
+struct PackArgs { const T* from[3]; T* to[3]; uint64_t ld[3]; uint32_t lines[3]; uint32_t width; };
+__global__ __launch_bounds__(256) void k_pack(PackArgs g) {
+	const uint32_t cc = up8(g.width) / 8;
+	uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+#pragma unroll
+	for (int k = 0; k < 3; ++k) {
+		const uint64_t n = (uint64_t)g.lines[k] * cc;
+		if (id < n) {
+			const uint32_t line = (uint32_t)(id / cc), c = (uint32_t)(id % cc) * 8;
+			const T* p = g.from[k] + (uint64_t)line * g.ld[k];
+			const int start = min((int)c, (int)g.width - 8);
+			*(T8*)(g.to[k] + ((uint64_t)line * cc * 8 + c)) = shift8(load8_odd(p + start), c, g.width);
+			return;
+		}
+		id -= n;
+	}
+}
+// what the products read: the caller's matrices, or packed ones
+struct Operands { const T* x; const T* w[2]; uint64_t ld_x, ld_w; bool whole_x, whole_w; };
+Operands operands(hipStream_t s, const DenseArgs& d, void* packed) {
+	Operands o{(const T*)d.x, {(const T*)d.w[0], (const T*)d.w[1]}, d.x_stride, d.w_stride, false, false};
+	if (dense_pack_bytes(d.m, d.n, d.k, d.gated)) {
+		PackArgs a{};
+		const uint64_t k8 = up8(d.k);
+		T* to = (T*)packed;
+		const void* from[3] = {d.x, d.w[0], d.gated ? d.w[1] : nullptr};
+		uint64_t chunks = 0;
+		a.width = d.k;
+		for (int i = 0; i < 3; ++i) {
+			a.from[i] = (const T*)from[i]; a.ld[i] = i ? d.w_stride : d.x_stride; a.lines[i] = from[i] ? (i ? d.n : d.m) : 0; a.to[i] = to;
+			to += (i ? d.n : d.m) * k8; chunks += a.lines[i] * (k8 / 8);
+		}
+		hipLaunchKernelGGL(k_pack, dim3(div_up(chunks, 256)), dim3(256), 0, s, a);
+		o = {a.to[0], {a.to[1], a.to[2]}, k8, k8, true, true};
+	} else {
+		o.whole_x = whole(d.x, d.x_stride, d.k); o.whole_w = whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
+	}
+	return o;
+}
 int join_groups(const GemmArgs& g) { return g.splits >= 16 ? 8 : 1; }
 uint32_t join_blocks(const GemmArgs& g) { return div_up((uint64_t)g.rows * (up8(g.cols) / 8), 256 / join_groups(g)) * g.problems; }
 template <int EPI> void launch_join(hipStream_t s, GemmArgs g) { g.problems = 1; hipLaunchKernelGGL((k_join_splits<EPI>), dim3(join_blocks(g)), dim3(256), 0, s, g, join_groups(g)); }
@@ -1056,15 +1120,19 @@ void launch_finish(hipStream_t s, const GemmArgs* x, const GemmArgs* w, const Bi
 	const uint32_t bx = x->splits > 1 ? join_blocks(*x) : 0, bw = w->splits > 1 ? join_blocks(*w) : 0, bb = bias.partial ? div_up(bias.cols, 16) * bias.problems : 0;
 	if (bx + bw + bb) hipLaunchKernelGGL(k_finish, dim3(bx + bw + bb), dim3(256), 0, s, *x, join_groups(*x), bx, *w, join_groups(*w), bw, bias);
 }
+bool odd_lines(const void* p, uint64_t ld) { return ((uintptr_t)p | ld * 2) & 3; }
 template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, float* partial) {
 	const DenseFewRows f = dense_few_rows(g.cols, g.steps);
 	const dim3 grid(div_up(div_up(g.cols, 16), 8 / f.slices), f.splits);
 	const uint32_t per = (div_up(g.steps, f.slices * f.splits) + 31) & ~31u;
+	const bool odd = odd_lines(g.a, g.lda) || odd_lines(g.b[0], g.ldb) || odd_lines(g.b[1], g.ldb);
 	g.splits = f.splits; g.partial = partial;
+	constexpr int PART = EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL;
 	if (f.splits > 1) {
-		hipLaunchKernelGGL((k_few_rows<MT, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>), grid, dim3(512), 0, s, g, f.slices, per);
+		if (odd) hipLaunchKernelGGL((k_few_rows<MT, PART, true>), grid, dim3(512), 0, s, g, f.slices, per); else hipLaunchKernelGGL((k_few_rows<MT, PART, false>), grid, dim3(512), 0, s, g, f.slices, per);
 		launch_join<EPI>(s, g);
-	} else hipLaunchKernelGGL((k_few_rows<MT, EPI>), grid, dim3(512), 0, s, g, f.slices, per);
+	} else if (odd) hipLaunchKernelGGL((k_few_rows<MT, EPI, true>), grid, dim3(512), 0, s, g, f.slices, per);
+	else hipLaunchKernelGGL((k_few_rows<MT, EPI, false>), grid, dim3(512), 0, s, g, f.slices, per);
 }
 template <int NF, int EPI> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
 	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI>), dim3(blocks), dim3(512), 0, s, g);
@@ -1104,7 +1172,9 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
 		return;
 	}
-	const bool wholes = whole(d.x, d.x_stride, d.k) && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
+	const Operands o = operands(s, d, (char*)d.workspace + dense_forward_bytes(d.m, d.n, d.k, d.gated) - dense_pack_bytes(d.m, d.n, d.k, d.gated));
+	const bool wholes = o.whole_x && o.whole_w;
+	g.a = o.x; g.lda = o.ld_x; g.b[0] = o.w[0]; g.b[1] = o.w[1]; g.ldb = o.ld_w;
 	if (d.gated) launch_forward<EPI_GATED>(s, g, wholes, partial); else launch_forward<EPI_LINEAR>(s, g, wholes, partial);
 }
 void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
@@ -1147,22 +1217,24 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	GemmArgs x{}, w{};
 	bool large_x = false, large_w = false;
 	const bool want_x = d.dx && d.m && d.k, want_w = d.dw[0] && d.n && d.k;
-	const bool whole_x = g_whole && whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k), whole_w = g_whole && whole(d.x, d.x_stride, d.k);
+	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack) : Operands{};
+	const bool whole_x = g_whole && o.whole_w, whole_w = g_whole && o.whole_x;
 	if (want_x) {
-		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = (const T*)d.w[0]; x.b[1] = (const T*)d.w[1]; x.ldb = d.w_stride;
+		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = o.w[0]; x.b[1] = o.w[1]; x.ldb = o.ld_w;
 		x.rows = d.m; x.cols = d.k; x.steps = d.n; x.problems = 1; x.c[0] = (T*)d.dx; x.ldc = d.dx_stride;
 		large_x = set_split(x, 1, (float*)(ws + p.partial_x)) && whole_x;
 	}
 	if (want_w) {
-		w.a = G; w.lda = ldg; w.a_problem = up8(d.n); w.problems = problems; w.b[0] = w.b[1] = (const T*)d.x; w.ldb = d.x_stride;
+		w.a = G; w.lda = ldg; w.a_problem = up8(d.n); w.problems = problems; w.b[0] = w.b[1] = o.x; w.ldb = o.ld_x;
 		w.rows = d.n; w.cols = d.k; w.steps = d.m; w.segments = 1; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
 		large_w = set_split(w, problems, (float*)(ws + p.partial)) && whole_w;
 	}
 	if (want_x && want_w && !large_x && !large_w && whole_x == whole_w) {
 		const uint32_t bx = tiles<EPI_STORE>(x, 128), bw = tiles<EPI_STORE>(w, 128);
-		if (!whole_x) hipLaunchKernelGGL(k_products, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
-		else if (bx + bw <= 256) hipLaunchKernelGGL(k_products_async<4>, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
-		else hipLaunchKernelGGL(k_products_async<2>, dim3(bx + bw), dim3(256), 0, s, x, w, bx);
+		const bool w_first = w.chunks_per_split > x.chunks_per_split;
+		if (!whole_x) hipLaunchKernelGGL(k_products, dim3(bx + bw), dim3(256), 0, s, x, w, bx, bw, w_first);
+		else if (bx + bw <= 256) hipLaunchKernelGGL(k_products_async<4>, dim3(bx + bw), dim3(256), 0, s, x, w, bx, bw, w_first);
+		else hipLaunchKernelGGL(k_products_async<2>, dim3(bx + bw), dim3(256), 0, s, x, w, bx, bw, w_first);
 	} else {
 		if (want_x) launch_tiles<true, false, EPI_STORE>(s, x, whole_x, large_x);
 		if (want_w) launch_tiles<false, false, EPI_STORE>(s, w, whole_w, large_w);
