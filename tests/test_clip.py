@@ -77,6 +77,17 @@ def test_clip(hip, spec, in_place, over, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("spec", [[(65535, H)], [(65536, B)], [(65537, F)], [(0, H)] * 111 + [(70000, B), (0, F), (9, H)], [(100, H)] * 112 + [(60000, F)], [(8192, B)] * 112 + [(0, F)] * 130 + [(8193, H)] * 3, [(0, F)] * 300 + [(5, H)]])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_tables(hip, spec, in_place):
+    """either side of what one block does alone; tensors over several tables, empty ones at their ends, a table of nothing"""
+    s = Set(spec, in_place, shift=1, seed=len(spec))
+    max_norm = float(np.float32(s.exact(64.0) * 0.7))
+    s.clip(64.0, max_norm)
+    s.check(64.0, max_norm)
+
+
+@pytest.mark.gpu
 def test_wide_range(hip):
     """squares beyond and below what 32 bits hold"""
     for scale in (1e30, 1e-30):

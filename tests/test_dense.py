@@ -486,6 +486,122 @@ def test_block_of_layers_with_the_trainer(hip):
         L.ngp_encmlp_destroy(em)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [A.TYPE_HALF, A.TYPE_BFLOAT16])
+@pytest.mark.parametrize("m,n,k,gated", [(333, 777, 501, False), (257, 650, 321, True), (1000, 1000, 1003, False), (40, 2100, 1202, False), (3000, 263, 255, False)])
+@pytest.mark.parametrize("pad,shift", [((0, 0, 0), 0), ((3, 2, 1), 1)])
+def test_odd_lines(hip, type_, m, n, k, gated, pad, shift):
+    """many products over lines that are no whole 16-byte pieces"""
+    run_layer(Layer(type_, A.ACT_SILU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 16, 17, 32])
+@pytest.mark.parametrize("n,k", [(8, 8192), (5, 4099), (40, 12290), (1000, 33), (2500, 129), (130, 1025)])
+@pytest.mark.parametrize("gated,pad,shift", [(False, (0, 0, 0), 0), (True, (0, 0, 0), 0), (False, (1, 0, 1), 1), (True, (2, 4, 0), 2)])
+def test_few_samples(hip, m, n, k, gated, pad, shift):
+    """the sum shared by wavefronts and, where the outputs are few, by blocks"""
+    run_layer(Layer(A.TYPE_HALF, A.ACT_GELU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift), backward=False)
+    run_layer(Layer(A.TYPE_BFLOAT16, A.ACT_SILU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift), save=False, backward=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated", [(33, 8, 8, False), (33, 16, 256, False), (50, 9, 11, True), (1000, 100, 200, False), (777, 64, 40, True), (2049, 128, 129, False), (515, 33, 250, True), (4100, 250, 100, False),
+                                         (33001, 256, 256, False), (32768, 255, 250, False), (33333, 128, 255, True), (40000, 200, 256, False)])
+@pytest.mark.parametrize("pad,shift", [((0, 0, 0), 0), ((1, 3, 5), 1)])
+def test_narrow_layers(hip, m, n, k, gated, pad, shift):
+    """all weights in one compute unit, every size of it, samples that do not fill the last block"""
+    run_layer(Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift))
+    run_layer(Layer(A.TYPE_BFLOAT16, A.ACT_GELU, m, n, k, gated=gated, bias=False, pad=pad, shift=shift), want="xw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [A.TYPE_HALF, A.TYPE_BFLOAT16])
+@pytest.mark.parametrize("m,n,k,gated", [(3700, 3593, 136, False), (3601, 1800, 72, True), (200, 96, 20000, False), (100, 40, 9001, True), (20000, 136, 264, True), (136, 264, 5008, False), (33, 4104, 1032, False), (4100, 4100, 40, False)])
+def test_tiles(hip, type_, m, n, k, gated):
+    """256 x 256 tiles with ragged edges; sums split over blocks in the forward pass, in dX, in dW; the two products of a backward pass side by side with either one the longer"""
+    run_layer(Layer(type_, A.ACT_RELU, m, n, k, gated=gated, residual=not gated))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated", [(2, 16, 8192, False), (100, 48, 9000, True), (257, 650, 321, True), (40000, 64, 64, False)])
+def test_bits_of_shared_sums(hip, m, n, k, gated):
+    """sums that blocks share are joined in a fixed order, whatever the workspace held"""
+    layer = Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=gated)
+    runs = []
+    for _ in range(3):
+        y, pre = layer.forward()
+        dx, dw, db = layer.backward(pre)
+        runs.append([v[1].clone() for v in [y, *pre, dx, *dw, *db]])
+    for r in runs[1:]:
+        assert all(bool((a == b).all()) for a, b in zip(r, runs[0]))
+    layer.untouched()
+
+
+@pytest.mark.gpu
+def test_two_layers_at_once(hip):
+    """two streams, and two graphs replayed on two streams, each layer with a workspace of its own"""
+    import torch
+    layers = [Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=g, seed=i) for i, (m, n, k, g) in enumerate([(300, 264, 1001, False), (300, 264, 1001, True), (5, 24, 9000, False), (900, 136, 2048, False)])]
+    L, want = lib(), []
+    P = Layer.p
+
+    def buffers(a):
+        y, pre = a.out(a.m, a.n), [a.out(a.m, a.n) for _ in a.w]
+        dx, dw, db = a.out(a.m, a.k), [a.out(a.n, a.k) for _ in a.w], [a.out(1, a.n) for _ in a.w]
+        size = (L.ngp_gated_workspace_size if a.gated else L.ngp_linear_workspace_size)
+        sizes = size(a.m, a.n, a.k, 0), size(a.m, a.n, a.k, 1)
+        return y, pre, dx, dw, db, torch.full((max(sizes) + 16,), 255, dtype=torch.uint8, device="cuda"), sizes
+
+    def run(a, b, s):
+        y, pre, dx, dw, db, ws, sizes = b
+        m, n, k = a.m, a.n, a.k
+        if a.gated:
+            A.check(L, L.ngp_gated_forward(s, a.type, a.act, m, n, k, P(a, a.x), k, P(a, a.w[0]), P(a, a.w[1]), k, P(a, a.bias[0]), P(a, a.bias[1]), P(a, y), n, P(a, pre[0]), P(a, pre[1]), n, ws.data_ptr(), sizes[0]))
+            A.check(L, L.ngp_gated_backward(s, a.type, a.act, m, n, k, P(a, a.x), k, P(a, a.w[0]), P(a, a.w[1]), k, P(a, pre[0]), P(a, pre[1]), n, P(a, a.dy), n, P(a, dx), k, P(a, dw[0]), P(a, dw[1]), k,
+                                            P(a, db[0]), P(a, db[1]), ws.data_ptr(), sizes[1]))
+        else:
+            A.check(L, L.ngp_linear_forward(s, a.type, a.act, m, n, k, P(a, a.x), k, P(a, a.w[0]), k, P(a, a.bias[0]), None, 0, P(a, y), n, P(a, pre[0]), n, ws.data_ptr(), sizes[0]))
+            A.check(L, L.ngp_linear_backward(s, a.type, a.act, m, n, k, P(a, a.x), k, P(a, a.w[0]), k, P(a, pre[0]), n, P(a, a.dy), n, P(a, dx), k, P(a, dw[0]), k, P(a, db[0]), ws.data_ptr(), sizes[1]))
+
+    def results(b):
+        return [v[1].clone() for v in [b[0], *b[1], b[2], *b[3], *b[4]]]
+    work = [buffers(a) for a in layers]
+    for a, b in zip(layers, work):
+        run(a, b, None)
+        torch.cuda.synchronize()
+        want.append(results(b))
+        for v in [b[0], *b[1], b[2], *b[3], *b[4]]:
+            v[1].fill_(3.0)
+    streams = [torch.cuda.Stream() for _ in layers]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for a, b, st in zip(layers, work, streams):
+            run(a, b, st.cuda_stream)
+    torch.cuda.synchronize()
+    for b, w in zip(work, want):
+        assert all(bool((p == q).all()) for p, q in zip(results(b), w))
+        for v in [b[0], *b[1], b[2], *b[3], *b[4]]:
+            v[1].fill_(4.0)
+    graphs = []
+    for a, b in zip(layers, work):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(a, b, torch.cuda.current_stream().cuda_stream)
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for b, w in zip(work, want):
+            assert all(bool((p == q).all()) for p, q in zip(results(b), w))
+            for v in [b[0], *b[1], b[2], *b[3], *b[4]]:
+                v[1].fill_(5.0)
+            b[5].fill_(255)
+        torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------------------------ refusals (host only: nothing is launched)
 
 def forward_args(**kw):
@@ -562,4 +678,21 @@ def test_workspace_sizes():
         for f, problems in ((L.ngp_linear_workspace_size, 1), (L.ngp_gated_workspace_size, 2)):
             assert f(m, n, k, 0) >= 0
             s = f(m, n, k, 1)
-            assert s >= problems * 2 * m * n and s <= problems * 2 * m * (n + 8) + (300 << 20)
+            # at most the gradients of the pre-activations and a bounded set of partial sums; layers whose weights fit a compute unit never store the former, the others have to
+            assert s <= problems * 2 * m * (n + 8) + (300 << 20) and (s >= problems * 2 * m * n or (problems * n <= 256 and k <= 256))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(2, 16, 8192), (100, 64, 9000), (333, 777, 501)])
+def test_forward_workspace(gated, m, n, k):
+    """sums that blocks share and padded operands need room in the forward pass too: its size is asked for and held to"""
+    L = lib()
+    size = (L.ngp_gated_workspace_size if gated else L.ngp_linear_workspace_size)(m, n, k, 0)
+    assert size > 0
+    a = [1 << 32 | i << 28 for i in range(8)]
+    for work, have, what in ((None, 0, "workspace"), (a[6], size - 1, "workspace"), (a[6] + 8, size, "workspace"), (a[3], size, "overlaps"), (a[0], size, "overlaps")):
+        if gated:
+            rc = L.ngp_gated_forward(None, A.TYPE_HALF, A.ACT_SILU, m, n, k, a[0], k, a[1], a[2], k, None, None, a[3], n, a[4], a[5], n, work, have)
+        else:
+            rc = L.ngp_linear_forward(None, A.TYPE_HALF, A.ACT_SILU, m, n, k, a[0], k, a[1], k, None, None, 0, a[3], n, a[4], n, work, have)
+        assert rc != 0 and what in L.ngp_last_error().decode()
