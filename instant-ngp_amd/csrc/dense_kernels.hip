@@ -94,7 +94,7 @@ __device__ inline T8 shift8(T8 raw, int c, int width) {
 	return r;
 }
 // COUNT chunks of 8 elements of lines of one width, all on their way together: at(q, line) gives the line and returns the column.  Lines of 8 elements and more are read in whole chunks
-// (at min(column, width - 8): shift8 puts them right later), shorter ones element by element.
+// (at min(column, width - 8): shift8 puts them right later), shorter ones element by element.  (By the dword, as above, tiles of odd lines ran 15 % longer: they wait for other things.)
 template <int COUNT, typename F> __device__ inline void load_chunks(T8* out, int width, F&& at) {
 	if (width >= 8) {
 #pragma unroll
@@ -104,7 +104,10 @@ template <int COUNT, typename F> __device__ inline void load_chunks(T8* out, int
 		for (int q = 0; q < COUNT; ++q) { const T* line; const int c = at(q, line); out[q] = load8(line + c, width - c); }
 	}
 }
-__device__ inline void store8(T* p, T8 v, int n) {
+// `streamed`: past the caches
+__device__ inline void store8(T* p, T8 v, int n, bool streamed = false) {
+	typedef float any4 __attribute__((ext_vector_type(4), aligned(2)));
+	if (streamed && n >= 8) { __builtin_nontemporal_store(__builtin_bit_cast(f4v, v), (any4*)p); return; }
 	if (n >= 8) { __builtin_memcpy(p, &v, 16); return; }
 #pragma unroll
 	for (int i = 0; i < 8; ++i) if (i < n) p[i] = v[i];
@@ -137,15 +140,16 @@ __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 va
 		default: break;
 	}
 }
-// f(activation as a constant): one branch for a whole loop, whose code then stays small (an epilogue with the branch in every row ran 2.5 times longer, waiting for instructions)
-template <typename F> __device__ inline void with_act(int act, F&& f) {
+// f(activation, streamed or not, as constants): one branch for a whole loop, whose code then stays small (an epilogue with the branch in every row ran 2.5 times longer, waiting for instructions)
+template <typename F> __device__ inline void with_act(int act, bool streamed, F&& f) {
+	auto g = [&](auto act_c) { if (streamed) f(act_c, std::true_type()); else f(act_c, std::false_type()); };
 	switch (act) {
-		case NGP_ACT_RELU: f(std::integral_constant<int, NGP_ACT_RELU>()); break;
-		case NGP_ACT_LOGISTIC: f(std::integral_constant<int, NGP_ACT_LOGISTIC>()); break;
-		case NGP_ACT_EXPONENTIAL: f(std::integral_constant<int, NGP_ACT_EXPONENTIAL>()); break;
-		case NGP_ACT_SILU: f(std::integral_constant<int, NGP_ACT_SILU>()); break;
-		case NGP_ACT_GELU: f(std::integral_constant<int, NGP_ACT_GELU>()); break;
-		default: f(std::integral_constant<int, NGP_ACT_NONE>()); break;
+		case NGP_ACT_RELU: g(std::integral_constant<int, NGP_ACT_RELU>()); break;
+		case NGP_ACT_LOGISTIC: g(std::integral_constant<int, NGP_ACT_LOGISTIC>()); break;
+		case NGP_ACT_EXPONENTIAL: g(std::integral_constant<int, NGP_ACT_EXPONENTIAL>()); break;
+		case NGP_ACT_SILU: g(std::integral_constant<int, NGP_ACT_SILU>()); break;
+		case NGP_ACT_GELU: g(std::integral_constant<int, NGP_ACT_GELU>()); break;
+		default: g(std::integral_constant<int, NGP_ACT_NONE>()); break;
 	}
 }
 // G of 8 outputs: dY act'(Z); gated: dY Zu act'(Zg) and dY act(Zg).  Zeros give zeros.
@@ -203,12 +207,13 @@ struct GemmArgs {
 	T* c[2]; uint64_t ldc;
 	float* partial;                        // [split][problem][rows][cols8]
 	int act; const T* bias[2]; const T* residual; uint64_t ld_residual; T* pre[2]; uint64_t ld_pre;
+	bool streamed; // a forward pass's outputs are more than the caches hold: written past them
 };
 __host__ __device__ inline uint32_t up8(uint32_t v) { return (v + 7) & ~7u; }
 
 // What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C.  Biases and the residual come as values: a caller
 // with several rows loads them ahead.
-template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual, int act) {
+template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual, int act, bool streamed = false) {
 	T8 o, s;
 	if constexpr (EPI == EPI_PARTIAL || EPI == EPI_PARTIAL2) {
 		const uint32_t parts = EPI == EPI_PARTIAL2 ? 2 : g.problems;
@@ -224,17 +229,17 @@ template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t 
 		return;
 	}
 	EACH z[e] += (float)bias0[e];
-	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n); }
+	if (g.pre[0]) { EACH s[e] = (T)z[e]; store8(g.pre[0] + (uint64_t)r * g.ld_pre + c, s, n, streamed); }
 	act_value8(act, z);
 	if constexpr (EPI == EPI_LINEAR) {
 		if (g.residual) { EACH z[e] += (float)residual[e]; }
 		EACH o[e] = (T)z[e];
 	} else {
 		EACH u[e] += (float)bias1[e];
-		if (g.pre[1]) { EACH s[e] = (T)u[e]; store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n); }
+		if (g.pre[1]) { EACH s[e] = (T)u[e]; store8(g.pre[1] + (uint64_t)r * g.ld_pre + c, s, n, streamed); }
 		EACH o[e] = (T)(z[e] * u[e]);
 	}
-	store8(g.c[0] + (uint64_t)r * g.ldc + c, o, n);
+	store8(g.c[0] + (uint64_t)r * g.ldc + c, o, n, streamed);
 }
 template <int EPI> constexpr bool GATED_TILE = EPI == EPI_GATED || EPI == EPI_PARTIAL2; // the tile's columns are gate and up outputs
 template <int EPI> __device__ inline T8 bias8(const GemmArgs& g, int k, uint32_t c, int n) { return (EPI == EPI_LINEAR || EPI == EPI_GATED) && g.bias[k] && n > 0 ? load8(g.bias[k] + c, n) : T8{}; }
@@ -568,7 +573,7 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS
 			}
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the strip is this wavefront's alone)
 		const uint32_t r_pass = r0 + wr * (BR / WR) + pass * PASS * 16 + er;
-		auto rows = [&](auto act_c) {
+		auto rows = [&](auto act_c, auto streamed_c) {
 			T8 next[AT_ONCE];
 			auto load_residual = [&](int k) {
 #pragma unroll
@@ -588,11 +593,11 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS
 					const float* p = strip + (k + q * ROWS + er) * STRIP + ec;
 					*(f4v*)z = *(const f4v*)p; *(f4v*)(z + 4) = *(const f4v*)(p + 4);
 					if constexpr (GATED_TILE<EPI>) { *(f4v*)u = *(const f4v*)(p + OUT / WC); *(f4v*)(u + 4) = *(const f4v*)(p + OUT / WC + 4); }
-					if (r < g.rows && n > 0) epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias0, bias1, residual[q], decltype(act_c)::value);
+					if (r < g.rows && n > 0) epilogue8<EPI>(g, problem, split, r, c, n, z, u, bias0, bias1, residual[q], decltype(act_c)::value, decltype(streamed_c)::value);
 				}
 			}
 		};
-		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) with_act(g.act, rows); else rows(std::integral_constant<int, NGP_ACT_NONE>());
+		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) with_act(g.act, g.streamed, rows); else rows(std::integral_constant<int, NGP_ACT_NONE>(), std::false_type());
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
 }
@@ -733,7 +738,7 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 			for (int f = 0; f < NF; ++f) acc[f] = mfma(*(const T8*)(w + ((f * KS + k) * 64 + lane) * 8), x[k], acc[f]);
 		if (slab + stride < slabs) load_x(slab + stride);
 		const uint32_t r = slab * 16 + li;
-		if (r < g.rows) with_act(g.act, [&](auto act_c) {
+		if (r < g.rows) with_act(g.act, g.streamed, [&](auto act_c, auto streamed_c) {
 #pragma unroll
 			for (int p = 0; p < OF / 2; ++p) {
 				const uint32_t c = p * 32 + gq * 8;
@@ -741,7 +746,7 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 				const int n = (int)min(8u, g.cols - c);
 				float z[8], u[8];
 				EACH { z[e] = acc[2 * p + e / 4][e & 3]; u[e] = GATED ? acc[(GATED ? OF : 0) + 2 * p + e / 4][e & 3] : 0.f; }
-				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), decltype(act_c)::value);
+				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), decltype(act_c)::value, decltype(streamed_c)::value);
 			}
 		});
 	}
@@ -939,14 +944,16 @@ struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; con
 template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
 	const uint32_t cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 256 + cx * 8, pc = up8(g.cols);
 	const uint32_t end = min(g.rows, (blockIdx.y + 1) * g.rows_per_block);
+	const bool odd = ((uintptr_t)g.dy | (uintptr_t)g.pre[0] | (uintptr_t)g.pre[1] | g.ld_dy * 2 | g.ld_pre * 2) & 3;
 	float sum[GATED ? 2 : 1][8] = {};
 	if (c < g.cols) {
 		const int n = (int)min(8u, g.cols - c);
 		for (uint32_t r = blockIdx.y * g.rows_per_block + ry; r < end; r += 8) {
-			const T8 dy = load8(g.dy + (uint64_t)r * g.ld_dy + c, n);
+			auto load = [&](const T* p) -> T8 { return n < 8 ? load8(p, n) : odd ? load8_odd(p) : load8(p); };
+			const T8 dy = load(g.dy + (uint64_t)r * g.ld_dy + c);
 			T8 z{}, u{}, o, o2;
-			if (g.pre[0]) z = load8(g.pre[0] + (uint64_t)r * g.ld_pre + c, n);
-			if (GATED) u = load8(g.pre[1] + (uint64_t)r * g.ld_pre + c, n);
+			if (g.pre[0]) z = load(g.pre[0] + (uint64_t)r * g.ld_pre + c);
+			if (GATED) u = load(g.pre[1] + (uint64_t)r * g.ld_pre + c);
 			float v[8], v2[8];
 			output_grad8<GATED>(g.act, dy, z, u, v, v2);
 			EACH { sum[0][e] += v[e]; o[e] = (T)v[e]; if (GATED) { sum[GATED ? 1 : 0][e] += v2[e]; o2[e] = (T)v2[e]; } }
@@ -1044,8 +1051,8 @@ __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 15) == 0 && (ld & 7) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces; a tile's offsets fit 31 bits
-// X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else
+bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 3) == 0 && (ld & 1) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces, each from a dword on; a tile's offsets fit 31 bits
+// X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else; memory bound
 struct PackArgs { const T* from[3]; T* to[3]; uint64_t ld[3]; uint32_t lines[3]; uint32_t width; };
 __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
 	const uint32_t cc = up8(g.width) / 8;
@@ -1063,26 +1070,25 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
 		id -= n;
 	}
 }
-// what the products read: the caller's matrices, or packed ones
+// what the products read: the caller's matrices, or (with `room` for them) packed ones
 struct Operands { const T* x; const T* w[2]; uint64_t ld_x, ld_w; bool whole_x, whole_w; };
-Operands operands(hipStream_t s, const DenseArgs& d, void* packed) {
-	Operands o{(const T*)d.x, {(const T*)d.w[0], (const T*)d.w[1]}, d.x_stride, d.w_stride, false, false};
-	if (dense_pack_bytes(d.m, d.n, d.k, d.gated)) {
-		PackArgs a{};
-		const uint64_t k8 = up8(d.k);
-		T* to = (T*)packed;
-		const void* from[3] = {d.x, d.w[0], d.gated ? d.w[1] : nullptr};
-		uint64_t chunks = 0;
-		a.width = d.k;
-		for (int i = 0; i < 3; ++i) {
-			a.from[i] = (const T*)from[i]; a.ld[i] = i ? d.w_stride : d.x_stride; a.lines[i] = from[i] ? (i ? d.n : d.m) : 0; a.to[i] = to;
-			to += (i ? d.n : d.m) * k8; chunks += a.lines[i] * (k8 / 8);
-		}
-		hipLaunchKernelGGL(k_pack, dim3(div_up(chunks, 256)), dim3(256), 0, s, a);
-		o = {a.to[0], {a.to[1], a.to[2]}, k8, k8, true, true};
-	} else {
-		o.whole_x = whole(d.x, d.x_stride, d.k); o.whole_w = whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k);
-	}
+Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room) {
+	Operands o{(const T*)d.x, {(const T*)d.w[0], (const T*)d.w[1]}, d.x_stride, d.w_stride, whole(d.x, d.x_stride, d.k), whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k)};
+	if (!room || (o.whole_x && o.whole_w)) return o;
+	PackArgs a{};
+	const uint64_t k8 = up8(d.k);
+	T* to = (T*)packed;
+	uint64_t chunks = 0;
+	auto pack = [&](int i, const T*& p, uint64_t lines, uint64_t ld) {
+		if (!p) return;
+		a.from[i] = p; a.ld[i] = ld; a.lines[i] = (uint32_t)lines; p = a.to[i] = to;
+		to += lines * k8; chunks += lines * (k8 / 8);
+	};
+	a.width = d.k;
+	if (!o.whole_x) { pack(0, o.x, d.m, d.x_stride); o.ld_x = k8; }
+	if (!o.whole_w) { pack(1, o.w[0], d.n, d.w_stride); pack(2, o.w[1], d.n, d.w_stride); o.ld_w = k8; }
+	if (chunks) hipLaunchKernelGGL(k_pack, dim3(div_up(chunks, 256)), dim3(256), 0, s, a);
+	o.whole_x = o.whole_w = true;
 	return o;
 }
 int join_groups(const GemmArgs& g) { return g.splits >= 16 ? 8 : 1; }
@@ -1162,6 +1168,9 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1;
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
+	// Outputs that the 256 MB of the last cache would not hold beside the inputs go past the caches (262144 x 256 from 64 inputs: 95 -> 78 us; 8192 x 4096 x 2 from 4096: 237 -> 224 us); smaller
+	// ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us)
+	g.streamed = (uint64_t)d.m * d.n * 2 * (1 + (d.pre[0] != nullptr) + (d.pre[1] != nullptr)) >= 128ull << 20;
 	float* partial = (float*)d.workspace;
 	if (d.m <= FEW_ROWS && d.k) {
 		if (d.m <= 16) { if (d.gated) launch_few_rows<1, EPI_GATED>(s, g, partial); else launch_few_rows<1, EPI_LINEAR>(s, g, partial); }
@@ -1172,7 +1181,8 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
 		return;
 	}
-	const Operands o = operands(s, d, (char*)d.workspace + dense_forward_bytes(d.m, d.n, d.k, d.gated) - dense_pack_bytes(d.m, d.n, d.k, d.gated));
+	const uint64_t room = dense_pack_bytes(d.m, d.n, d.k, d.gated, false);
+	const Operands o = operands(s, d, (char*)d.workspace + dense_forward_bytes(d.m, d.n, d.k, d.gated) - room, room != 0);
 	const bool wholes = o.whole_x && o.whole_w;
 	g.a = o.x; g.lda = o.ld_x; g.b[0] = o.w[0]; g.b[1] = o.w[1]; g.ldb = o.ld_w;
 	if (d.gated) launch_forward<EPI_GATED>(s, g, wholes, partial); else launch_forward<EPI_LINEAR>(s, g, wholes, partial);
@@ -1217,7 +1227,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	GemmArgs x{}, w{};
 	bool large_x = false, large_w = false;
 	const bool want_x = d.dx && d.m && d.k, want_w = d.dw[0] && d.n && d.k;
-	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack) : Operands{};
+	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack, p.bytes > p.pack) : Operands{};
 	const bool whole_x = g_whole && o.whole_w, whole_w = g_whole && o.whole_x;
 	if (want_x) {
 		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = o.w[0]; x.b[1] = o.w[1]; x.ldb = o.ld_w;

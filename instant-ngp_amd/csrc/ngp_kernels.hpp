@@ -389,16 +389,20 @@ inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint64_t cols = (gated ? 2 * (uint64_t)n : n);
 	return n >= 8 && k >= 8 && k <= 256 && cols <= 256 && m > FEW_ROWS && (cols * k <= 32768 || m >= 32768);
 }
-// Tiles read whole 16-byte pieces; lines of another length are copied first (into the workspace, padded) where the products are worth it, else read piecemeal: 4096 x 4096 outputs of 1001
-// inputs 73.6 us piecemeal, 43.3 us + the copy.
-inline uint64_t dense_pack_bytes(uint64_t m, uint64_t n, uint64_t k, bool gated) {
-	if (!(k & 7) || k < 8 || m <= FEW_ROWS || dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) || (double)m * (double)n * (double)k * (gated ? 2 : 1) < 1e8) return 0;
-	return ((m + (gated ? 2 : 1) * n) * ((k + 7) & ~7ull) * 2 + 255) & ~255ull;
+// Tiles take operands of whole 16-byte pieces at even elements straight to LDS; others are copied into the workspace first (lines padded) where that pays, else staged through registers.
+// us copied / staged, 1004 inputs: forward 65536 samples 400 outputs 125 / 117, 1032 outputs 229 / 264; 4096 samples 2056 outputs 45 / 53; 200 samples, 2004 inputs, 2056 outputs 23.5 / 19.7.
+// Backward 65536 samples 400 outputs 290 / 268, 1032 outputs 512 / 592; 4096 samples (8 MB of inputs, which caches hold) 400 outputs 34 / 38; 64 samples, 4100 inputs, 520 outputs 21 / 21.
+// The backward pass has the room whatever k is, for lines at odd strides (2000 samples 1000 x 1000: 70 staged); a forward pass only where lines are no whole pieces by themselves.
+inline uint64_t dense_pack_bytes(uint64_t m, uint64_t n, uint64_t k, bool gated, bool backward) {
+	const uint64_t cols = (gated ? 2 : 1) * n;
+	if ((!backward && !(k & 7)) || k < 8 || m <= FEW_ROWS || dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) || (double)m * (double)cols * (double)k < 1e8) return 0;
+	if (backward ? m < 128 || (cols < 768 && m * k > 8u << 20) : m < 512 || cols < 768) return 0;
+	return ((m + cols) * ((k + 7) & ~7ull) * 2 + 255) & ~255ull;
 }
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
-	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated); // the packed matrices last
+	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
 }
 // Where the pieces of a backward pass lie in the workspace (bytes); from the sizes alone, so that ngp_*_workspace_size and the launch agree.
 struct DensePlan { uint64_t grad, bias, partial, partial_x, pack, bytes; uint32_t rows_per_block, row_blocks; };
@@ -425,7 +429,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
 	const uint64_t dx = dense_split_bytes(m, k, n, problems, 1), dw = dense_split_bytes(n, k, m, 1, problems);
 	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
-	p.partial_x = p.partial + up(dw); p.pack = p.partial_x + up(dx); p.bytes = p.pack + dense_pack_bytes(m, n, k, gated); // (the two products run side by side)
+	p.partial_x = p.partial + up(dw); p.pack = p.partial_x + up(dx); p.bytes = p.pack + dense_pack_bytes(m, n, k, gated, true); // (the two products run side by side)
 	return p;
 }
 void launch_dense_forward_half(hipStream_t s, const DenseArgs& d);

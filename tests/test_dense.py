@@ -496,6 +496,14 @@ def test_odd_lines(hip, type_, m, n, k, gated, pad, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated", [(1500, 504, 200, False), (700, 400, 512, True), (150, 1001, 1000, False)])
+@pytest.mark.parametrize("pad,shift", [((5, 0, 5), 0), ((0, 3, 2), 0), ((2, 6, 4), 2), ((2, 4, 1), 1), ((0, 0, 0), 3)])
+def test_whole_pieces_at_any_stride(hip, m, n, k, gated, pad, shift):
+    """lines of whole 16-byte pieces that begin at even or odd elements, inputs and weights apart"""
+    run_layer(Layer(A.TYPE_BFLOAT16, A.ACT_GELU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 16, 17, 32])
 @pytest.mark.parametrize("n,k", [(8, 8192), (5, 4099), (40, 12290), (1000, 33), (2500, 129), (130, 1025)])
 @pytest.mark.parametrize("gated,pad,shift", [(False, (0, 0, 0), 0), (True, (0, 0, 0), 0), (False, (1, 0, 1), 1), (True, (2, 4, 0), 2)])
@@ -683,7 +691,7 @@ def test_workspace_sizes():
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("m,n,k", [(2, 16, 8192), (100, 64, 9000), (333, 777, 501)])
+@pytest.mark.parametrize("m,n,k", [(2, 16, 8192), (100, 64, 9000), (1000, 1000, 1003)])
 def test_forward_workspace(gated, m, n, k):
     """sums that blocks share and padded operands need room in the forward pass too: its size is asked for and held to"""
     L = lib()
