@@ -941,19 +941,26 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
 // one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
 struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; };
-template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
-	const uint32_t cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 256 + cx * 8, pc = up8(g.cols);
+template <bool GATED, uint32_t COLS> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
+	constexpr uint32_t CX = COLS / 8, RY = 256 / CX;
+	const uint32_t cx = threadIdx.x % CX, ry = threadIdx.x / CX, c = blockIdx.x * COLS + cx * 8, pc = up8(g.cols);
 	const uint32_t end = min(g.rows, (blockIdx.y + 1) * g.rows_per_block);
 	const bool odd = ((uintptr_t)g.dy | (uintptr_t)g.pre[0] | (uintptr_t)g.pre[1] | g.ld_dy * 2 | g.ld_pre * 2) & 3;
 	float sum[GATED ? 2 : 1][8] = {};
 	if (c < g.cols) {
-		const int n = (int)min(8u, g.cols - c);
-		for (uint32_t r = blockIdx.y * g.rows_per_block + ry; r < end; r += 8) {
-			auto load = [&](const T* p) -> T8 { return n < 8 ? load8(p, n) : odd ? load8_odd(p) : load8(p); };
-			const T8 dy = load(g.dy + (uint64_t)r * g.ld_dy + c);
+		// lines of 8 elements and more: the last chunk is read from 8 in front of the end and moved down
+		const bool ragged = g.cols & 7 && g.cols >= 8;
+		const int n = ragged ? 8 : (int)min(8u, g.cols - c), at = ragged ? min((int)c, (int)g.cols - 8) : (int)c;
+		for (uint32_t r = blockIdx.y * g.rows_per_block + ry; r < end; r += RY) {
+			auto load = [&](const T* p) -> T8 {
+				if (n < 8) return load8(p, n);
+				const T8 v = odd ? load8_odd(p) : load8(p);
+				return ragged ? shift8(v, c, g.cols) : v;
+			};
+			const T8 dy = load(g.dy + (uint64_t)r * g.ld_dy + at);
 			T8 z{}, u{}, o, o2;
-			if (g.pre[0]) z = load(g.pre[0] + (uint64_t)r * g.ld_pre + c);
-			if (GATED) u = load(g.pre[1] + (uint64_t)r * g.ld_pre + c);
+			if (g.pre[0]) z = load(g.pre[0] + (uint64_t)r * g.ld_pre + at);
+			if (GATED) u = load(g.pre[1] + (uint64_t)r * g.ld_pre + at);
 			float v[8], v2[8];
 			output_grad8<GATED>(g.act, dy, z, u, v, v2);
 			EACH { sum[0][e] += v[e]; o[e] = (T)v[e]; if (GATED) { sum[GATED ? 1 : 0][e] += v2[e]; o2[e] = (T)v2[e]; } }
@@ -964,20 +971,22 @@ template <bool GATED> __global__ __launch_bounds__(256) void k_output_grad(GradA
 		}
 	}
 	if (!g.bias_partial && !g.dbias[0] && !g.dbias[1]) return;
-	__shared__ float red[8][256 + 8];
+	__shared__ float red[RY][COLS + 8];
 #pragma unroll
 	for (int k = 0; k < (GATED ? 2 : 1); ++k) {
 		__syncthreads();
 #pragma unroll
 		for (int e = 0; e < 8; ++e) red[ry][cx * 8 + e] = sum[k][e];
 		__syncthreads();
-		float s = 0.f;
+		for (uint32_t i = threadIdx.x; i < COLS; i += 256) {
+			float s = 0.f;
 #pragma unroll
-		for (int y = 0; y < 8; ++y) s += red[y][threadIdx.x];
-		const uint32_t col = blockIdx.x * 256 + threadIdx.x;
-		if (col >= g.cols) continue;
-		if (g.bias_partial) g.bias_partial[((uint64_t)blockIdx.y * (GATED ? 2 : 1) + k) * g.cols + col] = s;
-		else if (g.dbias[k]) g.dbias[k][col] = (T)s; // (one block of rows: the sum is whole)
+			for (uint32_t y = 0; y < RY; ++y) s += red[y][i];
+			const uint32_t col = blockIdx.x * COLS + i;
+			if (col >= g.cols) break;
+			if (g.bias_partial) g.bias_partial[((uint64_t)blockIdx.y * (GATED ? 2 : 1) + k) * g.cols + col] = s;
+			else if (g.dbias[k]) g.dbias[k][col] = (T)s; // (one block of rows: the sum is whole)
+		}
 	}
 }
 // dbias = sum of the blocks' column sums: a block takes 16 columns, 16 threads each, then adds the shares up in their order
@@ -1217,9 +1226,11 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems; a.rows_per_block = p.rows_per_block;
 		if (p.row_blocks > 1) a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr; else for (int k = 0; k < 2; ++k) a.dbias[k] = (T*)d.dbias[k];
 		if (a.out) { G = a.out; ldg = a.ld_out; }
-		const dim3 grid(div_up(d.n, 256), std::max(1u, p.row_blocks)); // (no samples: the bias's gradient is zero)
+		const uint32_t cols = dense_grad_cols(d.m, d.n);
+		const dim3 grid(div_up(d.n, cols), std::max(1u, p.row_blocks)); // (no samples: the bias's gradient is zero)
 		if (d.n) {
-			if (d.gated) hipLaunchKernelGGL(k_output_grad<true>, grid, dim3(256), 0, s, a); else hipLaunchKernelGGL(k_output_grad<false>, grid, dim3(256), 0, s, a);
+			if (cols > 256) { if (d.gated) hipLaunchKernelGGL((k_output_grad<true, 1024>), grid, dim3(256), 0, s, a); else hipLaunchKernelGGL((k_output_grad<false, 1024>), grid, dim3(256), 0, s, a); }
+			else { if (d.gated) hipLaunchKernelGGL((k_output_grad<true, 256>), grid, dim3(256), 0, s, a); else hipLaunchKernelGGL((k_output_grad<false, 256>), grid, dim3(256), 0, s, a); }
 		}
 		b.partial = a.bias_partial;
 	}

@@ -364,12 +364,15 @@ inline DenseFewRows dense_few_rows(uint32_t cols, uint32_t steps) {
 	return f;
 }
 // A product of rows x cols with `steps * segments` terms a sum, `parts` times over: tile size and the number of pieces every sum is cut into (each a block of its own, joined by a
-// second launch).  From sizes alone.
+// second launch; the forward pass splits small tiles only).  From sizes alone.
 struct DenseSplit { uint32_t splits; bool large; };
 inline DenseSplit dense_split(uint64_t rows, uint64_t cols, uint64_t steps, uint32_t segments, uint32_t parts) {
 	auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
 	const uint64_t chunks = up(steps, 64) * segments, large = up(rows, 256) * up(cols, 256) * parts, small = up(rows, 128) * up(cols, 128) * parts;
 	if (large >= 200) return {1, true};
+	// a long sum fills the card with large tiles too, a piece of 40 chunks and more each, unless they hang over the edges (776 x 504, sums of 200000: 192 against 262 us by small tiles,
+	// 1928 x 240 of 90752: 118 / 148, 2048 x 1024 of 32768: 126 / 136; with 16 chunks, 256 x 1024 of 65536: 62 / 49; 264 x 264 of 100000: 56 / 42)
+	if (large && large <= 128 && chunks * large >= 40 * 256 && large * 16 <= small * 5 && 256 / large * large >= 200) return {(uint32_t)up(chunks, up(chunks, 256 / large)), true};
 	// time of a piece: a chunk of a 128 x 128 tile 0.35 us (two blocks a compute unit, 512 at a time); partial sums: written and read at 4 TB/s, a second launch 3 us
 	const double bytes = (double)rows * (double)((cols + 7) & ~7ull) * parts * 8;
 	double best = 1e30; uint32_t pick = 1;
@@ -404,6 +407,9 @@ inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gat
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
 	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
 }
+// Columns of a block of k_output_grad: longer runs of a line for matrices beyond the caches (gated, 90765 x 1928: 367 us, 450 in runs of 256), more blocks for the others (gated, 777 x 1333:
+// 12 us, 6.8 in runs of 256)
+inline uint32_t dense_grad_cols(uint64_t m, uint64_t n) { return n > 512 && m * n >= 1u << 24 ? 1024 : 256; }
 // Where the pieces of a backward pass lie in the workspace (bytes); from the sizes alone, so that ngp_*_workspace_size and the launch agree.
 struct DensePlan { uint64_t grad, bias, partial, partial_x, pack, bytes; uint32_t rows_per_block, row_blocks; };
 inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
@@ -423,7 +429,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 		return p;
 	}
 	// elementwise pass: about 1024 blocks of whole groups of 8 rows
-	const uint64_t col_blocks = ((uint64_t)n + 255) / 256, want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
+	const uint64_t col_blocks = ((uint64_t)n + dense_grad_cols(m, n) - 1) / dense_grad_cols(m, n), want = col_blocks < 1024 ? 1024 / (col_blocks ? col_blocks : 1) : 1;
 	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
 	if (!p.rows_per_block) p.rows_per_block = 8;
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
