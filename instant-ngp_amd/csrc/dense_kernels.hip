@@ -1118,15 +1118,14 @@ template <bool A_T, bool B_T, int EPI> void launch_tiles(hipStream_t s, const Ge
 	} else if (n <= 256) hipLaunchKernelGGL((k_gemm_async<128, A_T, B_T, EPI, 4>), dim3(n), dim3(256), 0, s, g);
 	else hipLaunchKernelGGL((k_gemm_async<128, A_T, B_T, EPI, 2>), dim3(n), dim3(256), 0, s, g);
 }
-// tile size and splits of a product; true: large tiles
-bool set_split(GemmArgs& g, uint32_t parts, float* partial) {
-	const DenseSplit d = dense_split(g.rows, g.cols, g.steps, g.segments, parts);
+// splits of a product; true: large tiles
+bool set_split(GemmArgs& g, const DenseSplit& d, float* partial) {
 	g.splits = d.splits; g.partial = partial;
 	g.chunks_per_split = div_up(div_up(g.steps, 64) * g.segments, g.splits);
 	return d.large;
 }
 template <int EPI> void launch_forward(hipStream_t s, GemmArgs& g, bool wholes, float* partial) {
-	const bool large = set_split(g, EPI == EPI_GATED ? 2 : 1, partial) && wholes;
+	const bool large = set_split(g, dense_split(g.rows, g.cols, g.steps, 1, EPI == EPI_GATED ? 2 : 1), partial) && wholes;
 	if (g.splits > 1) {
 		launch_tiles<true, true, EPI == EPI_GATED ? EPI_PARTIAL2 : EPI_PARTIAL>(s, g, wholes, false);
 		launch_join<EPI>(s, g);
@@ -1247,12 +1246,12 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	if (want_x) {
 		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = o.w[0]; x.b[1] = o.w[1]; x.ldb = o.ld_w;
 		x.rows = d.m; x.cols = d.k; x.steps = d.n; x.problems = 1; x.c[0] = (T*)d.dx; x.ldc = d.dx_stride;
-		large_x = set_split(x, 1, (float*)(ws + p.partial_x)) && whole_x;
+		large_x = set_split(x, dense_split(d.m, d.k, d.n, problems, 1), (float*)(ws + p.partial_x)) && whole_x;
 	}
 	if (want_w) {
 		w.a = G; w.lda = ldg; w.a_problem = up8(d.n); w.problems = problems; w.b[0] = w.b[1] = o.x; w.ldb = o.ld_x;
 		w.rows = d.n; w.cols = d.k; w.steps = d.m; w.segments = 1; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
-		large_w = set_split(w, problems, (float*)(ws + p.partial)) && whole_w;
+		large_w = set_split(w, dense_split_dw(d.m, d.n, d.k, problems), (float*)(ws + p.partial)) && whole_w;
 	}
 	if (want_x && want_w && !large_x && !large_w && whole_x == whole_w) {
 		const uint32_t bx = tiles<EPI_STORE>(x, 128), bw = tiles<EPI_STORE>(w, 128);

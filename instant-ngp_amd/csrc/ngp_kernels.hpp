@@ -382,9 +382,24 @@ inline DenseSplit dense_split(uint64_t rows, uint64_t cols, uint64_t steps, uint
 	}
 	return {(uint32_t)(chunks ? up(chunks, up(chunks, pick)) : 1), false};
 }
-inline uint64_t dense_split_bytes(uint64_t rows, uint64_t cols, uint64_t steps, uint32_t segments, uint32_t parts) {
-	const DenseSplit d = dense_split(rows, cols, steps, segments, parts);
-	return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0;
+inline uint64_t dense_split_bytes(const DenseSplit& d, uint64_t rows, uint64_t cols, uint32_t parts) { return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0; }
+// dW beside dX in one launch: a chunk takes 1 us of a block with a neighbour on its compute unit, 0.55 us without (0.5 with the whole of its LDS), so the launch takes the average over the card or its longest block alone;
+// then the partial sums (m 5003, n 777, k 1000: 3 pieces 40 us, 4 pieces, the best for dW alone, 46 us; 2000, 1000, 1000: 2 pieces 30 us, 4 34 us).  The same whether dX is wanted or not.
+inline DenseSplit dense_split_dw(uint64_t m, uint64_t n, uint64_t k, uint32_t problems) {
+	auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+	DenseSplit w = dense_split(n, k, m, 1, problems);
+	const DenseSplit x = dense_split(m, k, n, problems, 1);
+	if (w.large || x.large || !m || !n) return w;
+	const uint64_t chunks = up(m, 64), of_x = up(n, 64) * problems, bw = up(n, 128) * up(k, 128) * problems;
+	const uint64_t bx = up(m, 128) * up(k, 128) * x.splits, longest_x = up(of_x, x.splits);
+	const double average = (double)(up(m, 128) * up(k, 128) * of_x + bw * chunks) / 512.0, bytes = (double)n * (double)((k + 7) & ~7ull) * problems * 8;
+	double best = 1e30; uint64_t pick = 1;
+	for (uint64_t p = 1; p <= 256 && (p == 1 || (chunks >= 2 * p && bytes / 2 * p <= 256e6)); ++p) {
+		const double t = std::fmax(average, (bx + bw * p <= 256 ? 0.5 : 0.55) * (double)std::max(longest_x, up(chunks, p))) + (p > 1 ? bytes * p / 4e6 : 0.0);
+		if (t < best * 0.98) { best = t; pick = p; }
+	}
+	w.splits = (uint32_t)up(chunks, up(chunks, pick));
+	return w;
 }
 // Layers that k_narrow_forward / k_narrow_backward take: all weights in one compute unit.  Every block stages them, which pays from few samples on where they are small (64 x 64, 2048
 // samples: forward + backward 5.0 + 11 us against 8.9 + 20 us by tiles) and from many where they fill LDS (256 x 256, 65536 samples: 28 + 58 us against 30 + 66 us).
@@ -405,7 +420,7 @@ inline uint64_t dense_pack_bytes(uint64_t m, uint64_t n, uint64_t k, bool gated,
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
-	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(m, n, k, 1, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
+	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(dense_split(m, n, k, 1, parts), m, n, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
 }
 // Columns of a block of k_output_grad: longer runs of a line for matrices beyond the caches (gated, 90765 x 1928: 367 us, 450 in runs of 256), more blocks for the others (gated, 777 x 1333:
 // 12 us, 6.8 in runs of 256)
@@ -433,7 +448,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
 	if (!p.rows_per_block) p.rows_per_block = 8;
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
-	const uint64_t dx = dense_split_bytes(m, k, n, problems, 1), dw = dense_split_bytes(n, k, m, 1, problems);
+	const uint64_t dx = dense_split_bytes(dense_split(m, k, n, problems, 1), m, k, 1), dw = dense_split_bytes(dense_split_dw(m, n, k, problems), n, k, problems);
 	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
 	p.partial_x = p.partial + up(dw); p.pack = p.partial_x + up(dx); p.bytes = p.pack + dense_pack_bytes(m, n, k, gated, true); // (the two products run side by side)
 	return p;
