@@ -1180,8 +1180,9 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	g.rows = d.m; g.cols = d.n; g.steps = d.k; g.segments = 1; g.problems = 1;
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
-	// Outputs that the 256 MB of the last cache would not hold beside the inputs go past the caches (262144 x 256 from 64 inputs: 95 -> 78 us; 8192 x 4096 x 2 from 4096: 237 -> 224 us); smaller
-	// ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us)
+	// Outputs that the 256 MB of the last cache would not hold beside the inputs go past the caches (262144 x 256 from 64 inputs: 95 -> 78 us; 8192 x 4096 x 2 from 4096: 237 -> 230 us; 72112 x 1894
+	// from 1224: 405 -> 365 us); smaller ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us).  Narrow layers' only in whole cache lines: they are written in
+	// halves, which the caches join (262144 x 256 x 2 at a stride of 264: 194 us, past the caches 246 us).
 	g.streamed = (uint64_t)d.m * d.n * 2 * (1 + (d.pre[0] != nullptr) + (d.pre[1] != nullptr)) >= 128ull << 20;
 	float* partial = (float*)d.workspace;
 	if (d.m <= FEW_ROWS && d.k) {
@@ -1190,6 +1191,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		return;
 	}
 	if (dense_narrow(d.m, d.n, d.k, d.gated)) {
+		g.streamed &= (((uintptr_t)d.y | (uintptr_t)d.pre[0] | (uintptr_t)d.pre[1] | d.y_stride * 2 | (d.pre[0] || d.pre[1] ? d.pre_stride * 2 : 0)) & 127) == 0;
 		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
 		return;
 	}
@@ -1204,13 +1206,15 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const uint32_t problems = d.gated ? 2 : 1;
 	char* ws = (char*)d.workspace;
 	const bool bias = d.dbias[0] || d.dbias[1];
-	const bool identity = !d.gated && d.act == NGP_ACT_NONE; // G is dY as it stands
+	const bool none = !d.gated && d.act == NGP_ACT_NONE;
+	// G is dY as it stands, unless the products are worth a padded copy (14724 x 7414 from 2072 inputs: 1525 us without, 1198 us; 2000 x 1001 from 1000: 39.7, 29.8 us)
+	const bool identity = none && (whole(d.dy, d.dy_stride, d.n) || (double)d.m * d.n * d.k < 1e8);
 	const bool products = d.dx || d.dw[0] || d.dw[1];
 	if ((products || bias) && dense_narrow(d.m, d.n, d.k, d.gated)) {
 		NarrowArgs a{};
 		a.rows = d.m; a.n = d.n; a.k = d.k; a.act = d.act; a.x = (const T*)d.x; a.ld_x = d.x_stride; a.ld_w = d.w_stride; a.ld_pre = d.pre_stride; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride;
 		for (int i = 0; i < 2; ++i) { a.w[i] = (const T*)d.w[i]; a.pre[i] = (const T*)d.pre[i]; }
-		if (identity) { a.pre[0] = a.dy; a.ld_pre = a.ld_dy; } // (read, not used)
+		if (none) { a.pre[0] = a.dy; a.ld_pre = a.ld_dy; } // (read, not used)
 		if (!d.dw[0]) { a.x = a.dy; a.ld_x = 0; }              // (dW is not wanted: something to read in the place of X, where nothing looks)
 		a.dx = (T*)d.dx; a.ld_dx = d.dx_stride; a.partial = d.dw[0] ? (float*)(ws + p.partial) : nullptr; a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr;
 		if (d.gated) launch_narrow_backward<true>(s, a, p.row_blocks); else launch_narrow_backward<false>(s, a, p.row_blocks);
@@ -1225,7 +1229,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	if ((!identity && products) || bias) {
 		GradArgs a{};
 		a.rows = d.m; a.cols = d.n; a.act = d.act; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride; a.pre[0] = (const T*)d.pre[0]; a.pre[1] = (const T*)d.pre[1]; a.ld_pre = d.pre_stride;
-		if (identity) a.pre[0] = nullptr;
+		if (none) a.pre[0] = nullptr;
 		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems; a.rows_per_block = p.rows_per_block;
 		if (p.row_blocks > 1) a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr; else for (int k = 0; k < 2; ++k) a.dbias[k] = (T*)d.dbias[k];
 		if (a.out) { G = a.out; ldg = a.ld_out; }
