@@ -140,16 +140,15 @@ __device__ inline void act_value8(int act, float z[8]) { // (one branch for 8 va
 		default: break;
 	}
 }
-// f(activation, streamed or not, as constants): one branch for a whole loop, whose code then stays small (an epilogue with the branch in every row ran 2.5 times longer, waiting for instructions)
-template <typename F> __device__ inline void with_act(int act, bool streamed, F&& f) {
-	auto g = [&](auto act_c) { if (streamed) f(act_c, std::true_type()); else f(act_c, std::false_type()); };
+// f(activation as a constant): one branch for a whole loop, whose code then stays small (an epilogue with the branch in every row ran 2.5 times longer, waiting for instructions)
+template <typename F> __device__ inline void with_act(int act, F&& f) {
 	switch (act) {
-		case NGP_ACT_RELU: g(std::integral_constant<int, NGP_ACT_RELU>()); break;
-		case NGP_ACT_LOGISTIC: g(std::integral_constant<int, NGP_ACT_LOGISTIC>()); break;
-		case NGP_ACT_EXPONENTIAL: g(std::integral_constant<int, NGP_ACT_EXPONENTIAL>()); break;
-		case NGP_ACT_SILU: g(std::integral_constant<int, NGP_ACT_SILU>()); break;
-		case NGP_ACT_GELU: g(std::integral_constant<int, NGP_ACT_GELU>()); break;
-		default: g(std::integral_constant<int, NGP_ACT_NONE>()); break;
+		case NGP_ACT_RELU: f(std::integral_constant<int, NGP_ACT_RELU>()); break;
+		case NGP_ACT_LOGISTIC: f(std::integral_constant<int, NGP_ACT_LOGISTIC>()); break;
+		case NGP_ACT_EXPONENTIAL: f(std::integral_constant<int, NGP_ACT_EXPONENTIAL>()); break;
+		case NGP_ACT_SILU: f(std::integral_constant<int, NGP_ACT_SILU>()); break;
+		case NGP_ACT_GELU: f(std::integral_constant<int, NGP_ACT_GELU>()); break;
+		default: f(std::integral_constant<int, NGP_ACT_NONE>()); break;
 	}
 }
 // G of 8 outputs: dY act'(Z); gated: dY Zu act'(Zg) and dY act(Zg).  Zeros give zeros.
@@ -211,6 +210,15 @@ struct GemmArgs {
 };
 __host__ __device__ inline uint32_t up8(uint32_t v) { return (v + 7) & ~7u; }
 
+// 8 sums (gated: z of the gate, u of the up projection) to pre-activations and outputs
+template <int EPI> __device__ inline void outputs8(float z[8], float u[8], const T8& bias0, const T8& bias1, const T8* residual, int act, T8& pre0, T8& pre1, T8& o) {
+	EACH { z[e] += (float)bias0[e]; pre0[e] = (T)z[e]; }
+	act_value8(act, z);
+	if constexpr (EPI == EPI_LINEAR) {
+		if (residual) { EACH z[e] += (float)(*residual)[e]; }
+		EACH o[e] = (T)z[e];
+	} else EACH { u[e] += (float)bias1[e]; pre1[e] = (T)u[e]; o[e] = (T)(z[e] * u[e]); }
+}
 // What becomes of 8 consecutive sums of row r from column c on (gated: z of the gate, u of the up projection), n <= 8 of them inside C.  Biases and the residual come as values: a caller
 // with several rows loads them ahead.
 template <int EPI> __device__ inline void epilogue8(const GemmArgs& g, uint32_t problem, uint32_t split, uint32_t r, uint32_t c, int n, float z[8], float u[8], const T8& bias0, const T8& bias1, const T8& residual, int act, bool streamed = false) {
@@ -597,7 +605,7 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS
 				}
 			}
 		};
-		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) with_act(g.act, g.streamed, rows); else rows(std::integral_constant<int, NGP_ACT_NONE>(), std::false_type());
+		if constexpr (EPI == EPI_LINEAR || EPI == EPI_GATED) { if (g.streamed) with_act(g.act, [&](auto act_c) { rows(act_c, std::true_type()); }); else with_act(g.act, [&](auto act_c) { rows(act_c, std::false_type()); }); } else rows(std::integral_constant<int, NGP_ACT_NONE>(), std::false_type());
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	}
 }
@@ -688,7 +696,7 @@ template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_fe
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
-template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
+template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int OF = GATED ? NF / 2 : NF; // fragments of outputs
 	__shared__ __attribute__((aligned(16))) T w[NF * KS * 512];
@@ -738,7 +746,41 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 			for (int f = 0; f < NF; ++f) acc[f] = mfma(*(const T8*)(w + ((f * KS + k) * 64 + lane) * 8), x[k], acc[f]);
 		if (slab + stride < slabs) load_x(slab + stride);
 		const uint32_t r = slab * 16 + li;
-		if (r < g.rows) with_act(g.act, g.streamed, [&](auto act_c, auto streamed_c) {
+		if constexpr (EXCHANGE) with_act(g.act, [&](auto act_c) {
+			// EXCHANGE: two pieces of 32 columns at a time, neighbouring lanes (samples) swap one chunk each, so that a store writes 128 bytes of a line (262144 x 256 from 64 inputs 79 -> 58 us;
+			// 65536 samples 14 -> 16 us, where a wavefront goes through this code once: not there)
+			constexpr int PAIR = 2;
+#pragma unroll
+			for (int p = 0; p < OF / 2; p += PAIR) {
+				T8 pre0[PAIR], pre1[PAIR], o[PAIR];
+#pragma unroll
+				for (int h = 0; h < PAIR; ++h) {
+					const uint32_t c = (p + h) * 32 + gq * 8;
+					const int n = (int)min(8u, g.cols > c ? g.cols - c : 0u), q = p + h;
+					float z[8], u[8];
+					EACH { z[e] = acc[2 * q + e / 4][e & 3]; u[e] = GATED ? acc[(GATED ? OF : 0) + 2 * q + e / 4][e & 3] : 0.f; }
+					const T8 residual = r < g.rows ? residual8<EPI>(g, r, c, n) : T8{};
+					outputs8<EPI>(z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), g.residual ? &residual : nullptr, decltype(act_c)::value, pre0[h], pre1[h], o[h]);
+				}
+				auto store = [&](T* to, uint64_t ld, const T8 (&v)[PAIR]) {
+					const bool second = li & 1;
+					const uint32_t c = (p + second) * 32 + gq * 8, r0 = r & ~1u;
+					const int n = (int)min(8u, g.cols > c ? g.cols - c : 0u);
+					const T8 given = second ? v[0] : v[1], kept = second ? v[1] : v[0];
+					uint32_t d[4];
+					__builtin_memcpy(d, &given, 16);
+#pragma unroll
+					for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_mov_dpp(d[i], 0xb1 /* lanes 1, 0, 3, 2 of four */, 0xf, 0xf, true);
+					T8 got;
+					__builtin_memcpy(&got, d, 16);
+					if (n > 0 && r0 < g.rows) store8(to + (uint64_t)r0 * ld + c, second ? got : kept, n, g.streamed);
+					if (n > 0 && r0 + 1 < g.rows) store8(to + (uint64_t)(r0 + 1) * ld + c, second ? kept : got, n, g.streamed);
+				};
+				if (g.pre[0]) store(g.pre[0], g.ld_pre, pre0);
+				if (GATED && g.pre[1]) store(g.pre[1], g.ld_pre, pre1);
+				store(g.c[0], g.ldc, o);
+			}
+		}); else if (r < g.rows) with_act(g.act, [&](auto act_c) {
 #pragma unroll
 			for (int p = 0; p < OF / 2; ++p) {
 				const uint32_t c = p * 32 + gq * 8;
@@ -746,7 +788,7 @@ template <int NF, int KS, int EPI> __global__ __launch_bounds__(512, NF * KS <= 
 				const int n = (int)min(8u, g.cols - c);
 				float z[8], u[8];
 				EACH { z[e] = acc[2 * p + e / 4][e & 3]; u[e] = GATED ? acc[(GATED ? OF : 0) + 2 * p + e / 4][e & 3] : 0.f; }
-				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), decltype(act_c)::value, decltype(streamed_c)::value);
+				epilogue8<EPI>(g, 0, 0, r, c, n, z, u, bias8<EPI>(g, 0, c, n), bias8<EPI>(g, 1, c, n), residual8<EPI>(g, r, c, n), decltype(act_c)::value);
 			}
 		});
 	}
@@ -1152,14 +1194,15 @@ template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, floa
 	} else if (odd) hipLaunchKernelGGL((k_few_rows<MT, EPI, true>), grid, dim3(512), 0, s, g, f.slices, per);
 	else hipLaunchKernelGGL((k_few_rows<MT, EPI, false>), grid, dim3(512), 0, s, g, f.slices, per);
 }
-template <int NF, int EPI> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
-	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI>), dim3(blocks), dim3(512), 0, s, g);
-	else if (g.steps <= 128) hipLaunchKernelGGL((k_narrow_forward<NF, 4, EPI>), dim3(blocks), dim3(512), 0, s, g);
-	else hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI>), dim3(blocks), dim3(512), 0, s, g);
+template <int NF, int EPI, bool EXCHANGE> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
+	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
+	else if (g.steps <= 128) hipLaunchKernelGGL((k_narrow_forward<NF, 4, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
+	else hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
 }
-template <int EPI> void launch_narrow_forward(hipStream_t s, const GemmArgs& g) {
+template <int EPI, bool EXCHANGE> void launch_narrow_forward(hipStream_t s, const GemmArgs& g) {
 	const uint32_t cols = g.cols * (EPI == EPI_GATED ? 2 : 1), blocks = std::min(div_up(g.rows, 128), 512u);
-	if (cols <= 64) launch_narrow_forward_n<4, EPI>(s, g, blocks); else if (cols <= 128) launch_narrow_forward_n<8, EPI>(s, g, blocks); else launch_narrow_forward_n<16, EPI>(s, g, std::min(blocks, g.steps > 128 ? 256u : 512u));
+	if (cols <= 64) { if constexpr (!(EXCHANGE && EPI == EPI_GATED)) launch_narrow_forward_n<4, EPI, EXCHANGE>(s, g, blocks); } // (up to 32 gated outputs: one piece, nothing to exchange)
+	else if (cols <= 128) launch_narrow_forward_n<8, EPI, EXCHANGE>(s, g, blocks); else launch_narrow_forward_n<16, EPI, EXCHANGE>(s, g, std::min(blocks, g.steps > 128 ? 256u : 512u));
 }
 template <int NF, int KF, bool GATED> void launch_narrow_backward_nk(hipStream_t s, const NarrowArgs& a, uint32_t blocks) {
 	hipLaunchKernelGGL((k_narrow_backward<NF, KF, GATED>), dim3(blocks), dim3(512), 0, s, a);
@@ -1181,9 +1224,9 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
 	// Outputs that the 256 MB of the last cache would not hold beside the inputs go past the caches (262144 x 256 from 64 inputs: 95 -> 78 us; 8192 x 4096 x 2 from 4096: 237 -> 230 us; 72112 x 1894
-	// from 1224: 405 -> 365 us); smaller ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us).  Narrow layers' only in whole cache lines: they are written in
-	// halves, which the caches join (262144 x 256 x 2 at a stride of 264: 194 us, past the caches 246 us).
-	g.streamed = (uint64_t)d.m * d.n * 2 * (1 + (d.pre[0] != nullptr) + (d.pre[1] != nullptr)) >= 128ull << 20;
+	// from 1224: 405 -> 365 us); smaller ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us).  Narrow layers' only in whole cache lines,
+	// which the caches need not join (262144 x 256 x 2 at a stride of 264: 165 us, 246 us past the caches).
+	const bool large = g.streamed = (uint64_t)d.m * d.n * 2 * (1 + (d.pre[0] != nullptr) + (d.pre[1] != nullptr)) >= 128ull << 20;
 	float* partial = (float*)d.workspace;
 	if (d.m <= FEW_ROWS && d.k) {
 		if (d.m <= 16) { if (d.gated) launch_few_rows<1, EPI_GATED>(s, g, partial); else launch_few_rows<1, EPI_LINEAR>(s, g, partial); }
@@ -1192,7 +1235,8 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	}
 	if (dense_narrow(d.m, d.n, d.k, d.gated)) {
 		g.streamed &= (((uintptr_t)d.y | (uintptr_t)d.pre[0] | (uintptr_t)d.pre[1] | d.y_stride * 2 | (d.pre[0] || d.pre[1] ? d.pre_stride * 2 : 0)) & 127) == 0;
-		if (d.gated) launch_narrow_forward<EPI_GATED>(s, g); else launch_narrow_forward<EPI_LINEAR>(s, g);
+		if (large && d.n > 32) { if (d.gated) launch_narrow_forward<EPI_GATED, true>(s, g); else launch_narrow_forward<EPI_LINEAR, true>(s, g); }
+		else { if (d.gated) launch_narrow_forward<EPI_GATED, false>(s, g); else launch_narrow_forward<EPI_LINEAR, false>(s, g); }
 		return;
 	}
 	const uint64_t room = dense_pack_bytes(d.m, d.n, d.k, d.gated, false);

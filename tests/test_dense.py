@@ -496,6 +496,21 @@ def test_odd_lines(hip, type_, m, n, k, gated, pad, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(700, 777, 400), (300, 1001, 1000), (5000, 131, 264)])
+@pytest.mark.parametrize("pad,shift", [((0, 0, 0), 0), ((0, 0, 5), 1)])
+@pytest.mark.parametrize("want", ["xwb", "xw"])
+def test_no_activation(hip, m, n, k, pad, shift, want):
+    """the gradient of the outputs is that of the pre-activations, in whole pieces or not"""
+    run_layer(Layer(A.TYPE_HALF, A.ACT_NONE, m, n, k, pad=pad, shift=shift), want=want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated,pad", [(263001, 256, 16, False, 0), (131073, 256, 24, False, 8), (263001, 128, 16, True, 0), (17001, 4099, 40, False, 0)])
+def test_outputs_beyond_the_caches(hip, m, n, k, gated, pad):
+    run_layer(Layer(A.TYPE_HALF, A.ACT_RELU, m, n, k, gated=gated, residual=not gated, pad=(0, 0, pad)), backward=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,gated", [(1500, 504, 200, False), (700, 400, 512, True), (150, 1001, 1000, False)])
 @pytest.mark.parametrize("pad,shift", [((5, 0, 5), 0), ((0, 3, 2), 0), ((2, 6, 4), 2), ((2, 4, 1), 1), ((0, 0, 0), 3)])
 def test_whole_pieces_at_any_stride(hip, m, n, k, gated, pad, shift):
