@@ -2683,7 +2683,7 @@ static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t
 	for (size_t i = 0; i < nb; ++i) {
 		if (!b[i].p) continue;
 		REQUIRE(b[i].stride >= b[i].width, w + ": stride of " + b[i].name + " too small");
-		REQUIRE(b[i].stride < (1ull << 40), w + ": stride of " + b[i].name + " too large");
+		REQUIRE(b[i].stride < (1ull << 40) && b[i].stride <= (1ull << 47) / std::max<uint64_t>(1, b[i].rows), w + ": stride of " + b[i].name + " too large"); // (ranges fit 64 bits, and no address space holds more)
 		REQUIRE(((uintptr_t)b[i].p & 1) == 0, w + ": " + b[i].name + " is not aligned to its elements");
 	}
 	for (size_t i = 0; i < nb; ++i) if (b[i].written)
@@ -2697,7 +2697,7 @@ static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t
 extern "C" uint64_t ngp_linear_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, false).bytes : dense_forward_bytes(m, n, k, false); }
 extern "C" uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backward) { return backward ? dense_plan(m, n, k, true).bytes : dense_forward_bytes(m, n, k, true); }
 extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride, const void* bias,
-		const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+		const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) try {
 	const uint64_t need = dense_forward_bytes(m, n, k, false);
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w, n, k, w_stride, "w", false}, {bias, 1, n, n, "bias", false}, {residual, m, n, residual_stride, "residual", false},
 		{y, m, n, y_stride, "y", true}, {pre, m, n, pre_stride, "pre", true}, {workspace, 1, need, need, "workspace", true, 1}};
@@ -2711,9 +2711,9 @@ extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32
 	if (type == NGP_TYPE_HALF) launch_dense_forward_half((hipStream_t)stream, d); else launch_dense_forward_bf16((hipStream_t)stream, d);
 	HIPCHK(hipGetLastError());
 	return 0;
-}
+} catch (const std::bad_alloc&) { return fail("out of host memory"); }
 extern "C" int ngp_gated_forward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up, uint64_t w_stride,
-		const void* bias_gate, const void* bias_up, void* y, uint64_t y_stride, void* gate_pre, void* up_pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) {
+		const void* bias_gate, const void* bias_up, void* y, uint64_t y_stride, void* gate_pre, void* up_pre, uint64_t pre_stride, void* workspace, uint64_t workspace_size) try {
 	const uint64_t need = dense_forward_bytes(m, n, k, true);
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w_gate, n, k, w_stride, "w_gate", false}, {w_up, n, k, w_stride, "w_up", false}, {bias_gate, 1, n, n, "bias_gate", false},
 		{bias_up, 1, n, n, "bias_up", false}, {y, m, n, y_stride, "y", true}, {gate_pre, m, n, pre_stride, "gate_pre", true}, {up_pre, m, n, pre_stride, "up_pre", true}, {workspace, 1, need, need, "workspace", true, 1}};
@@ -2727,9 +2727,9 @@ extern "C" int ngp_gated_forward(void* stream, int type, int activation, uint32_
 	if (type == NGP_TYPE_HALF) launch_dense_forward_half((hipStream_t)stream, d); else launch_dense_forward_bf16((hipStream_t)stream, d);
 	HIPCHK(hipGetLastError());
 	return 0;
-}
+} catch (const std::bad_alloc&) { return fail("out of host memory"); }
 extern "C" int ngp_linear_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
-		const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias, void* workspace, uint64_t workspace_size) {
+		const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias, void* workspace, uint64_t workspace_size) try {
 	if (activation == NGP_ACT_NONE) pre = nullptr; // not read
 	const uint64_t need = dense_plan(m, n, k, false).bytes;
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w, n, k, w_stride, "w", false}, {pre, m, n, pre_stride, "pre", false}, {dy, m, n, dy_stride, "dy", false},
@@ -2746,10 +2746,10 @@ extern "C" int ngp_linear_backward(void* stream, int type, int activation, uint3
 	if (type == NGP_TYPE_HALF) launch_dense_backward_half((hipStream_t)stream, d); else launch_dense_backward_bf16((hipStream_t)stream, d);
 	HIPCHK(hipGetLastError());
 	return 0;
-}
+} catch (const std::bad_alloc&) { return fail("out of host memory"); }
 extern "C" int ngp_gated_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w_gate, const void* w_up, uint64_t w_stride,
 		const void* gate_pre, const void* up_pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw_gate, void* dw_up, uint64_t dw_stride,
-		void* dbias_gate, void* dbias_up, void* workspace, uint64_t workspace_size) {
+		void* dbias_gate, void* dbias_up, void* workspace, uint64_t workspace_size) try {
 	const uint64_t need = dense_plan(m, n, k, true).bytes;
 	const DenseBuffer b[] = {{x, m, k, x_stride, "x", false}, {w_gate, n, k, w_stride, "w_gate", false}, {w_up, n, k, w_stride, "w_up", false}, {gate_pre, m, n, pre_stride, "gate_pre", false},
 		{up_pre, m, n, pre_stride, "up_pre", false}, {dy, m, n, dy_stride, "dy", false}, {dx, m, k, dx_stride, "dx", true}, {dw_gate, n, k, dw_stride, "dw_gate", true}, {dw_up, n, k, dw_stride, "dw_up", true},
@@ -2767,7 +2767,7 @@ extern "C" int ngp_gated_backward(void* stream, int type, int activation, uint32
 	if (type == NGP_TYPE_HALF) launch_dense_backward_half((hipStream_t)stream, d); else launch_dense_backward_bf16((hipStream_t)stream, d);
 	HIPCHK(hipGetLastError());
 	return 0;
-}
+} catch (const std::bad_alloc&) { return fail("out of host memory"); }
 
 extern "C" uint64_t ngp_gradient_workspace_size(void) { return CLIP_SLOTS * sizeof(double); }
 static int gradient_norm(const char* what, void* stream, uint32_t n, const ngp_gradient* t, float loss_scale, bool clip, float max_norm, float* norm, void* workspace, uint64_t workspace_size) try {

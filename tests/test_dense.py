@@ -638,7 +638,7 @@ def forward_args(**kw):
     (dict(xs=31), "stride of x"), (dict(ws=31), "stride of w"), (dict(ys=15), "stride of y"), (dict(ps=15), "stride of pre"), (dict(residual=0x60000, rs=15), "stride of residual"),
     (dict(x=0x10001), "aligned"), (dict(bias=0x30001), "aligned"), (dict(y=0x10010), "y overlaps x"), (dict(y=0x20000), "y overlaps w"), (dict(pre=0x40000), "overlaps"), (dict(y=0x30000), "y overlaps bias"),
     (dict(residual=0x40010, rs=16), "y overlaps residual"), (dict(residual=0x40000, rs=17), "y overlaps residual"), (dict(m=1 << 31), "at most"), (dict(n=(1 << 24) + 1, ys=1 << 25, ps=1 << 25), "at most"),
-    (dict(m=0x7fffffff, n=1 << 20, ys=1 << 20, pre=None), "tiles"), (dict(xs=1 << 50), "too large")])
+    (dict(m=0x7fffffff, n=1 << 20, ys=1 << 20, pre=None), "tiles"), (dict(xs=1 << 50), "too large"), (dict(m=1 << 20, xs=1 << 39), "stride of x too large"), (dict(m=1 << 20, ys=1 << 30), "stride of y too large")])
 def test_forward_refusals(kw, what):
     L = lib()
     assert L.ngp_linear_forward(*forward_args(**kw)) != 0
