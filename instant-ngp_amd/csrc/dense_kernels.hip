@@ -261,6 +261,8 @@ __device__ inline Work work_of(const GemmArgs& g, uint32_t index, uint32_t n, ui
 	const uint32_t which = t / tiles, in = t - which * tiles, strip = 8 * col_tiles, s = in / strip, k = in - s * strip, rows = min(8u, row_tiles - s * 8);
 	return {s * 8 + k % rows, k / rows, which % g.problems, which / g.problems};
 }
+// Staged through registers: operands at odd addresses, or with lines that are no whole 16-byte pieces, any size from 1.  The way to LDS bounds it (4096 x 4096 of 1000 inputs at an odd
+// stride: 70 us, 480 TFLOP/s, half the rate of async_tile's), at 128 x 128 so that two blocks a compute unit cover each other's barriers.
 // C tile BR x BC by WR x WC wavefronts; each owns (BR / WR) x (BC / WC) as 16 x 16 fragments (matrix instruction 16x16x32, C^T: a lane holds one row of C and 4 columns
 // of each fragment).  EPI_GATED: the tile's columns are BC / 2 gate outputs and the same BC / 2 up outputs, every wavefront owns both of its columns.
 template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI> __device__ inline void any_tile(const GemmArgs& g, T* lds_a, T* lds_b, uint32_t index, uint32_t count) {
@@ -387,6 +389,8 @@ __global__ __launch_bounds__(256) void k_products(GemmArgs x, GemmArgs w, uint32
 // unit has one block to itself (144 KB), 2 where it has two.  The matrix instructions run through a unit in two halves of 32 steps; A fragments
 // come in three ahead of their use, the next half's B fragments into a second set of registers.  4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128
 // products is what LDS can deliver beside the incoming units (96 of the 128 bytes a clock; with 8 wavefronts of 128 x 64 it would be all of them).
+// Bound by the matrix instructions: 8192 x 8192 x 8192 765 us, 1440 TFLOP/s, what a library product reaches here; a unit of a 256 x 256 tile takes 1.46 us, and a tile's outputs some 9 us
+// more that nothing hides (8192 x 4096 of 4096 with gelu, residual and Z 230 us, 1195 TFLOP/s; gated, 4096 x 4096 x 2 of 1024 with both Z 74 us, 930).
 constexpr int AK = 64, A_RING = 4;
 typedef int i4v __attribute__((ext_vector_type(4)));
 template <int EXTENT, bool T_CONTIG, int WAVES> struct Async {
@@ -624,6 +628,7 @@ template <int UNITS> __global__ __launch_bounds__(256, UNITS > 2 ? 1 : 2) void k
 // ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
 // straight from memory to registers as the matrix instruction's fragments, U loads on the way at a time; the samples (MT x 16 rows, the last one repeated where there are fewer)
 // come out of the caches.  `slices` wavefronts share the sum and add up in LDS, in their order; where there are few outputs blocks share it too (EPI_PARTIAL*).
+// 1 x 2048 -> 2 x 8192 (67 MB) 13.2 us, 5.1 TB/s; 1 x 2048 -> 2048 (8.4 MB) 5.8 us, of which a launch is most.
 template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4;
@@ -695,6 +700,7 @@ template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_fe
 // ---- narrow layers (up to 256 inputs and outputs) over many samples: bound by reading and writing the samples once.
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
+// 262144 x 256 of 256 (268 MB) 67 us, 4.0 TB/s; 65521 x 256 and Z of 63 (75 MB) 23 us, of which staging the weights and filling the card take about 6.
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
 template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
 	constexpr bool GATED = GATED_TILE<EPI>;
@@ -795,7 +801,7 @@ template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(5
 }
 // Backward in one pass: a block takes 32 samples at a time (the next 32 on their way), forms G = dY * act'(Z) and lays it and X into LDS; its 8 wavefronts multiply G with the weights
 // (in LDS too) to dX, and G^T with X into their parts of dW, which stay in registers to the end: one partial sum a block, joined by a second launch.  Every sample's
-// dY, Z, X is read once, dX written once.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
+// dY, Z, X is read once, dX written once.  262144 samples, 256 x 256 (537 MB): 145 us, 3.7 TB/s, bound by LDS (both products read G from it) as much as by memory.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
 struct NarrowArgs {
 	uint32_t rows, n, k; int act; const T* x; uint64_t ld_x; const T* w[2]; uint64_t ld_w; const T* pre[2]; uint64_t ld_pre; const T* dy; uint64_t ld_dy; T* dx; uint64_t ld_dx;
 	float* partial; float* bias_partial;
@@ -981,7 +987,8 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
-// one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound.  32 x 8 threads: 256 columns x 8 rows at a time.
+// one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound (gated,
+// 8192 x 8192, 671 MB: 116 us, 5.8 TB/s; 90765 x 1928, 1.75 GB: 367 us, 4.8 TB/s).  256 threads: COLS / 8 along a line, the rest on further lines.
 struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; };
 template <bool GATED, uint32_t COLS> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
 	constexpr uint32_t CX = COLS / 8, RY = 256 / CX;
@@ -1094,7 +1101,7 @@ template <int EPI> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs
 	__shared__ float shared[(EPI == EPI_GATED ? 2 : 1) * 256 * 9];
 	join_any<EPI>(g, groups, blockIdx.x, shared);
 }
-// what is left of a backward pass in one launch: dX's and dW's split sums, the bias's
+// what is left of a backward pass in one launch: dX's and dW's split sums, the bias's (256 x 256 of 256 pieces, 67 MB: 11.5 us, 5.8 TB/s, out of the last cache)
 __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32_t blocks_x, GemmArgs w, int groups_w, uint32_t blocks_w, BiasArgs bias) {
 	__shared__ float shared[256 * 9];
 	uint32_t b = blockIdx.x;
@@ -1106,7 +1113,7 @@ __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 3) == 0 && (ld & 1) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces, each from a dword on; a tile's offsets fit 31 bits
-// X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else; memory bound
+// X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else; memory bound (200000 x 500: 64 us, 6.3 TB/s)
 struct PackArgs { const T* from[3]; T* to[3]; uint64_t ld[3]; uint32_t lines[3]; uint32_t width; };
 __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
 	const uint32_t cc = up8(g.width) / 8;
