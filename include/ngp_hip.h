@@ -292,7 +292,7 @@ int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint3
                        const void* bias, const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride,
                        void* workspace, uint64_t workspace_size);
 /* G = dY * act'(Z);  dX = G W;  dW = G^T X;  dbias = column sums of G (each NULL = not wanted; overwritten).  The residual's gradient is dY itself.  `pre` is not read with
- * NGP_ACT_NONE.  G is rounded to `type` between the two products. */
+ * NGP_ACT_NONE.  G is rounded to `type` between the two products (small sets of G, whose roundings would not average out, keep what the rounding loses). */
 int ngp_linear_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
                         const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias,
                         void* workspace, uint64_t workspace_size);

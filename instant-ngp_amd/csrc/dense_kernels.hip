@@ -200,7 +200,7 @@ enum { EPI_LINEAR, EPI_GATED, EPI_STORE /* as it is; partial sums where they are
 struct GemmArgs {
 	const T* a; const T* b[2]; uint64_t lda, ldb;
 	uint32_t rows, cols, steps;      // C is rows x cols; the sum runs over `segments` pieces of `steps`
-	uint32_t segments; uint64_t a_segment; // dX of a gated layer: A's second piece is a_segment elements further along t, B's is b[1]
+	uint32_t segments; uint64_t a_segment; // A's next piece is a_segment elements further (dX of a gated layer, second terms of G), B's is the other one of b
 	uint64_t a_problem; uint32_t problems; // dW of a gated layer: two products with the same B (A a_problem elements further)
 	uint32_t splits, chunks_per_split;     // the sum is split over blocks: partial sums to `partial`
 	T* c[2]; uint64_t ldc;
@@ -322,7 +322,7 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI> __device_
 		left = (int)min((uint32_t)TK, g.steps - t0);
 		load_operand(TA{}, std::integral_constant<bool, A_T>(), ra, std::integral_constant<int, NA>(), [&](uint32_t&) { return a + seg * g.a_segment; }, g.lda, r0, g.rows, t0, left);
 		load_operand(TB{}, std::integral_constant<bool, B_T>(), rb, std::integral_constant<int, NB>(), [&](uint32_t& line) -> const T* {
-			if (!B_T) return g.b[seg];
+			if (!B_T) return g.b[seg & 1];
 			const uint32_t which = GATED_TILE<EPI> && line >= OUT; // (gated: the tile's second half is the up projection's)
 			line -= which * OUT;
 			return which ? g.b[1] : g.b[0];
@@ -461,7 +461,7 @@ template <int BR, int BC, int WR, int WC, bool A_T, bool B_T, int EPI, int UNITS
 	LA la; LB lb;
 	la.setup(lane, wave, g.lda, 0); lb.setup(lane, wave, g.ldb, which * OUT);
 	auto start_a = [&](uint32_t seg) -> const T* { return uniform(g.a + problem * g.a_problem + seg * g.a_segment + (A_T ? (uint64_t)r0 * g.lda : (uint64_t)r0)); };
-	auto start_b = [&](uint32_t seg) -> const T* { return uniform(B_T ? g.b[which] + (uint64_t)c0 * g.ldb : g.b[seg] + c0); };
+	auto start_b = [&](uint32_t seg) -> const T* { return uniform(B_T ? g.b[which] + (uint64_t)c0 * g.ldb : g.b[seg & 1] + c0); };
 	Cursor<A_T, UNITS_A, LA::BYTES> ca; Cursor<B_T, UNITS_B, LB::BYTES> cb;
 	{
 		const uint32_t seg = units_per_segment ? t_begin / units_per_segment : 0, t0 = (t_begin - seg * units_per_segment) * AK, steps8 = up8(g.steps);
@@ -986,10 +986,10 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 }
 
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
-// instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own), and its column sums (in 32 bits,
+// instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own; small sets in two terms), and its column sums (in 32 bits,
 // one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound (gated,
 // 8192 x 8192, 671 MB: 116 us, 5.8 TB/s; 90765 x 1928, 1.75 GB: 367 us, 4.8 TB/s).  256 threads: COLS / 8 along a line, the rest on further lines.
-struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; };
+struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; bool two_terms; };
 template <bool GATED, uint32_t COLS> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
 	constexpr uint32_t CX = COLS / 8, RY = 256 / CX;
 	const uint32_t cx = threadIdx.x % CX, ry = threadIdx.x / CX, c = blockIdx.x * COLS + cx * 8, pc = up8(g.cols);
@@ -1016,6 +1016,12 @@ template <bool GATED, uint32_t COLS> __global__ __launch_bounds__(256) void k_ou
 			if (g.out) {
 				*(T8*)(g.out + (uint64_t)r * g.ld_out + c) = o;
 				if (GATED) *(T8*)(g.out + (uint64_t)r * g.ld_out + pc + c) = o2;
+				if (g.two_terms) { // what the rounding lost, behind all rounded ones
+					auto lost = [](float exact, T rounded) -> T { const float d = exact - (float)rounded; return (T)(fabsf(d) < __builtin_inff() ? d : 0.f); }; // (nothing of what is not finite)
+					EACH { o[e] = lost(v[e], o[e]); if (GATED) o2[e] = lost(v2[e], o2[e]); }
+					*(T8*)(g.out + (uint64_t)r * g.ld_out + (GATED ? 2 : 1) * pc + c) = o;
+					if (GATED) *(T8*)(g.out + (uint64_t)r * g.ld_out + 3 * pc + c) = o2;
+				}
 			}
 		}
 	}
@@ -1261,7 +1267,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	// G is dY as it stands, unless the products are worth a padded copy (14724 x 7414 from 2072 inputs: 1525 us without, 1198 us; 2000 x 1001 from 1000: 39.7, 29.8 us)
 	const bool identity = none && (whole(d.dy, d.dy_stride, d.n) || (double)d.m * d.n * d.k < 1e8);
 	const bool products = d.dx || d.dw[0] || d.dw[1];
-	if ((products || bias) && dense_narrow(d.m, d.n, d.k, d.gated)) {
+	if ((products || bias) && dense_narrow_backward(d.m, d.n, d.k, d.gated)) {
 		NarrowArgs a{};
 		a.rows = d.m; a.n = d.n; a.k = d.k; a.act = d.act; a.x = (const T*)d.x; a.ld_x = d.x_stride; a.ld_w = d.w_stride; a.ld_pre = d.pre_stride; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride;
 		for (int i = 0; i < 2; ++i) { a.w[i] = (const T*)d.w[i]; a.pre[i] = (const T*)d.pre[i]; }
@@ -1275,13 +1281,14 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 		launch_finish(s, nullptr, a.partial ? &w : nullptr, b);
 		return;
 	}
+	const uint32_t terms = !none && dense_two_terms(d.m, d.n, d.k) ? 2 : 1;
 	const T* G = (const T*)d.dy; uint64_t ldg = d.dy_stride;
 	BiasArgs b{nullptr, p.row_blocks, d.n, problems, {(T*)d.dbias[0], (T*)d.dbias[1]}};
 	if ((!identity && products) || bias) {
 		GradArgs a{};
 		a.rows = d.m; a.cols = d.n; a.act = d.act; a.dy = (const T*)d.dy; a.ld_dy = d.dy_stride; a.pre[0] = (const T*)d.pre[0]; a.pre[1] = (const T*)d.pre[1]; a.ld_pre = d.pre_stride;
 		if (none) a.pre[0] = nullptr;
-		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems; a.rows_per_block = p.rows_per_block;
+		a.out = products && !identity ? (T*)(ws + p.grad) : nullptr; a.ld_out = (uint64_t)up8(d.n) * problems * terms; a.two_terms = terms == 2; a.rows_per_block = p.rows_per_block;
 		if (p.row_blocks > 1) a.bias_partial = bias ? (float*)(ws + p.bias) : nullptr; else for (int k = 0; k < 2; ++k) a.dbias[k] = (T*)d.dbias[k];
 		if (a.out) { G = a.out; ldg = a.ld_out; }
 		const uint32_t cols = dense_grad_cols(d.m, d.n);
@@ -1299,14 +1306,14 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack, p.bytes > p.pack) : Operands{};
 	const bool whole_x = g_whole && o.whole_w, whole_w = g_whole && o.whole_x;
 	if (want_x) {
-		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems; x.b[0] = o.w[0]; x.b[1] = o.w[1]; x.ldb = o.ld_w;
+		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems * terms; x.b[0] = o.w[0]; x.b[1] = d.gated ? o.w[1] : o.w[0]; x.ldb = o.ld_w;
 		x.rows = d.m; x.cols = d.k; x.steps = d.n; x.problems = 1; x.c[0] = (T*)d.dx; x.ldc = d.dx_stride;
-		large_x = set_split(x, dense_split(d.m, d.k, d.n, problems, 1), (float*)(ws + p.partial_x)) && whole_x;
+		large_x = set_split(x, dense_split(d.m, d.k, d.n, problems * terms, 1), (float*)(ws + p.partial_x)) && whole_x;
 	}
 	if (want_w) {
 		w.a = G; w.lda = ldg; w.a_problem = up8(d.n); w.problems = problems; w.b[0] = w.b[1] = o.x; w.ldb = o.ld_x;
-		w.rows = d.n; w.cols = d.k; w.steps = d.m; w.segments = 1; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
-		large_w = set_split(w, dense_split_dw(d.m, d.n, d.k, problems), (float*)(ws + p.partial)) && whole_w;
+		w.rows = d.n; w.cols = d.k; w.steps = d.m; w.segments = terms; w.a_segment = (uint64_t)up8(d.n) * problems; w.c[0] = (T*)d.dw[0]; w.c[1] = (T*)d.dw[1]; w.ldc = d.dw_stride;
+		large_w = set_split(w, dense_split_dw(d.m, d.n, d.k, problems, terms), (float*)(ws + p.partial)) && whole_w;
 	}
 	if (want_x && want_w && !large_x && !large_w && whole_x == whole_w) {
 		const uint32_t bx = tiles<EPI_STORE>(x, 128), bw = tiles<EPI_STORE>(w, 128);

@@ -385,12 +385,12 @@ inline DenseSplit dense_split(uint64_t rows, uint64_t cols, uint64_t steps, uint
 inline uint64_t dense_split_bytes(const DenseSplit& d, uint64_t rows, uint64_t cols, uint32_t parts) { return d.splits > 1 ? (uint64_t)d.splits * parts * rows * ((cols + 7) & ~7ull) * 4 : 0; }
 // dW beside dX in one launch: a chunk takes 1 us of a block with a neighbour on its compute unit, 0.55 us without (0.5 with the whole of its LDS), so the launch takes the average over the card or its longest block alone;
 // then the partial sums (m 5003, n 777, k 1000: 3 pieces 40 us, 4 pieces, the best for dW alone, 46 us; 2000, 1000, 1000: 2 pieces 30 us, 4 34 us).  The same whether dX is wanted or not.
-inline DenseSplit dense_split_dw(uint64_t m, uint64_t n, uint64_t k, uint32_t problems) {
+inline DenseSplit dense_split_dw(uint64_t m, uint64_t n, uint64_t k, uint32_t problems, uint32_t terms) {
 	auto up = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
-	DenseSplit w = dense_split(n, k, m, 1, problems);
-	const DenseSplit x = dense_split(m, k, n, problems, 1);
+	DenseSplit w = dense_split(n, k, m, terms, problems);
+	const DenseSplit x = dense_split(m, k, n, problems * terms, 1);
 	if (w.large || x.large || !m || !n) return w;
-	const uint64_t chunks = up(m, 64), of_x = up(n, 64) * problems, bw = up(n, 128) * up(k, 128) * problems;
+	const uint64_t chunks = up(m, 64) * terms, of_x = up(n, 64) * problems * terms, bw = up(n, 128) * up(k, 128) * problems;
 	const uint64_t bx = up(m, 128) * up(k, 128) * x.splits, longest_x = up(of_x, x.splits);
 	const double average = (double)(up(m, 128) * up(k, 128) * of_x + bw * chunks) / 512.0, bytes = (double)n * (double)((k + 7) & ~7ull) * problems * 8;
 	double best = 1e30; uint64_t pick = 1;
@@ -407,6 +407,10 @@ inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint64_t cols = (gated ? 2 * (uint64_t)n : n);
 	return n >= 8 && k >= 8 && k <= 256 && cols <= 256 && m > FEW_ROWS && (cols * k <= 32768 || m >= 32768);
 }
+// The gradients of the pre-activations are rounded to 16 bits between the products.  In small sets of them a few decide (exponential, 160 x 16: some 15), whose roundings do not average out:
+// there each goes as two terms, the rounded value and what it lost, and the products read both (their sums are short; weights up to 8 MB stay in the caches).
+inline bool dense_two_terms(uint64_t m, uint64_t n, uint64_t k) { return m * n <= 32768 && n * k <= 4u << 20; }
+inline bool dense_narrow_backward(uint32_t m, uint32_t n, uint32_t k, bool gated) { return dense_narrow(m, n, k, gated) && !dense_two_terms(m, n, k); }
 // Tiles take operands of whole 16-byte pieces at even elements straight to LDS; others are copied into the workspace first (lines padded) where that pays, else staged through registers.
 // us copied / staged, 1004 inputs: forward 65536 samples 400 outputs 125 / 117, 1032 outputs 229 / 264; 4096 samples 2056 outputs 45 / 53; 200 samples, 2004 inputs, 2056 outputs 23.5 / 19.7.
 // Backward 65536 samples 400 outputs 290 / 268, 1032 outputs 512 / 592; 4096 samples (8 MB of inputs, which caches hold) 400 outputs 34 / 38; 64 samples, 4100 inputs, 520 outputs 21 / 21.
@@ -432,7 +436,7 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t problems = gated ? 2 : 1;
 	const uint64_t n8 = ((uint64_t)n + 7) & ~7ull;
 	auto up = [](uint64_t v) { return (v + 255) & ~255ull; };
-	if (dense_narrow(m, n, k, gated)) { // one pass, a partial sum a block
+	if (dense_narrow_backward(m, n, k, gated)) { // one pass, a partial sum a block
 		const uint32_t slabs = (m + 31) / 32;
 		// two blocks a compute unit where their registers and LDS allow it; fewer where the partial sums (written and read at 4 TB/s) would cost more than the blocks save (2 us a slab)
 		const uint32_t most = (gated ? 2 * n : n) <= 128 && k <= 128 ? 512 : 256;
@@ -448,8 +452,13 @@ inline DensePlan dense_plan(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	p.rows_per_block = (uint32_t)((((uint64_t)m + want - 1) / want + 7) & ~7ull);
 	if (!p.rows_per_block) p.rows_per_block = 8;
 	p.row_blocks = (uint32_t)(((uint64_t)m + p.rows_per_block - 1) / p.rows_per_block);
-	const uint64_t dx = dense_split_bytes(dense_split(m, k, n, problems, 1), m, k, 1), dw = dense_split_bytes(dense_split_dw(m, n, k, problems), n, k, problems);
-	p.grad = 0; p.bias = up(p.grad + problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
+	uint64_t dx = 0, dw = 0;
+	const uint32_t terms = dense_two_terms(m, n, k) ? 2 : 1;
+	for (uint32_t t = 1; t <= terms; ++t) { // (one term without an activation: nothing is rounded)
+		const uint64_t x = dense_split_bytes(dense_split(m, k, n, problems * t, 1), m, k, 1), w = dense_split_bytes(dense_split_dw(m, n, k, problems, t), n, k, problems);
+		dx = x > dx ? x : dx; dw = w > dw ? w : dw;
+	}
+	p.grad = 0; p.bias = up(p.grad + (uint64_t)terms * problems * m * n8 * 2); p.partial = up(p.bias + (uint64_t)problems * p.row_blocks * n * 4);
 	p.partial_x = p.partial + up(dw); p.pack = p.partial_x + up(dx); p.bytes = p.pack + dense_pack_bytes(m, n, k, gated, true); // (the two products run side by side)
 	return p;
 }

@@ -147,14 +147,14 @@ class Layer:
             bound = da + 2 * F32 * (a.abs() + want.abs())
         self.close(y[1], want, bound, "y")
 
-    def check_backward(self, pre, dx, dw, db):
+    def check_backward(self, pre, dx, dw, db, g_rounding=None):
         z = [p[1].double() for p in pre]
         value, slope = act64(self.act, z[0])
         dy = self.dy[1].double()
         g = [dy * slope * z[1], dy * value] if self.gated else [dy * slope]
         # G: a few 32-bit operations (slopes of magnitude <= 1.2 or the value itself), then one rounding
         fine = [64 * F32 * (v.abs() + (dy * (z[1] if self.gated else 1)).abs()) if i == 0 else 64 * F32 * (v.abs() + dy.abs()) for i, v in enumerate(g)]
-        off = [U[self.type] * v.abs() + f + TINY[self.type] for v, f in zip(g, fine)]
+        off = [(U[self.type] if g_rounding is None else g_rounding) * v.abs() + f + TINY[self.type] for v, f in zip(g, fine)]
         x, w = self.x[1].double(), [v[1].double() for v in self.w]
         if dx is not None:
             want = sum(a @ b for a, b in zip(g, w))
@@ -493,6 +493,19 @@ def test_block_of_layers_with_the_trainer(hip):
 def test_odd_lines(hip, type_, m, n, k, gated, pad, shift):
     """many products over lines that are no whole 16-byte pieces"""
     run_layer(Layer(type_, A.ACT_SILU, m, n, k, gated=gated, residual=not gated, pad=pad, shift=shift))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [A.TYPE_HALF, A.TYPE_BFLOAT16])
+@pytest.mark.parametrize("m,n,k,gated,act", [(160, 16, 3223, False, A.ACT_EXPONENTIAL), (1, 40, 500, True, A.ACT_SILU), (100, 16, 64, False, A.ACT_EXPONENTIAL), (37, 200, 136, True, A.ACT_GELU),
+                                             (4, 8192, 500, False, A.ACT_RELU), (2000, 16, 8, False, A.ACT_LOGISTIC), (300, 33, 1000, True, A.ACT_NONE), (2, 129, 63, False, A.ACT_NONE)])
+def test_few_gradients(hip, type_, m, n, k, gated, act):
+    """small sets of gradients of the pre-activations are not rounded between the products: a value and what it lost leave u^2 of it (the lost part is rounded), and 2 u^2 covers that"""
+    layer = Layer(type_, act, m, n, k, gated=gated, x_scale=0.5)
+    layer.residual64 = None
+    _, pre = layer.forward()
+    layer.check_backward(pre, *layer.backward(pre), g_rounding=2 * U[type_] ** 2)
+    layer.untouched()
 
 
 @pytest.mark.gpu
