@@ -3,7 +3,8 @@
 // Memory bound: one pass reads every gradient for the sum, one reads and writes it (nothing is written in place where c = 1): 400 M bfloat16 in 300 tensors 515 us, 4.7 TB/s over the
 // three; 12.2 M half in 9 tensors 18 us; 7168 elements 8.5 us, a launch.  The tensors' table travels in the
 // kernel arguments (no upload that a captured graph would have to keep alive), TABLE tensors a launch.  Every block owns a contiguous range of the tensors' chunks;
-// the second pass takes launches and ranges backwards, so that it begins with what the first one left in the caches.  Up to SMALL elements one block does it all, in one launch.  Sums are double, in a fixed order: the result
+// the second pass takes launches and ranges backwards, so that it begins with what the first one left in the caches.  Up to SMALL elements in
+// FEW tensors one block does it all, in one launch: 4096 elements in 2 tensors 4.2 us against 9.7, in 8 tensors, one after the other, 8.0 against 7.4, in 100 48 against 11.  Sums are double, in a fixed order: the result
 // does not depend on timing, and squares of any bfloat16 / float fit.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
@@ -13,7 +14,7 @@
 
 namespace ngp {
 namespace {
-constexpr uint32_t TABLE = 112, CHUNK = 8192, THREADS = 256, SMALL = 65536;
+constexpr uint32_t TABLE = 112, CHUNK = 8192, THREADS = 256, SMALL = 65536, FEW = 8;
 struct ClipTable { const void* grad[TABLE]; void* clipped[TABLE]; uint64_t size[TABLE]; uint32_t first[TABLE + 1]; uint8_t type[TABLE]; uint32_t n; };
 struct Range { uint32_t begin, end; };
 __device__ inline Range block_range(uint32_t chunks) {
@@ -156,7 +157,7 @@ void launch_gradient_norm(hipStream_t s, uint32_t n, const ngp_gradient* tensors
 	uint32_t i = 0;
 	if (total <= SMALL) {
 		table(i, t);
-		if (i >= n) { hipLaunchKernelGGL(k_clip_small, dim3(1), dim3(1024), 0, s, t, loss_scale, max_norm, norm); return; }
+		if (i >= n && t.n <= FEW) { hipLaunchKernelGGL(k_clip_small, dim3(1), dim3(1024), 0, s, t, loss_scale, max_norm, norm); return; }
 		i = 0;
 	}
 	std::vector<uint32_t> starts; // first tensor of each table

@@ -77,6 +77,16 @@ def test_clip(hip, spec, in_place, over, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [7, 8, 9, 111, 112, 113])
+def test_many_small_tensors(hip, n):
+    """either side of the number that one block takes, with empty ones between"""
+    s = Set([(40 + 3 * i, (H, F, B)[i % 3]) for i in range(n)] + [(0, F)] * 5, True, seed=n)
+    max_norm = float(np.float32(s.exact(2.0) * 0.5))
+    s.clip(2.0, max_norm)
+    s.check(2.0, max_norm)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("spec", [[(65535, H)], [(65536, B)], [(65537, F)], [(0, H)] * 111 + [(70000, B), (0, F), (9, H)], [(100, H)] * 112 + [(60000, F)], [(8192, B)] * 112 + [(0, F)] * 130 + [(8193, H)] * 3, [(0, F)] * 300 + [(5, H)]])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_tables(hip, spec, in_place):
