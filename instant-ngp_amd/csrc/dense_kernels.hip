@@ -1210,7 +1210,8 @@ template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, floa
 template <int NF, int EPI, bool EXCHANGE> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
 	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
 	else if (g.steps <= 128) hipLaunchKernelGGL((k_narrow_forward<NF, 4, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
-	else hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
+	else if (NF > 4 || g.steps <= 256) hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
+	else if constexpr (NF == 4) hipLaunchKernelGGL((k_narrow_forward<NF, 16, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
 }
 template <int EPI, bool EXCHANGE> void launch_narrow_forward(hipStream_t s, const GemmArgs& g) {
 	const uint32_t cols = g.cols * (EPI == EPI_GATED ? 2 : 1), blocks = std::min(div_up(g.rows, 128), 512u);
@@ -1246,7 +1247,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		else { if (d.gated) launch_few_rows<2, EPI_GATED>(s, g, partial); else launch_few_rows<2, EPI_LINEAR>(s, g, partial); }
 		return;
 	}
-	if (dense_narrow(d.m, d.n, d.k, d.gated)) {
+	if (dense_narrow_forward(d.m, d.n, d.k, d.gated)) {
 		g.streamed &= (((uintptr_t)d.y | (uintptr_t)d.pre[0] | (uintptr_t)d.pre[1] | d.y_stride * 2 | (d.pre[0] || d.pre[1] ? d.pre_stride * 2 : 0)) & 127) == 0;
 		if (large && d.n > 32) { if (d.gated) launch_narrow_forward<EPI_GATED, true>(s, g); else launch_narrow_forward<EPI_LINEAR, true>(s, g); }
 		else { if (d.gated) launch_narrow_forward<EPI_GATED, false>(s, g); else launch_narrow_forward<EPI_LINEAR, false>(s, g); }

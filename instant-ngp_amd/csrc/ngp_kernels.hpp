@@ -407,6 +407,12 @@ inline bool dense_narrow(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint64_t cols = (gated ? 2 * (uint64_t)n : n);
 	return n >= 8 && k >= 8 && k <= 256 && cols <= 256 && m > FEW_ROWS && (cols * k <= 32768 || m >= 32768);
 }
+// The forward pass alone takes twice the inputs for up to 64 outputs (149211 samples, 352 inputs, 2 x 32 outputs: 62 us by tiles, 35 us; 262144, 512, 64: 105, 65 us; 65536, 300, 128 the other
+// way: 17, 26 us), in even numbers (262144, 511, 32: 87, 122 us).
+inline bool dense_narrow_forward(uint32_t m, uint32_t n, uint32_t k, bool gated) {
+	const uint64_t cols = (gated ? 2 * (uint64_t)n : n);
+	return dense_narrow(m, n, k, gated) || (n >= 8 && k > 256 && k <= 512 && !(k & 1) && cols <= 64 && m > FEW_ROWS);
+}
 // The gradients of the pre-activations are rounded to 16 bits between the products.  In small sets of them a few decide (exponential, 160 x 16: some 15), whose roundings do not average out:
 // there each goes as two terms, the rounded value and what it lost, and the products read both (their sums are short; weights up to 8 MB stay in the caches).
 inline bool dense_two_terms(uint64_t m, uint64_t n, uint64_t k) { return m * n <= 32768 && n * k <= 4u << 20; }
@@ -417,14 +423,14 @@ inline bool dense_narrow_backward(uint32_t m, uint32_t n, uint32_t k, bool gated
 // The backward pass has the room whatever k is, for lines at odd strides (2000 samples 1000 x 1000: 70 staged); a forward pass only where lines are no whole pieces by themselves.
 inline uint64_t dense_pack_bytes(uint64_t m, uint64_t n, uint64_t k, bool gated, bool backward) {
 	const uint64_t cols = (gated ? 2 : 1) * n;
-	if ((!backward && !(k & 7)) || k < 8 || m <= FEW_ROWS || dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) || (double)m * (double)cols * (double)k < 1e8) return 0;
+	if ((!backward && !(k & 7)) || k < 8 || m <= FEW_ROWS || (backward ? dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) : dense_narrow_forward((uint32_t)m, (uint32_t)n, (uint32_t)k, gated)) || (double)m * (double)cols * (double)k < 1e8) return 0;
 	if (backward ? m < 128 || (cols < 768 && m * k > 8u << 20) : m < 512 || cols < 768) return 0;
 	return ((m + cols) * ((k + 7) & ~7ull) * 2 + 255) & ~255ull;
 }
 inline uint64_t dense_forward_bytes(uint32_t m, uint32_t n, uint32_t k, bool gated) {
 	const uint32_t parts = gated ? 2 : 1, splits = dense_few_rows(n, k).splits;
 	const uint64_t few = splits > 1 ? (uint64_t)splits * parts * m * (((uint64_t)n + 7) & ~7ull) * 4 : 0;
-	return (((m <= FEW_ROWS ? few : dense_narrow(m, n, k, gated) ? 0 : dense_split_bytes(dense_split(m, n, k, 1, parts), m, n, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
+	return (((m <= FEW_ROWS ? few : dense_narrow_forward(m, n, k, gated) ? 0 : dense_split_bytes(dense_split(m, n, k, 1, parts), m, n, parts)) + 255) & ~255ull) + dense_pack_bytes(m, n, k, gated, false); // the packed matrices last
 }
 // Columns of a block of k_output_grad: longer runs of a line for matrices beyond the caches (gated, 90765 x 1928: 367 us, 450 in runs of 256), more blocks for the others (gated, 777 x 1333:
 // 12 us, 6.8 in runs of 256)

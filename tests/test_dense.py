@@ -518,7 +518,7 @@ def test_no_activation(hip, m, n, k, pad, shift, want):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k,gated,pad", [(263001, 256, 16, False, 0), (131073, 256, 24, False, 8), (263001, 128, 16, True, 0), (17001, 4099, 40, False, 0)])
+@pytest.mark.parametrize("m,n,k,gated,pad", [(263001, 256, 16, False, 0), (131073, 256, 24, False, 8), (263001, 128, 16, True, 0), (17001, 4099, 40, False, 0), (600001, 120, 400, False, 8)])
 def test_outputs_beyond_the_caches(hip, m, n, k, gated, pad):
     run_layer(Layer(A.TYPE_HALF, A.ACT_RELU, m, n, k, gated=gated, residual=not gated, pad=(0, 0, pad)), backward=False)
 
@@ -543,7 +543,8 @@ def test_few_samples(hip, m, n, k, gated, pad, shift):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k,gated", [(33, 8, 8, False), (33, 16, 256, False), (50, 9, 11, True), (1000, 100, 200, False), (777, 64, 40, True), (2049, 128, 129, False), (515, 33, 250, True), (4100, 250, 100, False),
-                                         (33001, 256, 256, False), (32768, 255, 250, False), (33333, 128, 255, True), (40000, 200, 256, False)])
+                                         (33001, 256, 256, False), (32768, 255, 250, False), (33333, 128, 255, True), (40000, 200, 256, False), (100, 64, 512, False), (1000, 33, 257, False), (513, 31, 500, True), (33000, 128, 509, False),
+                                         (32770, 64, 300, True)])
 @pytest.mark.parametrize("pad,shift", [((0, 0, 0), 0), ((1, 3, 5), 1)])
 def test_narrow_layers(hip, m, n, k, gated, pad, shift):
     """all weights in one compute unit, every size of it, samples that do not fill the last block"""
