@@ -701,8 +701,9 @@ template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_fe
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
 // 262144 x 256 of 256 (268 MB) 67 us, 4.0 TB/s; 65521 x 256 and Z of 63 (75 MB) 23 us, of which staging the weights and filling the card take about 6.
+// ODD: lines that begin between two dwords are read by the dword (65521 x 256 and Z of 63 21.8 -> 20.6 us, 262144 x 64 of 255 68 -> 55 us; a kernel of its own, since the others lose 3 to 10 %).
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
-template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
+template <int NF, int KS, int EPI, bool EXCHANGE, bool ODD> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int OF = GATED ? NF / 2 : NF; // fragments of outputs
 	__shared__ __attribute__((aligned(16))) T w[NF * KS * 512];
@@ -711,12 +712,29 @@ template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(5
 	uint32_t slab = blockIdx.x * 8 + wave;
 	const int steps = (int)g.steps, whole_ks = steps / 32; // steps of 32 without a line's end
 	T8 x[KS];
+	uint32_t last[ODD ? KS : 1]; // fifth dwords
 	auto load_x = [&](uint32_t s) {
 		const T* line = g.a + (uint64_t)min(s * 16 + li, g.rows - 1) * g.lda; // (samples behind the last one repeat it and are dropped)
 #pragma unroll
-		for (int k = 0; k < KS; ++k) x[k] = load8(line + min(k * 32 + (int)gq * 8, steps - 8));
+		for (int k = 0; k < KS; ++k) {
+			const T* p = line + min(k * 32 + (int)gq * 8, steps - 8);
+			if (ODD) { const uint32_t* q = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3); __builtin_memcpy(&x[k], q, 16); last[ODD ? k : 0] = q[(uintptr_t)p & 2 ? 4 : 3]; }
+			else x[k] = load8(p);
+		}
 	};
-	auto tail_x = [&]() { // the line's end
+	auto tail_x = [&](uint32_t s) { // the line's end
+		if constexpr (ODD) { // elements out of the dwords (load8_odd in two steps: these loads were on their way)
+			const bool odd_line = (uintptr_t)(g.a + (uint64_t)min(s * 16 + li, g.rows - 1) * g.lda) & 2;
+#pragma unroll
+			for (int k = 0; k < KS; ++k) {
+				const bool odd = odd_line != (k * 32 + (int)gq * 8 > steps - 8 && (steps & 1));
+				uint32_t v[4];
+				__builtin_memcpy(v, &x[k], 16);
+				const uint32_t r[4] = {odd ? __builtin_amdgcn_alignbit(v[1], v[0], 16) : v[0], odd ? __builtin_amdgcn_alignbit(v[2], v[1], 16) : v[1],
+					odd ? __builtin_amdgcn_alignbit(v[3], v[2], 16) : v[2], odd ? __builtin_amdgcn_alignbit(last[ODD ? k : 0], v[3], 16) : v[3]};
+				__builtin_memcpy(&x[k], r, 16);
+			}
+		}
 		if (whole_ks == KS) return;
 #pragma unroll
 		for (int k = 0; k < KS; ++k) if (k >= whole_ks) x[k] = shift8(x[k], k * 32 + gq * 8, steps);
@@ -745,7 +763,7 @@ template <int NF, int KS, int EPI, bool EXCHANGE> __global__ __launch_bounds__(5
 		f4v acc[NF];
 #pragma unroll
 		for (int f = 0; f < NF; ++f) acc[f] = f4v{0.f, 0.f, 0.f, 0.f};
-		tail_x();
+		tail_x(slab);
 #pragma unroll
 		for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -1207,11 +1225,15 @@ template <int MT, int EPI> void launch_few_rows(hipStream_t s, GemmArgs& g, floa
 	} else if (odd) hipLaunchKernelGGL((k_few_rows<MT, EPI, true>), grid, dim3(512), 0, s, g, f.slices, per);
 	else hipLaunchKernelGGL((k_few_rows<MT, EPI, false>), grid, dim3(512), 0, s, g, f.slices, per);
 }
+template <int NF, int KS, int EPI, bool EXCHANGE> void launch_narrow_forward_nk(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
+	if (odd_lines(g.a, g.lda)) hipLaunchKernelGGL((k_narrow_forward<NF, KS, EPI, EXCHANGE, true>), dim3(blocks), dim3(512), 0, s, g);
+	else hipLaunchKernelGGL((k_narrow_forward<NF, KS, EPI, EXCHANGE, false>), dim3(blocks), dim3(512), 0, s, g);
+}
 template <int NF, int EPI, bool EXCHANGE> void launch_narrow_forward_n(hipStream_t s, const GemmArgs& g, uint32_t blocks) {
-	if (g.steps <= 64) hipLaunchKernelGGL((k_narrow_forward<NF, 2, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
-	else if (g.steps <= 128) hipLaunchKernelGGL((k_narrow_forward<NF, 4, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
-	else if (NF > 4 || g.steps <= 256) hipLaunchKernelGGL((k_narrow_forward<NF, 8, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
-	else if constexpr (NF == 4) hipLaunchKernelGGL((k_narrow_forward<NF, 16, EPI, EXCHANGE>), dim3(blocks), dim3(512), 0, s, g);
+	if (g.steps <= 64) launch_narrow_forward_nk<NF, 2, EPI, EXCHANGE>(s, g, blocks);
+	else if (g.steps <= 128) launch_narrow_forward_nk<NF, 4, EPI, EXCHANGE>(s, g, blocks);
+	else if (NF > 4 || g.steps <= 256) launch_narrow_forward_nk<NF, 8, EPI, EXCHANGE>(s, g, blocks);
+	else if constexpr (NF == 4) launch_narrow_forward_nk<NF, 16, EPI, EXCHANGE>(s, g, blocks);
 }
 template <int EPI, bool EXCHANGE> void launch_narrow_forward(hipStream_t s, const GemmArgs& g) {
 	const uint32_t cols = g.cols * (EPI == EPI_GATED ? 2 : 1), blocks = std::min(div_up(g.rows, 128), 512u);
