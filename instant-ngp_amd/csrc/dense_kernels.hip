@@ -700,7 +700,7 @@ template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_fe
 // ---- narrow layers (up to 256 inputs and outputs) over many samples: bound by reading and writing the samples once.
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
-// 262144 x 256 of 256 (268 MB) 67 us, 4.0 TB/s; 65521 x 256 and Z of 63 (75 MB) 23 us, of which staging the weights and filling the card take about 6.
+// 262144 x 256 of 256 (268 MB) 67 us, 4.0 TB/s; 65521 x 256 and Z of 63 (75 MB) 20.7 us, 3.6 TB/s, of which staging the weights and filling the card take about 5.
 // ODD: lines that begin between two dwords are read by the dword (65521 x 256 and Z of 63 21.8 -> 20.6 us, 262144 x 64 of 255 68 -> 55 us; a kernel of its own, since the others lose 3 to 10 %).
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
 template <int NF, int KS, int EPI, bool EXCHANGE, bool ODD> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
@@ -1260,7 +1260,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 	for (int i = 0; i < 2; ++i) { g.b[i] = (const T*)d.w[i]; g.bias[i] = (const T*)d.bias[i]; g.pre[i] = (T*)d.pre[i]; }
 	g.c[0] = (T*)d.y; g.ldc = d.y_stride; g.act = d.act; g.residual = (const T*)d.residual; g.ld_residual = d.residual_stride; g.ld_pre = d.pre_stride;
 	// Outputs that the 256 MB of the last cache would not hold beside the inputs go past the caches (262144 x 256 from 64 inputs: 95 -> 78 us; 8192 x 4096 x 2 from 4096: 237 -> 230 us; 72112 x 1894
-	// from 1224: 405 -> 365 us); smaller ones stay there for their readers (65521 x 256 x 2 from 63: 23 us, past the caches 25 us).  Narrow layers' only in whole cache lines,
+	// from 1224: 405 -> 365 us); smaller ones stay there for their readers (65521 x 256 x 2 from 63: 23 us then, past the caches 25 us).  Narrow layers' only in whole cache lines,
 	// which the caches need not join (262144 x 256 x 2 at a stride of 264: 165 us, 246 us past the caches).
 	const bool large = g.streamed = (uint64_t)d.m * d.n * 2 * (1 + (d.pre[0] != nullptr) + (d.pre[1] != nullptr)) >= 128ull << 20;
 	float* partial = (float*)d.workspace;
