@@ -1136,7 +1136,7 @@ __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32
 }
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 3) == 0 && (ld & 1) == 0 && (width & 7) == 0 && ld <= (1u << 21); } // 16-byte pieces, each from a dword on; a tile's offsets fit 31 bits
+bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 3) == 0 && (ld & 1) == 0 && (width & 7) == 0 && ld <= DENSE_LINE; } // 16-byte pieces, each from a dword on; a tile's offsets fit 31 bits
 // X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else; memory bound (200000 x 500: 64 us, 6.3 TB/s)
 struct PackArgs { const T* from[3]; T* to[3]; uint64_t ld[3]; uint32_t lines[3]; uint32_t width; };
 __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
@@ -1173,7 +1173,7 @@ Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room) {
 	if (!o.whole_x) { pack(0, o.x, d.m, d.x_stride); o.ld_x = k8; }
 	if (!o.whole_w) { pack(1, o.w[0], d.n, d.w_stride); pack(2, o.w[1], d.n, d.w_stride); o.ld_w = k8; }
 	if (chunks) hipLaunchKernelGGL(k_pack, dim3(div_up(chunks, 256)), dim3(256), 0, s, a);
-	o.whole_x = o.whole_w = true;
+	o.whole_x = whole(o.x, o.ld_x, k8); o.whole_w = whole(o.w[0], o.ld_w, k8) && whole(o.w[1], o.ld_w, k8);
 	return o;
 }
 // threads that share the pieces of 8 sums: more for many pieces of few sums (56 x 56 of 512 pieces, with the bias: 6.4 us, 9.6 with 8; 256 x 256 of 256 the other way: 14.3 and 11.9)

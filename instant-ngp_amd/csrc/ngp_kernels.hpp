@@ -421,9 +421,11 @@ inline bool dense_narrow_backward(uint32_t m, uint32_t n, uint32_t k, bool gated
 // us copied / staged, 1004 inputs: forward 65536 samples 400 outputs 125 / 117, 1032 outputs 229 / 264; 4096 samples 2056 outputs 45 / 53; 200 samples, 2004 inputs, 2056 outputs 23.5 / 19.7.
 // Backward 65536 samples 400 outputs 290 / 268, 1032 outputs 512 / 592; 4096 samples (8 MB of inputs, which caches hold) 400 outputs 34 / 38; 64 samples, 4100 inputs, 520 outputs 21 / 21.
 // The backward pass has the room whatever k is, for lines at odd strides (2000 samples 1000 x 1000: 70 staged); a forward pass only where lines are no whole pieces by themselves.
+// Longer lines than DENSE_LINE are never copied: the tiles that take copies reach a tile's lines by 31-bit offsets.
+constexpr uint32_t DENSE_LINE = 1u << 21; // elements from line to line, at most: 255 lines of a tile times 2^21 times 2 bytes is 2^30
 inline uint64_t dense_pack_bytes(uint64_t m, uint64_t n, uint64_t k, bool gated, bool backward) {
 	const uint64_t cols = (gated ? 2 : 1) * n;
-	if ((!backward && !(k & 7)) || k < 8 || m <= FEW_ROWS || (backward ? dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) : dense_narrow_forward((uint32_t)m, (uint32_t)n, (uint32_t)k, gated)) || (double)m * (double)cols * (double)k < 1e8) return 0;
+	if ((!backward && !(k & 7)) || k < 8 || k > DENSE_LINE || m <= FEW_ROWS || (backward ? dense_narrow((uint32_t)m, (uint32_t)n, (uint32_t)k, gated) : dense_narrow_forward((uint32_t)m, (uint32_t)n, (uint32_t)k, gated)) || (double)m * (double)cols * (double)k < 1e8) return 0;
 	if (backward ? m < 128 || (cols < 768 && m * k > 8u << 20) : m < 512 || cols < 768) return 0;
 	return ((m + cols) * ((k + 7) & ~7ull) * 2 + 255) & ~255ull;
 }

@@ -733,3 +733,17 @@ def test_forward_workspace(gated, m, n, k):
         else:
             rc = L.ngp_linear_forward(None, A.TYPE_HALF, A.ACT_SILU, m, n, k, a[0], k, a[1], k, None, None, 0, a[3], n, a[4], n, work, have)
         assert rc != 0 and what in L.ngp_last_error().decode()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(512, 768, 8500001), (512, 1000, (1 << 24) - 1), (1000, 2000, (1 << 21) + 1), (128, 64, 1 << 24), (70000, 800, (1 << 21) + 8)])
+def test_no_copies_of_very_long_lines(gated, m, n, k):
+    """the tiles that read copied operands reach a tile's lines by 31-bit offsets (255 lines of 2^21 elements): longer lines are not copied, so no size asks for room for them"""
+    L = lib()
+    size = L.ngp_gated_workspace_size if gated else L.ngp_linear_workspace_size
+    cols = (2 if gated else 1) * n
+    copies = 2 * (m + cols) * (k // 8 * 8)
+    partial = 600 << 20  # two sets of partial sums of at most 256 MB and a little, and G
+    assert size(m, n, k, 0) < min(copies, partial) + 2 * cols * m and size(m, n, k, 1) < min(copies, partial) + 4 * cols * (m + 8)
+    k = 1 << 21  # the longest that are (the backward pass has the room for lines at odd strides)
+    assert size(2000, 1000, k, 1) >= 2 * (2000 + (2000 if gated else 1000)) * k and size(2000, 1000, k - 1, 0) >= 2 * (2000 + (2000 if gated else 1000)) * k
