@@ -359,8 +359,8 @@ struct DenseFewRows { uint32_t slices, splits; };
 inline DenseFewRows dense_few_rows(uint32_t cols, uint32_t steps) {
 	DenseFewRows f{8, 1};
 	while (f.slices > 1 && steps < f.slices * 128) f.slices /= 2;
-	const uint32_t blocks = ((cols + 15) / 16 + 8 / f.slices - 1) / (8 / f.slices);
-	while (blocks * f.splits < 128 && steps >= f.splits * 2 * 2048) f.splits *= 2;
+	const uint64_t blocks = (((uint64_t)cols + 15) / 16 + 8 / f.slices - 1) / (8 / f.slices);
+	while (blocks && blocks * f.splits < 128 && steps >= (uint64_t)f.splits * 2 * 2048) f.splits *= 2; // (64 bits: sizes are asked for before they are checked)
 	return f;
 }
 // A product of rows x cols with `steps * segments` terms a sum, `parts` times over: tile size and the number of pieces every sum is cut into (each a block of its own, joined by a

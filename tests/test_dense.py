@@ -747,3 +747,24 @@ def test_no_copies_of_very_long_lines(gated, m, n, k):
     assert size(m, n, k, 0) < min(copies, partial) + 2 * cols * m and size(m, n, k, 1) < min(copies, partial) + 4 * cols * (m + 8)
     k = 1 << 21  # the longest that are (the backward pass has the room for lines at odd strides)
     assert size(2000, 1000, k, 1) >= 2 * (2000 + (2000 if gated else 1000)) * k and size(2000, 1000, k - 1, 0) >= 2 * (2000 + (2000 if gated else 1000)) * k
+
+
+def test_sizes_out_of_range_are_answered():
+    """a size may be asked for before anything is checked: every value has an answer, and the call itself refuses what is out of range.  (In a process of its own: a rule that never ends is to fail.)"""
+    import os
+    import subprocess
+    import sys
+    code = """
+import itertools, ngp_abi as A
+L, big = A.load_hip(), 0xffffffff
+for m, n, k, back in itertools.product((0, 5, big), (0, 3, big), (0, 7, 1 << 31, big), (0, 1)):
+    L.ngp_linear_workspace_size(m, n, k, back), L.ngp_gated_workspace_size(m, n, k, back)
+assert L.ngp_linear_workspace_size(5, 0, big, 0) == 0 and L.ngp_gated_workspace_size(5, 0, 1 << 31, 0) == 0
+for n, k in ((0, big), (0, 1 << 31), (big, big)):
+    assert L.ngp_linear_forward(None, A.TYPE_HALF, A.ACT_RELU, 5, n, k, 0x1000, k, 0x2000, k, None, None, 0, 0x3000, n, None, 0, 1 << 32, 1 << 60) != 0
+    assert 'at most' in L.ngp_last_error().decode(), L.ngp_last_error()
+print('answered')
+"""
+    path = os.pathsep.join([os.path.dirname(os.path.abspath(A.__file__)), os.environ.get("PYTHONPATH", "")])
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "answered" in r.stdout, r.stderr
