@@ -88,8 +88,8 @@ template <uint32_t THREADS = 256> __device__ inline double block_sum(double s) {
 	for (uint32_t i = 0; i < THREADS / 64; ++i) s += red[i];
 	return s;
 }
-// max_norm / norm where the norm is finite and beyond it
-__device__ inline float clip_factor(double norm, float max_norm) { return norm <= 1.7976931348623157e308 && norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f; }
+// max_norm / norm where the norm is beyond it and finite as the caller sees it, in 32 bits
+__device__ inline float clip_factor(double norm, float max_norm) { return (float)norm <= 3.402823466e38f && norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f; }
 __global__ __launch_bounds__(THREADS) void k_norm_partial(ClipTable t, double* slots, uint32_t written) {
 	const Range r = block_range(t.first[t.n]);
 	double s = 0;

@@ -108,6 +108,25 @@ def test_wide_range(hip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("spec", [[(2, F)], [(3, B), (9, H)], [(300_000, F), (5, B)]])
+@pytest.mark.parametrize("loss_scale", [1.0, 2.0 ** -20])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_norm_beyond_the_largest_float(hip, spec, loss_scale, in_place):
+    """finite gradients whose norm is no 32-bit number: what is reported is infinite, so the gradients are left as they are"""
+    import torch
+    s = Set(spec, in_place)
+    for buf, out, v, n, t, sh in s.items:
+        if t != H:
+            v.copy_(torch.where(torch.arange(n, device="cuda") % 2 == 0, 3e38, -3e38).to(v.dtype))
+            buf[sh:sh + n] = v
+    assert 3.4028235e38 < s.exact(loss_scale) < 1e300
+    s.clip(loss_scale, 1e30)
+    assert float(s.norm[1]) == float("inf")
+    for buf, out, v, n, t, sh in s.items:
+        assert bool((out[sh:sh + n] == v).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("t", [H, B, F])
 def test_not_finite(hip, bad, t):
