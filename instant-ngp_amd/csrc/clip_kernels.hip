@@ -45,19 +45,20 @@ template <uint32_t THREADS, typename T> __device__ inline double sum_squares(con
 	}
 	return s;
 }
-template <uint32_t THREADS, typename T> __device__ inline void scale(const T* p, T* q, uint32_t n, float c) {
+// C: float, or double for factors below what a float holds in full (1e-3 / 1e37: g c is an ordinary number, c is not)
+template <uint32_t THREADS, typename C, typename T> __device__ inline void scale(const T* p, T* q, uint32_t n, C c) {
 	constexpr int N = 16 / sizeof(T);
 	const uint32_t head = head_of(q, n); // (whole lines are written; p has the same alignment or is read across it)
-	if (threadIdx.x < head) q[threadIdx.x] = (T)((float)p[threadIdx.x] * c);
+	if (threadIdx.x < head) q[threadIdx.x] = (T)(float)((C)(float)p[threadIdx.x] * c);
 	p += head; q += head; n -= head;
 	const uint32_t tail = n % N;
-	if (threadIdx.x >= THREADS - tail) { const uint32_t i = n - (THREADS - threadIdx.x); q[i] = (T)((float)p[i] * c); }
+	if (threadIdx.x >= THREADS - tail) { const uint32_t i = n - (THREADS - threadIdx.x); q[i] = (T)(float)((C)(float)p[i] * c); }
 #pragma unroll 4
 	for (uint32_t i = threadIdx.x * N; i + N <= n; i += THREADS * N) {
 		Vec<T, N> v;
 		__builtin_memcpy(&v, p + i, 16);
 #pragma unroll
-		for (int e = 0; e < N; ++e) v.v[e] = (T)((float)v.v[e] * c); // rounded once, to the gradient's own type
+		for (int e = 0; e < N; ++e) v.v[e] = (T)(float)((C)(float)v.v[e] * c); // rounded once, to the gradient's own type
 		typedef float f4 __attribute__((ext_vector_type(4)));
 		__builtin_nontemporal_store(__builtin_bit_cast(f4, v), (f4*)(q + i)); // (not wanted again: the caches keep gradients that are still to be read)
 	}
@@ -69,12 +70,15 @@ template <uint32_t THREADS> __device__ inline double sum_tensor(int type, const 
 		default: return sum_squares<THREADS>((const float*)p + at, n);
 	}
 }
-template <uint32_t THREADS> __device__ inline void scale_tensor(int type, const void* p, void* q, uint64_t at, uint32_t n, float c) {
+template <uint32_t THREADS, typename C> __device__ inline void scale_typed(int type, const void* p, void* q, uint64_t at, uint32_t n, C c) {
 	switch (type) {
 		case NGP_TYPE_HALF: scale<THREADS>((const _Float16*)p + at, (_Float16*)q + at, n, c); break;
 		case NGP_TYPE_BFLOAT16: scale<THREADS>((const __bf16*)p + at, (__bf16*)q + at, n, c); break;
 		default: scale<THREADS>((const float*)p + at, (float*)q + at, n, c); break;
 	}
+}
+template <uint32_t THREADS> __device__ inline void scale_tensor(int type, const void* p, void* q, uint64_t at, uint32_t n, double c) {
+	if (c >= 1.17549435e-38) scale_typed<THREADS>(type, p, q, at, n, (float)c); else scale_typed<THREADS>(type, p, q, at, n, c);
 }
 template <uint32_t THREADS = 256> __device__ inline double block_sum(double s) { // the sum over the block, in every thread
 	__shared__ double red[THREADS / 64];
@@ -88,8 +92,12 @@ template <uint32_t THREADS = 256> __device__ inline double block_sum(double s) {
 	for (uint32_t i = 0; i < THREADS / 64; ++i) s += red[i];
 	return s;
 }
-// max_norm / norm where the norm is beyond it and finite as the caller sees it, in 32 bits
-__device__ inline float clip_factor(double norm, float max_norm) { return (float)norm <= 3.402823466e38f && norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f; }
+// max_norm / norm where the norm is beyond it and finite as the caller sees it, in 32 bits; itself a 32-bit number unless it is too small for one
+__device__ inline double clip_factor(double norm, float max_norm) {
+	if (!((float)norm <= 3.402823466e38f && norm > (double)max_norm)) return 1.0;
+	const double c = (double)max_norm / norm;
+	return c >= 1.17549435e-38 ? (double)(float)c : c;
+}
 __global__ __launch_bounds__(THREADS) void k_norm_partial(ClipTable t, double* slots, uint32_t written) {
 	const Range r = block_range(t.first[t.n]);
 	double s = 0;
@@ -115,13 +123,13 @@ __global__ __launch_bounds__(THREADS) void k_norm_finish(const double* slots, ui
 __global__ __launch_bounds__(THREADS) void k_clip(ClipTable t, const double* slots, uint32_t n_slots, float loss_scale, float max_norm, float* norm) {
 	const double v = norm_of(slots, n_slots, loss_scale);
 	if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-	const float c = clip_factor(v, max_norm);
+	const double c = clip_factor(v, max_norm);
 	const Range r = block_range(t.first[t.n]);
 	if (r.begin >= r.end) return;
 	uint32_t i = tensor_of(t, r.end - 1);
 	for (uint32_t k = r.end; k-- > r.begin;) {
 		while (t.first[i] > k) --i;
-		if (!t.clipped[i] || (c == 1.f && t.clipped[i] == t.grad[i])) continue;
+		if (!t.clipped[i] || (c == 1.0 && t.clipped[i] == t.grad[i])) continue;
 		const uint64_t at = (uint64_t)(k - t.first[i]) * CHUNK, left = t.size[i] - at;
 		const uint32_t n = left < CHUNK ? (uint32_t)left : CHUNK;
 		scale_tensor<THREADS>(t.type[i], t.grad[i], t.clipped[i], at, n, c);
@@ -133,9 +141,9 @@ __global__ __launch_bounds__(1024) void k_clip_small(ClipTable t, float loss_sca
 	for (uint32_t i = 0; i < t.n; ++i) s += sum_tensor<1024>(t.type[i], t.grad[i], 0, (uint32_t)t.size[i]);
 	const double v = sqrt(block_sum<1024>(s)) / (double)loss_scale;
 	if (threadIdx.x == 0) *norm = (float)v;
-	const float c = clip_factor(v, max_norm);
+	const double c = clip_factor(v, max_norm);
 	for (uint32_t i = 0; i < t.n; ++i)
-		if (t.clipped[i] && !(c == 1.f && t.clipped[i] == t.grad[i])) scale_tensor<1024>(t.type[i], t.grad[i], t.clipped[i], 0, (uint32_t)t.size[i], c);
+		if (t.clipped[i] && !(c == 1.0 && t.clipped[i] == t.grad[i])) scale_tensor<1024>(t.type[i], t.grad[i], t.clipped[i], 0, (uint32_t)t.size[i], c);
 }
 } // namespace
 

@@ -127,6 +127,19 @@ def test_norm_beyond_the_largest_float(hip, spec, loss_scale, in_place):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("spec", [[(5, F), (40, B)], [(70_000, F), (8195, B)]])
+@pytest.mark.parametrize("scale,loss_scale,max_norm", [(1e35, 1.0, 1e-3), (1e35, 1.0, 1e-7), (1e35, 2.0 ** 60, 1e-21), (1e35, 1.0, 1e-20)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_factors_below_the_smallest_float(hip, spec, scale, loss_scale, max_norm, in_place):
+    """huge gradients and a small bound: the factor is no 32-bit number in full, the clipped gradients are ordinary ones"""
+    s = Set(spec, in_place, scale=scale)
+    max_norm = float(np.float32(max_norm))
+    assert max_norm / s.exact(loss_scale) < 1.17e-38
+    s.clip(loss_scale, max_norm)
+    s.check(loss_scale, max_norm)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("t", [H, B, F])
 def test_not_finite(hip, bad, t):
