@@ -2792,7 +2792,7 @@ static int gradient_norm(const char* what, void* stream, uint32_t n, const ngp_g
 		const uint32_t bytes = t[i].type == NGP_TYPE_FLOAT ? 4 : 2;
 		REQUIRE(t[i].grad, w + ": null gradient");
 		REQUIRE(t[i].size <= (1ull << 43), w + ": a tensor of more than 2^43 elements");
-		REQUIRE((((uintptr_t)t[i].grad | (uintptr_t)t[i].clipped) & (bytes - 1)) == 0, w + ": a tensor is not aligned to its elements");
+		REQUIRE((((uintptr_t)t[i].grad | (clip ? (uintptr_t)t[i].clipped : 0)) & (bytes - 1)) == 0, w + ": a tensor is not aligned to its elements");
 		const bool in_place = clip && t[i].clipped == t[i].grad;
 		const uint64_t a = (uint64_t)t[i].grad, b = (uint64_t)t[i].clipped, len = t[i].size * bytes;
 		spans.push_back({a, a + len, in_place});

@@ -249,3 +249,14 @@ def test_refusals():
     if not L.ngp_device_available():
         ok = [good, (0x1020, 0x1020, 16, H, 0), (0x4000, 0x5000, 3, F, 0), (None, None, 0, B, 0)]
         assert "no HIP device" in call(ok) and "no HIP device" in call(ok[::-1]) and "no HIP device" in call([good, good], f="norm")  # (the norm may count a tensor twice)
+
+
+def test_norm_does_not_look_at_clipped():
+    """ngp_gradient_norm takes a table whose `clipped` was never set: whatever stands there is no reason to refuse it"""
+    L = A.load_hip()
+    if L.ngp_device_available():
+        pytest.skip("has a GPU: these addresses are not its own")
+    for clipped in (0x2001, 0x1001, 0x100000, 0x200000, 0x1008, (1 << 64) - 1):
+        table = (A.Gradient * 2)(A.Gradient(0x1000, clipped, 16, H, 0), A.Gradient(0x4000, clipped, 16, F, 0))
+        assert L.ngp_gradient_norm(None, 2, table, 1.0, 0x100000, 0x200000, 1 << 20) != 0
+        assert "no HIP device" in L.ngp_last_error().decode()
