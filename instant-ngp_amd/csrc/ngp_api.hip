@@ -2785,6 +2785,8 @@ static int gradient_norm(const char* what, void* stream, uint32_t n, const ngp_g
 	spans.clear(); buffers.clear();
 	spans.push_back({(uint64_t)workspace, (uint64_t)workspace + ngp_gradient_workspace_size(), true});
 	spans.push_back({(uint64_t)norm, (uint64_t)norm + 4, true});
+	buffers.push_back({workspace, 1, ngp_gradient_workspace_size(), ngp_gradient_workspace_size(), "workspace", true, 1});
+	buffers.push_back({norm, 1, 1, 1, "norm", true, 4});
 	bool sorted = true;
 	for (uint32_t i = 0; i < n; ++i) {
 		REQUIRE(t[i].type == NGP_TYPE_HALF || t[i].type == NGP_TYPE_BFLOAT16 || t[i].type == NGP_TYPE_FLOAT, w + ": type must be NGP_TYPE_HALF, NGP_TYPE_BFLOAT16 or NGP_TYPE_FLOAT");
