@@ -2674,12 +2674,30 @@ static int dense_check_device(const char* what, hipStream_t s, const DenseBuffer
 	}
 	return 0;
 }
-static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t n, uint32_t k, hipStream_t s, const DenseBuffer* b, size_t nb, const void* may_share_a, const void* may_share_b) {
+// Blocks of the largest launch of tiles that a layer's products take, 128 x 128 outputs each; a launch holds fewer than 2^32 threads.  (Every other kernel's grid is bounded by the sizes' own
+// limits: few rows and narrow layers, shared sums of at most 256 MB, the gradients of the pre-activations.)
+static uint64_t dense_forward_blocks(uint32_t m, uint32_t n, uint32_t k, bool gated) {
+	if (!m || !n || (m <= FEW_ROWS && k) || dense_narrow_forward(m, n, k, gated)) return 0;
+	return ((uint64_t)m + 127) / 128 * (((uint64_t)n * (gated ? 2 : 1) + 127) / 128) * dense_split(m, n, k, 1, gated ? 2 : 1).splits;
+}
+static uint64_t dense_backward_blocks(uint32_t m, uint32_t n, uint32_t k, bool gated, bool dx, bool dw) {
+	if (dense_narrow_backward(m, n, k, gated)) return 0;
+	const uint32_t problems = gated ? 2 : 1, terms = dense_two_terms(m, n, k) ? 2 : 1;
+	uint64_t most = 0;
+	for (uint32_t t = 1; t <= terms; ++t) {
+		uint64_t blocks = 0;
+		if (dx && m && k) blocks += ((uint64_t)m + 127) / 128 * (((uint64_t)k + 127) / 128) * dense_split(m, k, n, problems * t, 1).splits;
+		if (dw && n && k) blocks += ((uint64_t)n + 127) / 128 * (((uint64_t)k + 127) / 128) * problems * dense_split_dw(m, n, k, problems, t).splits;
+		most = std::max(most, blocks);
+	}
+	return most;
+}
+static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t n, uint32_t k, uint64_t blocks, hipStream_t s, const DenseBuffer* b, size_t nb, const void* may_share_a, const void* may_share_b) {
 	const std::string w = what;
 	REQUIRE(type == NGP_TYPE_HALF || type == NGP_TYPE_BFLOAT16, w + ": type must be NGP_TYPE_HALF or NGP_TYPE_BFLOAT16");
 	REQUIRE(act >= NGP_ACT_NONE && act <= NGP_ACT_GELU, w + ": unknown activation");
 	REQUIRE(m <= 0x7fffffffu && n <= (1u << 24) && k <= (1u << 24), w + ": at most 2^31 - 1 samples and 2^24 inputs / outputs");
-	REQUIRE((((uint64_t)m + 15) / 16) * (((uint64_t)n + 15) / 16) < (1ull << 31) && (((uint64_t)m + 15) / 16) * (((uint64_t)k + 15) / 16) < (1ull << 31), w + ": more output tiles than one launch takes; pass the samples in pieces");
+	REQUIRE(blocks < (1u << 24) && (((uint64_t)m + 15) / 16) * (((uint64_t)n + 15) / 16) < (1ull << 31) && (((uint64_t)m + 15) / 16) * (((uint64_t)k + 15) / 16) < (1ull << 31), w + ": more output tiles than one launch takes; pass the samples in pieces");
 	for (size_t i = 0; i < nb; ++i) {
 		if (!b[i].p) continue;
 		REQUIRE(b[i].stride >= b[i].width, w + ": stride of " + b[i].name + " too small");
@@ -2704,7 +2722,7 @@ extern "C" int ngp_linear_forward(void* stream, int type, int activation, uint32
 	REQUIRE((x && w) || !m || !n || !k, "ngp_linear_forward: null argument");
 	REQUIRE(y || !m || !n, "ngp_linear_forward: null argument");
 	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_linear_forward: workspace smaller than ngp_linear_workspace_size() or not 16-byte aligned");
-	if (int rc = dense_check("ngp_linear_forward", type, activation, m, n, k, (hipStream_t)stream, b, 7, y, residual)) return rc;
+	if (int rc = dense_check("ngp_linear_forward", type, activation, m, n, k, dense_forward_blocks(m, n, k, false), (hipStream_t)stream, b, 7, y, residual)) return rc;
 	DenseArgs d{};
 	d.gated = false; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w; d.w_stride = w_stride; d.bias[0] = bias;
 	d.residual = residual; d.residual_stride = residual_stride; d.y = y; d.y_stride = y_stride; d.pre[0] = pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;
@@ -2720,7 +2738,7 @@ extern "C" int ngp_gated_forward(void* stream, int type, int activation, uint32_
 	REQUIRE((x && w_gate && w_up) || !m || !n || !k, "ngp_gated_forward: null argument");
 	REQUIRE(y || !m || !n, "ngp_gated_forward: null argument");
 	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_gated_forward: workspace smaller than ngp_gated_workspace_size() or not 16-byte aligned");
-	if (int rc = dense_check("ngp_gated_forward", type, activation, m, n, k, (hipStream_t)stream, b, 9, nullptr, nullptr)) return rc;
+	if (int rc = dense_check("ngp_gated_forward", type, activation, m, n, k, dense_forward_blocks(m, n, k, true), (hipStream_t)stream, b, 9, nullptr, nullptr)) return rc;
 	DenseArgs d{};
 	d.gated = true; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w_gate; d.w[1] = w_up; d.w_stride = w_stride; d.bias[0] = bias_gate; d.bias[1] = bias_up;
 	d.y = y; d.y_stride = y_stride; d.pre[0] = gate_pre; d.pre[1] = up_pre; d.pre_stride = pre_stride; d.workspace = workspace; d.workspace_size = workspace_size;
@@ -2739,7 +2757,7 @@ extern "C" int ngp_linear_backward(void* stream, int type, int activation, uint3
 	REQUIRE(!dx || w || !m || !n || !k, "ngp_linear_backward: dx without w");
 	REQUIRE(!dw || x || !m || !n || !k, "ngp_linear_backward: dw without x");
 	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_linear_backward: workspace smaller than ngp_linear_workspace_size() or not 16-byte aligned");
-	if (int rc = dense_check("ngp_linear_backward", type, activation, m, n, k, (hipStream_t)stream, b, 8, nullptr, nullptr)) return rc;
+	if (int rc = dense_check("ngp_linear_backward", type, activation, m, n, k, dense_backward_blocks(m, n, k, false, dx, dw), (hipStream_t)stream, b, 8, nullptr, nullptr)) return rc;
 	DenseArgs d{};
 	d.gated = false; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w; d.w_stride = w_stride; d.pre[0] = (void*)pre; d.pre_stride = pre_stride;
 	d.dy = dy; d.dy_stride = dy_stride; d.dx = dx; d.dx_stride = dx_stride; d.dw[0] = dw; d.dw_stride = dw_stride; d.dbias[0] = dbias; d.workspace = workspace; d.workspace_size = workspace_size;
@@ -2759,7 +2777,7 @@ extern "C" int ngp_gated_backward(void* stream, int type, int activation, uint32
 	REQUIRE((dw_gate != nullptr) == (dw_up != nullptr), "ngp_gated_backward: dw_gate and dw_up come together");
 	REQUIRE(!dw_gate || x || !m || !n || !k, "ngp_gated_backward: dw without x");
 	REQUIRE((workspace && workspace_size >= need && ((uintptr_t)workspace & 15) == 0) || !need, "ngp_gated_backward: workspace smaller than ngp_gated_workspace_size() or not 16-byte aligned");
-	if (int rc = dense_check("ngp_gated_backward", type, activation, m, n, k, (hipStream_t)stream, b, 12, nullptr, nullptr)) return rc;
+	if (int rc = dense_check("ngp_gated_backward", type, activation, m, n, k, dense_backward_blocks(m, n, k, true, dx, dw_gate), (hipStream_t)stream, b, 12, nullptr, nullptr)) return rc;
 	DenseArgs d{};
 	d.gated = true; d.act = activation; d.m = m; d.n = n; d.k = k; d.x = x; d.x_stride = x_stride; d.w[0] = w_gate; d.w[1] = w_up; d.w_stride = w_stride; d.pre[0] = (void*)gate_pre; d.pre[1] = (void*)up_pre;
 	d.pre_stride = pre_stride; d.dy = dy; d.dy_stride = dy_stride; d.dx = dx; d.dx_stride = dx_stride; d.dw[0] = dw_gate; d.dw[1] = dw_up; d.dw_stride = dw_stride; d.dbias[0] = dbias_gate; d.dbias[1] = dbias_up;
