@@ -1139,20 +1139,24 @@ uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 bool whole(const void* p, uint64_t ld, uint64_t width) { return ((uintptr_t)p & 3) == 0 && (ld & 1) == 0 && (width & 7) == 0 && ld <= DENSE_LINE; } // 16-byte pieces, each from a dword on; a tile's offsets fit 31 bits
 // X and the weights with their lines padded with zeros to whole 16-byte pieces, for the tiles that take nothing else; memory bound (200000 x 500: 64 us, 6.3 TB/s)
 struct PackArgs { const T* from[3]; T* to[3]; uint64_t ld[3]; uint32_t lines[3]; uint32_t width; };
+constexpr uint32_t PACK_BLOCKS = 1u << 16; // at most; each then goes on to further chunks (X may have more chunks than a launch has threads)
 __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
 	const uint32_t cc = up8(g.width) / 8;
-	uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+	const uint64_t total = ((uint64_t)g.lines[0] + g.lines[1] + g.lines[2]) * cc;
+	for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (uint64_t)gridDim.x * 256) {
+		uint64_t id = at;
 #pragma unroll
-	for (int k = 0; k < 3; ++k) {
-		const uint64_t n = (uint64_t)g.lines[k] * cc;
-		if (id < n) {
-			const uint32_t line = (uint32_t)(id / cc), c = (uint32_t)(id % cc) * 8;
-			const T* p = g.from[k] + (uint64_t)line * g.ld[k];
-			const int start = min((int)c, (int)g.width - 8);
-			*(T8*)(g.to[k] + ((uint64_t)line * cc * 8 + c)) = shift8(load8_odd(p + start), c, g.width);
-			return;
+		for (int k = 0; k < 3; ++k) {
+			const uint64_t n = (uint64_t)g.lines[k] * cc;
+			if (id < n) {
+				const uint32_t line = (uint32_t)(id / cc), c = (uint32_t)(id % cc) * 8;
+				const T* p = g.from[k] + (uint64_t)line * g.ld[k];
+				const int start = min((int)c, (int)g.width - 8);
+				*(T8*)(g.to[k] + ((uint64_t)line * cc * 8 + c)) = shift8(load8_odd(p + start), c, g.width);
+				break;
+			}
+			id -= n;
 		}
-		id -= n;
 	}
 }
 // what the products read: the caller's matrices, or (with `room` for them) packed ones
@@ -1172,7 +1176,7 @@ Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room) {
 	a.width = d.k;
 	if (!o.whole_x) { pack(0, o.x, d.m, d.x_stride); o.ld_x = k8; }
 	if (!o.whole_w) { pack(1, o.w[0], d.n, d.w_stride); pack(2, o.w[1], d.n, d.w_stride); o.ld_w = k8; }
-	if (chunks) hipLaunchKernelGGL(k_pack, dim3(div_up(chunks, 256)), dim3(256), 0, s, a);
+	if (chunks) hipLaunchKernelGGL(k_pack, dim3((uint32_t)std::min<uint64_t>((chunks + 255) / 256, PACK_BLOCKS)), dim3(256), 0, s, a);
 	o.whole_x = whole(o.x, o.ld_x, k8); o.whole_w = whole(o.w[0], o.ld_w, k8) && whole(o.w[1], o.ld_w, k8);
 	return o;
 }

@@ -768,3 +768,10 @@ print('answered')
     path = os.pathsep.join([os.path.dirname(os.path.abspath(A.__file__)), os.environ.get("PYTHONPATH", "")])
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and "answered" in r.stdout, r.stderr
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated", [(34001, 770, 4001, False), (17001, 390, 8003, True)])
+def test_long_copies(hip, m, n, k, gated):
+    """more 16-byte pieces than the copying launch has threads"""
+    run_layer(Layer(A.TYPE_HALF, A.ACT_RELU, m, n, k, gated=gated))

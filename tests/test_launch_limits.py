@@ -47,8 +47,16 @@ for gated in (0, 1):
 print("done")
 """
 
+COPIES = CALLS + """
+# lines that are no whole pieces, 64 GB of them: copied before the products, more 16-byte pieces than a launch has threads
+for gated, m, n, k in ((0, 16500, 768, (1 << 21) - 1), (1, 20000, 500, (1 << 21) - 1), (0, 40000000, 800, 1003), (0, 16500, 900, (1 << 21) - 3)):
+    for backward in (0, 1):
+        assert call(gated, backward, m, n, k)
+print("done")
+"""
 
-@pytest.mark.parametrize("calls", [TILES], ids=["tiles"])
+
+@pytest.mark.parametrize("calls", [TILES, COPIES], ids=["tiles", "copies"])
 def test_grids(calls, tmp_path):
     if A.load_hip().ngp_device_available():
         pytest.skip("has a GPU: the runtime is not to be played there")
