@@ -1159,11 +1159,12 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs g) {
 		}
 	}
 }
-// what the products read: the caller's matrices, or (with `room` for them) packed ones
+// what the products read: the caller's matrices, or (with `room` for them) packed ones; X and the weights as far as they are wanted
 struct Operands { const T* x; const T* w[2]; uint64_t ld_x, ld_w; bool whole_x, whole_w; };
-Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room) {
+Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room, bool want_x, bool want_w) {
 	Operands o{(const T*)d.x, {(const T*)d.w[0], (const T*)d.w[1]}, d.x_stride, d.w_stride, whole(d.x, d.x_stride, d.k), whole(d.w[0], d.w_stride, d.k) && whole(d.w[1], d.w_stride, d.k)};
-	if (!room || (o.whole_x && o.whole_w)) return o;
+	const bool pack_x = room && want_x && !o.whole_x, pack_w = room && want_w && !o.whole_w;
+	if (!pack_x && !pack_w) return o;
 	PackArgs a{};
 	const uint64_t k8 = up8(d.k);
 	T* to = (T*)packed;
@@ -1174,10 +1175,11 @@ Operands operands(hipStream_t s, const DenseArgs& d, void* packed, bool room) {
 		to += lines * k8; chunks += lines * (k8 / 8);
 	};
 	a.width = d.k;
-	if (!o.whole_x) { pack(0, o.x, d.m, d.x_stride); o.ld_x = k8; }
-	if (!o.whole_w) { pack(1, o.w[0], d.n, d.w_stride); pack(2, o.w[1], d.n, d.w_stride); o.ld_w = k8; }
+	if (pack_x) { pack(0, o.x, d.m, d.x_stride); o.ld_x = k8; }
+	if (pack_w) { pack(1, o.w[0], d.n, d.w_stride); pack(2, o.w[1], d.n, d.w_stride); o.ld_w = k8; }
 	if (chunks) hipLaunchKernelGGL(k_pack, dim3((uint32_t)std::min<uint64_t>((chunks + 255) / 256, PACK_BLOCKS)), dim3(256), 0, s, a);
-	o.whole_x = whole(o.x, o.ld_x, k8); o.whole_w = whole(o.w[0], o.ld_w, k8) && whole(o.w[1], o.ld_w, k8);
+	if (pack_x) o.whole_x = whole(o.x, o.ld_x, k8);
+	if (pack_w) o.whole_w = whole(o.w[0], o.ld_w, k8) && whole(o.w[1], o.ld_w, k8);
 	return o;
 }
 // threads that share the pieces of 8 sums: more for many pieces of few sums (56 x 56 of 512 pieces, with the bias: 6.4 us, 9.6 with 8; 256 x 256 of 256 the other way: 14.3 and 11.9)
@@ -1280,7 +1282,7 @@ void DENSE_NAME(launch_dense_forward)(hipStream_t s, const DenseArgs& d) {
 		return;
 	}
 	const uint64_t room = dense_pack_bytes(d.m, d.n, d.k, d.gated, false);
-	const Operands o = operands(s, d, (char*)d.workspace + dense_forward_bytes(d.m, d.n, d.k, d.gated) - room, room != 0);
+	const Operands o = operands(s, d, (char*)d.workspace + dense_forward_bytes(d.m, d.n, d.k, d.gated) - room, room != 0, true, true);
 	const bool wholes = o.whole_x && o.whole_w;
 	g.a = o.x; g.lda = o.ld_x; g.b[0] = o.w[0]; g.b[1] = o.w[1]; g.ldb = o.ld_w;
 	if (d.gated) launch_forward<EPI_GATED>(s, g, wholes, partial); else launch_forward<EPI_LINEAR>(s, g, wholes, partial);
@@ -1330,7 +1332,7 @@ void DENSE_NAME(launch_dense_backward)(hipStream_t s, const DenseArgs& d) {
 	GemmArgs x{}, w{};
 	bool large_x = false, large_w = false;
 	const bool want_x = d.dx && d.m && d.k, want_w = d.dw[0] && d.n && d.k;
-	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack, p.bytes > p.pack) : Operands{};
+	const Operands o = want_x || want_w ? operands(s, d, ws + p.pack, p.bytes > p.pack, want_w, want_x) : Operands{}; // (dW reads X, dX the weights)
 	const bool whole_x = g_whole && o.whole_w, whole_w = g_whole && o.whole_x;
 	if (want_x) {
 		x.a = G; x.lda = ldg; x.a_segment = up8(d.n); x.segments = problems * terms; x.b[0] = o.w[0]; x.b[1] = d.gated ? o.w[1] : o.w[0]; x.ldb = o.ld_w;

@@ -775,3 +775,27 @@ print('answered')
 def test_long_copies(hip, m, n, k, gated):
     """more 16-byte pieces than the copying launch has threads"""
     run_layer(Layer(A.TYPE_HALF, A.ACT_RELU, m, n, k, gated=gated))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,gated,want", [(700, 777, 501, False, "x"), (700, 777, 501, False, "w"), (600, 400, 333, True, "x"), (600, 400, 333, True, "w"), (700, 777, 501, False, "xw")])
+def test_copies_of_what_is_read(hip, m, n, k, gated, want):
+    """dX alone reads the weights and dW alone the inputs: the other operand's copy is not made (as much of the workspace is written with it as without), and the results are those of the whole call"""
+    import torch
+    layer = Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=gated)
+    _, pre = layer.forward()
+    parts = layer.backward(pre, want)
+    written = int((layer.ws != 255).sum())
+    x, w = layer.x, layer.w
+    if want == "x":
+        layer.x = None
+    elif want == "w":
+        layer.w = [None for _ in w]
+    without = layer.backward(pre, want)
+    assert written == int((layer.ws != 255).sum())
+    layer.x, layer.w = x, w
+    whole = layer.backward(pre)
+    for a, b, c in zip([parts[0], *parts[1]], [without[0], *without[1]], [whole[0], *whole[1]]):
+        assert (a is None and b is None) or (torch.equal(a[1], b[1]) and torch.equal(a[1], c[1]))
+    layer.untouched()
+
