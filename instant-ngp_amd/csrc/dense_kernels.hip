@@ -157,7 +157,7 @@ template <bool GATED> __device__ inline void output_grad8(int act, const T8& dy,
 	EACH { d[e] = (float)dy[e]; z[e] = (float)zt[e]; m[e] = GATED ? d[e] * (float)ut[e] : d[e]; }
 	switch (act) {
 		case NGP_ACT_RELU: EACH { g[e] = z[e] > 0.f ? m[e] : 0.f; if (GATED) g2[e] = z[e] > 0.f ? d[e] * z[e] : 0.f; } break; // (a closed unit passes nothing, whatever arrives)
-		case NGP_ACT_LOGISTIC: EACH { const float p = logistic(z[e]); g[e] = m[e] * (p * (1.f - p)); if (GATED) g2[e] = d[e] * p; } break;
+		case NGP_ACT_LOGISTIC: EACH { const float x = __expf(-fabsf(z[e])), r = __builtin_amdgcn_rcpf(1.f + x); g[e] = m[e] * (x * r * r); if (GATED) g2[e] = d[e] * (z[e] < 0.f ? x * r : r); } break; // (p (1 - p) would lose its bits where p is near 1)
 		case NGP_ACT_EXPONENTIAL: EACH { const float p = __expf(z[e]); g[e] = m[e] * p; if (GATED) g2[e] = d[e] * p; } break;
 		case NGP_ACT_SILU: EACH { const float p = logistic(z[e]); g[e] = m[e] * (p * fmaf(z[e], 1.f - p, 1.f)); if (GATED) g2[e] = d[e] * (z[e] * p); } break;
 		case NGP_ACT_GELU: EACH { float x; const float c = normal_cdf(z[e], x); g[e] = m[e] * fmaf(z[e] * 0.39894228f, x, c); if (GATED) g2[e] = d[e] * (z[e] * c); } break;

@@ -799,3 +799,27 @@ def test_copies_of_what_is_read(hip, m, n, k, gated, want):
         assert (a is None and b is None) or (torch.equal(a[1], b[1]) and torch.equal(a[1], c[1]))
     layer.untouched()
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_,most", [(A.TYPE_HALF, 16.0), (A.TYPE_BFLOAT16, 60.0)])
+@pytest.mark.parametrize("m,n", [(1, 64), (40, 64), (3000, 64), (3000, 520)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_logistic_slope_in_both_tails(hip, type_, most, m, n, gated):
+    """p (1 - p) keeps its bits far from zero, on either side.  The weights are the unit matrix, so dX is G itself: a 16-bit rounding (u) and 32-bit operations, of which the exponential's are off by
+    its argument times 2^-24 twice (log2 e and the product with it are rounded) and a few steps, the other ones by one or two each: (2 |z| + 16) 2^-24."""
+    import torch
+    layer = Layer(type_, A.ACT_LOGISTIC, m, n, n, gated=gated, bias=False)
+    g = torch.Generator().manual_seed(m + n)
+    pre = [layer.matrix((torch.rand(m, n, generator=g) * 2 - 1) * most, 0)] + [layer.matrix(torch.randn(m, n, generator=g), 0) for _ in layer.w[1:]]
+    layer.dy[1].copy_((2.0 ** 12 * (1 + torch.rand(m, n, generator=g))).to(layer.dtype).cuda())
+    z, dy = pre[0][1].double(), layer.dy[1].double()
+    p, q = torch.sigmoid(z), torch.sigmoid(-z)
+    for which, want in enumerate([dy * p * q * (pre[1][1].double() if gated else 1)] + ([dy * p] if gated else [])):
+        for i, w in enumerate(layer.w):
+            w[1].copy_(torch.eye(n, device="cuda") * (i == which))
+        dx = layer.backward(pre, "x")[0]
+        tol = (U[type_] + 1.01 * (2 * z.abs() + 16) * F32) * want.abs() + TINY[type_]
+        off = (dx[1].double() - want).abs() / tol
+        assert bool((off <= 1).all()), f"{float(off.max()):.2f} of the tolerance at z = {float(z.reshape(-1)[off.argmax()]):.2f}"
+    layer.untouched()
