@@ -823,3 +823,73 @@ def test_logistic_slope_in_both_tails(hip, type_, most, m, n, gated):
         off = (dx[1].double() - want).abs() / tol
         assert bool((off <= 1).all()), f"{float(off.max()):.2f} of the tolerance at z = {float(z.reshape(-1)[off.argmax()]):.2f}"
     layer.untouched()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [A.TYPE_HALF, A.TYPE_BFLOAT16])
+@pytest.mark.parametrize("m,n,k", [(3700, 3593, 136), (300, 264, 512), (100, 48, 9000), (5, 16, 8192), (20, 100, 200), (300, 200, 333), (100, 48, 9001), (1000, 1000, 1003), (263001, 256, 16), (1000001, 72, 24), (700003, 100, 17),
+                                   (5000, 64, 64)])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_residual_in_place_every_way(hip, type_, m, n, k, pad):
+    """large and small tiles, shared sums, few rows with and without, tiles through registers, copied operands, narrow layers with and without the exchange between neighbouring samples"""
+    layer = Layer(type_, A.ACT_GELU, m, n, k, residual=True, pad=(0, 0, pad))
+    layer.residual64 = layer.residual[1].double().clone()
+    y, pre = layer.forward(save=m < 100000, y_is_residual=True)
+    layer.check_forward(y, pre)
+    layer.untouched()
+    y[1].fill_(float("nan"))
+    assert bool(y[0].isnan().all()), "written beside y"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type_", [A.TYPE_HALF, A.TYPE_BFLOAT16])
+@pytest.mark.parametrize("m,n,k,gated", [(3000, 64, 72, True), (2001, 30, 255, True), (33000, 128, 256, True), (3000, 64, 72, False), (5001, 16, 250, False), (33000, 250, 256, False)])
+def test_parts_of_the_gradient_of_narrow_layers(hip, type_, m, n, k, gated):
+    """each output alone is bit for bit the one of the whole call, and no operand that it does not need is looked at"""
+    layer = Layer(type_, A.ACT_SILU, m, n, k, gated=gated)
+    layer.residual64 = None
+    _, pre = layer.forward()
+    whole = layer.backward(pre)
+    layer.check_backward(pre, *whole)
+    x, w = layer.x, layer.w
+    for want, pick in (("x", lambda r: [r[0]]), ("w", lambda r: r[1]), ("b", lambda r: r[2]), ("xb", lambda r: [r[0], *r[2]]), ("wb", lambda r: [*r[1], *r[2]])):
+        layer.x = x if "w" in want else None
+        layer.w = w if "x" in want else [None for _ in w]
+        part = layer.backward(pre, want)
+        for a, b in zip(pick(part), pick(whole)):
+            assert bool((a[1] == b[1]).all())
+    layer.untouched()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [1 << 21, (1 << 21) + 2, (1 << 21) + 8])
+@pytest.mark.parametrize("m,n,k,gated", [(130, 264, 64, False), (130, 136, 64, True), (90, 64, 64, False), (257, 130, 72, False), (5, 40, 64, True)])
+def test_far_lines(hip, stride, m, n, k, gated):
+    """lines either side of what a tile's 31-bit offsets allow (2^21 elements from line to line)"""
+    run_layer(Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=gated, residual=not gated, pad=(stride - k, stride - k, stride - n)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(2, 16, 8192), (100, 64, 9000), (100, 64, 9001), (1000, 1000, 1003), (17, 40, 12290), (600, 400, 1003)])
+def test_behind_the_forward_workspace(hip, gated, m, n, k):
+    layer = Layer(A.TYPE_HALF, A.ACT_SILU, m, n, k, gated=gated)
+    layer.residual64 = None
+    layer.check_forward(*layer.forward())
+    size = (lib().ngp_gated_workspace_size if gated else lib().ngp_linear_workspace_size)(m, n, k, 0)
+    assert layer.ws.numel() == size + 64 and bool((layer.ws[size:] == 255).all())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_forward_workspace_sizes(gated):
+    """nothing where one launch does it all; room for partial sums, at most 256 MB of them, and for the operands' padded copies elsewhere"""
+    L = lib()
+    size = L.ngp_gated_workspace_size if gated else L.ngp_linear_workspace_size
+    cols = 2 if gated else 1
+    for m, n, k in ((1, 1, 1), (0, 8, 8), (8, 0, 8), (8, 8, 0), (1, 8192, 2048), (262144, 256 // cols, 256), (65521, 256 // cols, 63), (8192, 8192, 2048), (1 << 20, 64, 64)):
+        assert size(m, n, k, 0) == 0, (m, n, k)
+    for m, n, k in ((2, 16, 8192), (32, 100, 10000), (100, 64, 9000), (64, 200, 100000)):
+        assert 0 < size(m, n, k, 0) <= 256 << 20, (m, n, k)
+    for m, n, k in ((1000, 1000, 1003), (65536, 1032, 1004)):
+        copies = 2 * (m + cols * n) * ((k + 7) // 8 * 8)
+        assert copies <= size(m, n, k, 0) <= copies + (256 << 20), (m, n, k)
