@@ -2675,21 +2675,22 @@ static int dense_check_device(const char* what, hipStream_t s, const DenseBuffer
 	return 0;
 }
 // Blocks of the largest launch of tiles that a layer's products take, 128 x 128 outputs each; a launch holds fewer than 2^32 threads.  (Every other kernel's grid is bounded by the sizes' own
-// limits: few rows and narrow layers, shared sums of at most 256 MB, the gradients of the pre-activations.)
+// limits: few rows and narrow layers, shared sums of at most 256 MB, the gradients of the pre-activations.)  A sum has at most 256 pieces, so fewer than 2^16 tiles always fit and their pieces
+// need not be counted.
 static uint64_t dense_forward_blocks(uint32_t m, uint32_t n, uint32_t k, bool gated) {
-	if (!m || !n || (m <= FEW_ROWS && k) || dense_narrow_forward(m, n, k, gated)) return 0;
-	return ((uint64_t)m + 127) / 128 * (((uint64_t)n * (gated ? 2 : 1) + 127) / 128) * dense_split(m, n, k, 1, gated ? 2 : 1).splits;
+	const uint64_t tiles = ((uint64_t)m + 127) / 128 * (((uint64_t)n * (gated ? 2 : 1) + 127) / 128);
+	if (tiles < 1u << 16) return tiles;
+	if ((m <= FEW_ROWS && k) || dense_narrow_forward(m, n, k, gated)) return 0;
+	return tiles * dense_split(m, n, k, 1, gated ? 2 : 1).splits;
 }
 static uint64_t dense_backward_blocks(uint32_t m, uint32_t n, uint32_t k, bool gated, bool dx, bool dw) {
+	const uint32_t problems = gated ? 2 : 1;
+	const uint64_t tiles_x = dx ? ((uint64_t)m + 127) / 128 * (((uint64_t)k + 127) / 128) : 0, tiles_w = dw ? ((uint64_t)n + 127) / 128 * (((uint64_t)k + 127) / 128) * problems : 0;
+	if (tiles_x + tiles_w < 1u << 16) return tiles_x + tiles_w;
 	if (dense_narrow_backward(m, n, k, gated)) return 0;
-	const uint32_t problems = gated ? 2 : 1, terms = dense_two_terms(m, n, k) ? 2 : 1;
 	uint64_t most = 0;
-	for (uint32_t t = 1; t <= terms; ++t) {
-		uint64_t blocks = 0;
-		if (dx && m && k) blocks += ((uint64_t)m + 127) / 128 * (((uint64_t)k + 127) / 128) * dense_split(m, k, n, problems * t, 1).splits;
-		if (dw && n && k) blocks += ((uint64_t)n + 127) / 128 * (((uint64_t)k + 127) / 128) * problems * dense_split_dw(m, n, k, problems, t).splits;
-		most = std::max(most, blocks);
-	}
+	for (uint32_t t = 1; t <= (dense_two_terms(m, n, k) ? 2u : 1u); ++t) // (one term without an activation)
+		most = std::max(most, tiles_x * dense_split(m, k, n, problems * t, 1).splits + tiles_w * dense_split_dw(m, n, k, problems, t).splits);
 	return most;
 }
 static int dense_check(const char* what, int type, int act, uint32_t m, uint32_t n, uint32_t k, uint64_t blocks, hipStream_t s, const DenseBuffer* b, size_t nb, const void* may_share_a, const void* may_share_b) {
