@@ -176,3 +176,15 @@ def test_no_packed_floats(code_objects):
             assert p.wait() == 0 and not found, (path, found[:3])
             checked += 1
     assert checked == 3
+
+
+def test_no_packed_floats_in_any_kernel(code_objects):
+    """all of the library is compiled without them"""
+    found = {}
+    for path, symbols in code_objects.items():
+        p = subprocess.Popen([os.path.join(TOOLS, "llvm-objdump"), "-d", "--no-show-raw-insn", path], stdout=subprocess.PIPE, text=True)
+        n = sum("v_pk_" in line and re.search(r"\bv_pk_(add|mul|fma)_f32\b", line) is not None for line in p.stdout)
+        assert p.wait() == 0
+        if n:
+            found[os.path.basename(path)] = n
+    assert len(code_objects) >= 9 and not found, found
