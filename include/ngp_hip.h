@@ -282,7 +282,7 @@ uint32_t ngp_encmlp_step(const ngp_encmlp*);
 /* ------------------------------------------------------------------ dense layers --------- */
 /* Layers of any width beside the 64-wide fused networks above (the reference reaches for tiny-cuda-nn's layer-by-layer CutlassMLP there): one layer per call, activations in
  * global memory.  m samples, n outputs, k inputs; matrices are row-major with `*_stride` elements from row to row, weights [outputs][inputs] like the parameters above; any size
- * from 0, any stride >= the row's length, any address aligned to its elements.  `type` (NGP_TYPE_HALF | NGP_TYPE_BFLOAT16) is that of every matrix and vector of the call; products,
+ * from 0 (samples below 2^31, inputs and outputs up to 2^24; a product of more tiles than one launch holds is refused), any stride >= the row's length, any address aligned to its elements.  `type` (NGP_TYPE_HALF | NGP_TYPE_BFLOAT16) is that of every matrix and vector of the call; products,
  * sums and activations are computed in 32 bits and rounded once into each output.  Outputs must not overlap each other, an input or the workspace (columns of one wider matrix
  * may be shared out among them); y may be the residual itself.  `workspace` (16-byte aligned, at least ngp_*_workspace_size bytes; a call with a size of 0 takes NULL) is scratch:
  * calls that can run at the same time -- on two streams, in two graphs -- need one each.  Nothing is kept from call to call, nothing is allocated: calls can be captured. */
@@ -292,7 +292,8 @@ int ngp_linear_forward(void* stream, int type, int activation, uint32_t m, uint3
                        const void* bias, const void* residual, uint64_t residual_stride, void* y, uint64_t y_stride, void* pre, uint64_t pre_stride,
                        void* workspace, uint64_t workspace_size);
 /* G = dY * act'(Z);  dX = G W;  dW = G^T X;  dbias = column sums of G (each NULL = not wanted; overwritten).  The residual's gradient is dY itself.  `pre` is not read with
- * NGP_ACT_NONE.  G is rounded to `type` between the two products (small sets of G, whose roundings would not average out, keep what the rounding loses). */
+ * NGP_ACT_NONE.  G is rounded to `type` between the two products, which adds a rounding to dX's and dW's own (1.41 times one rounding's error, up to 1.65 where a few values decide) and holds G to
+ * the type's range, as a loss scale does dY; sets of up to 32768 of them with up to 4M weights keep what the rounding loses as a second term.  dbias sums G before it is rounded. */
 int ngp_linear_backward(void* stream, int type, int activation, uint32_t m, uint32_t n, uint32_t k, const void* x, uint64_t x_stride, const void* w, uint64_t w_stride,
                         const void* pre, uint64_t pre_stride, const void* dy, uint64_t dy_stride, void* dx, uint64_t dx_stride, void* dw, uint64_t dw_stride, void* dbias,
                         void* workspace, uint64_t workspace_size);
@@ -311,7 +312,9 @@ uint64_t ngp_gated_workspace_size(uint32_t m, uint32_t n, uint32_t k, int backwa
 
 /* ------------------------------------------------------------------ gradient clipping ---- */
 /* Between the gradients (ngp_model_training_step, ngp_encmlp_training_step, ngp_linear_backward ...) and the optimizer step, over tensors of any number, size and type.  Gradients
- * carry the loss scale; `norm` (device, one float) receives the norm of what the optimizer sees, sqrt(sum of g^2) / loss_scale, summed in 64 bits in a fixed order. */
+ * carry the loss scale; `norm` (device, one float) receives the norm of what the optimizer sees, sqrt(sum of g^2) / loss_scale, summed in 64 bits in a fixed order.  The gradients have to be there:
+ * ngp_nerf_train applies the optimizer to the hashed levels in its scatter and leaves none of them, so with a NeRF trainer the place is between ngp_nerf_train_forward_backward and
+ * ngp_nerf_train_finish. */
 typedef struct ngp_gradient {
 	const void* grad;    /* `size` elements, aligned to their type */
 	void* clipped;       /* where the clipped gradient goes: grad itself, another buffer, or NULL (counted in the norm, not clipped); not read by ngp_gradient_norm */
@@ -320,8 +323,8 @@ typedef struct ngp_gradient {
 	int32_t reserved;
 } ngp_gradient;
 int ngp_gradient_norm(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float* norm, void* workspace, uint64_t workspace_size);
-/* clipped = grad * min(1, max_norm / norm), rounded once; in place nothing is written where the factor is 1.  A norm that is not finite is reported and leaves the gradients as they
- * are (the caller skips the step).  What is written must not overlap another tensor.  The table is read before the call returns; `workspace` as for the dense layers. */
+/* clipped = grad * min(1, max_norm / norm), rounded once; in place nothing is written where the factor is 1.  A norm that is not finite as a float is reported and leaves the gradients as
+ * they are (the caller skips the step).  What is written must not overlap another tensor.  The table is read before the call returns; `workspace` as for the dense layers. */
 int ngp_clip_gradients(void* stream, uint32_t n_tensors, const ngp_gradient* tensors_host, float loss_scale, float max_norm, float* norm, void* workspace, uint64_t workspace_size);
 uint64_t ngp_gradient_workspace_size(void);
 

@@ -39,7 +39,8 @@ __device__ inline f4v mfma(T8 a, T8 b, f4v c) {
 #endif
 }
 // the same with the sums held in place in accumulation registers (the compiler, left to itself, moves 256 of them about and spills).  Whoever reads the sums with
-// other instructions waits first: settle().  The operands come from LDS reads alone (a vector instruction that wrote one would need two wait states in front).
+// other instructions waits first: settle().  The operands come from LDS reads alone (a vector instruction that wrote one would need two wait states in front).  The compiler does not see
+// these instructions' hazards: tests/test_dense_instructions.py looks for them in the built library, and has to be run whenever this file or the compiler changes.
 __device__ inline void mfma_in_place(T8 a, T8 b, f4v& c) {
 #ifdef DENSE_BF16
 	asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(256) void k_products(GemmArgs x, GemmArgs w, uint32
 // come in three ahead of their use, the next half's B fragments into a second set of registers.  4 wavefronts with 128 x 128 of C each: 2 x 128 fragment rows per 128 x 128
 // products is what LDS can deliver beside the incoming units (96 of the 128 bytes a clock; with 8 wavefronts of 128 x 64 it would be all of them).
 // Bound by the matrix instructions: 8192 x 8192 x 8192 765 us, 1440 TFLOP/s, what a library product reaches here; a unit of a 256 x 256 tile takes 1.46 us, and a tile's outputs some 9 us
-// more that nothing hides (8192 x 4096 of 4096 with gelu, residual and Z 230 us, 1195 TFLOP/s; gated, 4096 x 4096 x 2 of 1024 with both Z 74 us, 930).
+// more that nothing hides (8192 x 4096 of 4096 with gelu, residual and Z 231 to 245 us from card to card, 1120 to 1190 TFLOP/s; gated, 4096 x 4096 x 2 of 1024 with both Z 74 to 77 us, 890 to 930).
 constexpr int AK = 64, A_RING = 4;
 typedef int i4v __attribute__((ext_vector_type(4)));
 template <int EXTENT, bool T_CONTIG, int WAVES> struct Async {
@@ -409,7 +410,7 @@ template <int EXTENT, bool T_CONTIG, int WAVES> struct Async {
 		}
 	}
 	// one of this wavefront's loads: 1024 bytes to LDS from `lds` on; chunks behind the last of the `left` steps are out of range: zero.  (M0 lives inside this block alone: the
-	// compiler sets it anew wherever it needs it)
+	// compiler sets it anew wherever it needs it; the same test finds no other use)
 	__device__ void load(int q, i4v rsrc, uint32_t lds, int left) const {
 		const uint32_t off = T_CONTIG && (int)step >= left ? 0x80000000u : at[q];
 		asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc));
@@ -628,7 +629,7 @@ template <int UNITS> __global__ __launch_bounds__(256, UNITS > 2 ? 1 : 2) void k
 // ---- few rows (a query at a time, a token at a time): bound by reading the weights once.  A wavefront takes 16 outputs (gated: of both projections) and a slice of the sum, weights
 // straight from memory to registers as the matrix instruction's fragments, U loads on the way at a time; the samples (MT x 16 rows, the last one repeated where there are fewer)
 // come out of the caches.  `slices` wavefronts share the sum and add up in LDS, in their order; where there are few outputs blocks share it too (EPI_PARTIAL*).
-// 1 x 2048 -> 2 x 8192 (67 MB) 13.2 us, 5.1 TB/s; 1 x 2048 -> 2048 (8.4 MB) 5.8 us, of which a launch is most.
+// 1 x 2048 -> 2 x 8192 (67 MB) 13.5 us, 5.0 TB/s; 1 x 2048 -> 2048 (8.4 MB) 5.9 us, of which a launch is most.
 template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_few_rows(GemmArgs g, uint32_t slices, uint32_t steps_per_slice) {
 	constexpr bool GATED = GATED_TILE<EPI>;
 	constexpr int P = GATED ? 2 : 1, U = MT == 1 && !GATED ? 8 : 4;
@@ -700,7 +701,9 @@ template <int MT, int EPI, bool ODD> __global__ __launch_bounds__(512) void k_fe
 // ---- narrow layers (up to 256 inputs and outputs) over many samples: bound by reading and writing the samples once.
 // Forward: the weights lie in LDS as fragments (1 KB each, lane by lane), every wavefront takes 16 samples at a time straight from memory into its matrix operands, the next 16 on
 // their way meanwhile, and has all of their outputs in registers.  No barrier after the first one.  Columns are dealt to fragments so that a lane owns 8 consecutive ones.
-// 262144 x 256 of 256 (268 MB) 67 us, 4.0 TB/s; 65521 x 256 and Z of 63 (75 MB) 20.7 us, 3.6 TB/s, of which staging the weights and filling the card take about 5.
+// 262144 x 256 of 256 (268 MB) 77 us, 3.5 TB/s; 65521 x 256 and Z of 63 (75 MB) 20.9 us a call, 21.2 to 22.5 us traced alone, 3.6 TB/s, of which staging the weights and filling the card take
+// about 5.  Variants with 32 fragments of weights are held to 128 registers so that two blocks share a compute unit: 12 of these 22, gated ones or for EXCHANGE or odd lines,
+// spill 1 to 38 registers.
 // ODD: lines that begin between two dwords are read by the dword (65521 x 256 and Z of 63 21.8 -> 20.6 us, 262144 x 64 of 255 68 -> 55 us; a kernel of its own, since the others lose 3 to 10 %).
 // NF: 16-column fragments of weights (gated: gate, then up), KS: steps of 32 inputs.
 template <int NF, int KS, int EPI, bool EXCHANGE, bool ODD> __global__ __launch_bounds__(512, NF * KS <= 32 ? 4 : 2) void k_narrow_forward(GemmArgs g) {
@@ -819,7 +822,8 @@ template <int NF, int KS, int EPI, bool EXCHANGE, bool ODD> __global__ __launch_
 }
 // Backward in one pass: a block takes 32 samples at a time (the next 32 on their way), forms G = dY * act'(Z) and lays it and X into LDS; its 8 wavefronts multiply G with the weights
 // (in LDS too) to dX, and G^T with X into their parts of dW, which stay in registers to the end: one partial sum a block, joined by a second launch.  Every sample's
-// dY, Z, X is read once, dX written once.  262144 samples, 256 x 256 (537 MB): 145 us, 3.7 TB/s, bound by LDS (both products read G from it) as much as by memory.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
+// dY, Z, X is read once, dX written once.  262144 samples, 256 x 256 (537 MB): 142 us, 3.8 TB/s, bound by LDS (both products read G from it) as much as by memory.  NF: 16-column fragments of G (gated: gate, then up), KF: of X.
+// No variant of a linear layer spills; two gated ones do (128 x 128: 18 registers, 256 x 256: 3).
 struct NarrowArgs {
 	uint32_t rows, n, k; int act; const T* x; uint64_t ld_x; const T* w[2]; uint64_t ld_w; const T* pre[2]; uint64_t ld_pre; const T* dy; uint64_t ld_dy; T* dx; uint64_t ld_dx;
 	float* partial; float* bias_partial;
@@ -1006,7 +1010,7 @@ template <int NF, int KF, bool GATED> __global__ __launch_bounds__(512, NF <= 8 
 // G = dY * act'(Z) (gated: [dH * Zu * act'(Zg) | dH * act(Zg)]), lines padded with zeros to multiples of 8 columns, rounded once to the layer's type (the matrix
 // instructions take 16-bit operands; the relative error of a rounding, 2^-12 / 2^-9 on average, is that of the result's own; small sets in two terms), and its column sums (in 32 bits,
 // one line per block of rows, before the rounding; the gradient itself where there is one block).  Memory bound (gated,
-// 8192 x 8192, 671 MB: 116 us, 5.8 TB/s; 90765 x 1928, 1.75 GB: 367 us, 4.8 TB/s).  256 threads: COLS / 8 along a line, the rest on further lines.
+// 8192 x 8192, 671 MB: 117 us, 5.7 TB/s; 90765 x 1928, 1.75 GB: 370 us, 4.7 TB/s).  256 threads: COLS / 8 along a line, the rest on further lines.
 struct GradArgs { uint32_t rows, cols; int act; const T* dy; uint64_t ld_dy; const T* pre[2]; uint64_t ld_pre; T* out; uint64_t ld_out; float* bias_partial; T* dbias[2]; uint32_t rows_per_block; bool two_terms; };
 template <bool GATED, uint32_t COLS> __global__ __launch_bounds__(256) void k_output_grad(GradArgs g) {
 	constexpr uint32_t CX = COLS / 8, RY = 256 / CX;
@@ -1125,7 +1129,7 @@ template <int EPI> __global__ __launch_bounds__(256) void k_join_splits(GemmArgs
 	__shared__ float shared[(EPI == EPI_GATED ? 2 : 1) * 256 * 9];
 	join_any<EPI>(g, groups, blockIdx.x, shared);
 }
-// what is left of a backward pass in one launch: dX's and dW's split sums, the bias's (256 x 256 of 256 pieces, 67 MB: 11.5 us, 5.8 TB/s, out of the last cache)
+// what is left of a backward pass in one launch: dX's and dW's split sums, the bias's (256 x 256 of 256 pieces, 67 MB: 12 us, 5.6 TB/s, out of the last cache)
 __global__ __launch_bounds__(256) void k_finish(GemmArgs x, int groups_x, uint32_t blocks_x, GemmArgs w, int groups_w, uint32_t blocks_w, BiasArgs bias) {
 	__shared__ float shared[256 * 9];
 	uint32_t b = blockIdx.x;
